@@ -202,6 +202,112 @@ tb_status tb_paged_attention_dev_noalloc(void *stream, const float *q_dev, int32
  * word was last cleared.  Allocates nothing. */
 tb_status tb_paged_attention_noalloc_status(void *stream, int32_t clear);
 
+/* ------------------------------------ one step over the paged KV cache -- */
+/* No counterparts in the reference (its runner keeps pages on the host and
+ * steps one token at a time).  Four operators for a caller that runs its own
+ * projections over the pool layout of tb_paged_attention_dev and does not stop
+ * for the host inside a step: page tables and slot maps from lengths, RoPE with
+ * the write to the cache, attention of every sequence's new tokens (one, a
+ * chunk, a whole prompt; mixed in one call), and sampling.
+ *
+ * Shared rules.  Each call enqueues on `stream` (a cudaStream_t, NULL = default
+ * stream) of the device that holds the memory it writes, which need not be the
+ * current one, and returns without waiting; it allocates nothing, keeps nothing
+ * between calls, and may be captured into a graph.  All pointers are device
+ * memory of one device.  A batch's rows are its sequences' new tokens, one
+ * sequence after the other; buffers may hold more rows than the step has, and
+ * what lies behind the last row is left as it was.  Pages and positions that
+ * lie outside the pool or a table are skipped (read as zeros, not written) and
+ * recorded in the device's error word: tb_paged_attention_noalloc_status. */
+
+/* Status of tb_page_tables_build_dev, in info_dev[2]. */
+typedef enum {
+    TB_PAGES_OK = 0,
+    TB_PAGES_BAD_LENGTH = 1,    /* a length is negative or exceeds its table row */
+    TB_PAGES_ROWS_EXCEEDED = 2, /* more new tokens than max_rows */
+    TB_PAGES_EXHAUSTED = 3      /* the free list is too short */
+} tb_pages_status;
+
+/* Page tables and slot maps of a step.  Sequence s holds cached_lens[s] tokens
+ * in its first ceil(cached / 16) table entries and brings new_lens[s] more; the
+ * pages it lacks come off the front of free_pages, sequence by sequence in
+ * logical order, and enter page_table_dev [batch][ptab_stride].  Written:
+ *   row_offsets_dev [batch + 1]  first row of each sequence, then their number
+ *   total_lens_dev [batch]       cached + new
+ *   row_seq_dev, row_pos_dev, row_slot_dev [max_rows]  a row's sequence, its
+ *                                position, and page * 16 + position % 16 (-1
+ *                                where its page is evicted)
+ *   info_dev [4]                 rows, pages taken, tb_pages_status, and the
+ *                                first bad sequence (-1 if none)
+ * A step that does not fit takes no page and has no rows: info_dev holds 0, 0
+ * and the status, row_offsets_dev zeros, total_lens_dev the cached lengths, and
+ * the rest stays as it was.  The pages taken are the caller's to remove from
+ * its list. */
+tb_status tb_page_tables_build_dev(void *stream, const int32_t *cached_lens_dev, const int32_t *new_lens_dev,
+                                   int32_t batch, const int32_t *free_pages_dev, int32_t num_free,
+                                   int32_t *page_table_dev, int32_t ptab_stride, int32_t max_rows,
+                                   int32_t *row_offsets_dev, int32_t *total_lens_dev, int32_t *row_seq_dev,
+                                   int32_t *row_pos_dev, int64_t *row_slot_dev, int32_t *info_dev);
+
+/* The runner's RoPE table: table_host [positions][head_dim / 2][2] = (cos, sin)
+ * by the reference's fp32 formula (ModelRunner.swift:478-486). */
+tb_status tb_rope_table(int32_t positions, int32_t head_dim, float *table_host);
+
+/* RoPE on q and k (pairs of neighbouring dims, ModelRunner.swift:488-489), q to
+ * q_out_dev [rows][num_heads * head_dim], k and v to their slots in the pool
+ * [num_pages][num_layers][2][num_kv_heads][16][head_dim].  q, k, v and q_out
+ * have row strides ld_* in floats, so the columns of one fused projection can
+ * be passed; q_out may be q.  rope_dev [rope_positions][head_dim / 2][2] holds
+ * (cos, sin).  num_rows_dev (one number, or NULL for `rows`) is the step's row
+ * count, such as row_offsets_dev + batch.  A slot of -1 writes no k and v; slots
+ * must differ.  A row whose position has no table row is skipped and recorded.
+ * head_dim is even. */
+tb_status tb_rope_append_paged_dev(void *stream, const float *q_dev, int64_t ld_q, const float *k_dev, int64_t ld_k,
+                                   const float *v_dev, int64_t ld_v, int32_t rows, const int32_t *num_rows_dev,
+                                   const int32_t *row_pos_dev, const int64_t *row_slot_dev, const float *rope_dev,
+                                   int32_t rope_positions, int32_t layer, int32_t num_layers, int32_t num_heads,
+                                   int32_t num_kv_heads, int32_t head_dim, float *kv_pool_dev, int32_t num_pages,
+                                   float *q_out_dev, int64_t ld_out);
+
+/* Attention of each sequence's new tokens over its pages.  Row i of a sequence
+ * with n = row_offsets[s + 1] - row_offsets[s] rows and length total_lens[s]
+ * (its new tokens included, already in the cache) attends over positions
+ * 0 .. total - n + i, scaled by 1 / sqrt(head_dim); rows of evicted pages are
+ * zeros, as in tb_paged_attention_dev, and a row with no position gets zeros.
+ * `rows` is what q_dev and out_dev hold; max_new and max_len bound a sequence's
+ * new tokens and length for the launch's shape only (larger ones stay right).
+ * The workspace is tb_paged_attention_chunk_workspace bytes of device memory,
+ * 16-byte aligned, for this call's use until it has run: calls that may overlap
+ * need their own.  head_dim 16, 32, 64 or 128; num_heads / num_kv_heads <= 128. */
+tb_status tb_paged_attention_chunk_workspace(int32_t rows, int32_t batch, int32_t max_new, int32_t max_len,
+                                             int32_t num_heads, int32_t num_kv_heads, int32_t head_dim,
+                                             int64_t *bytes);
+tb_status tb_paged_attention_chunk_dev(void *stream, const float *q_dev, int64_t ld_q, int32_t rows,
+                                       const int32_t *row_offsets_dev, const int32_t *total_lens_dev, int32_t batch,
+                                       const float *kv_pool_dev, int32_t num_pages, const int32_t *page_table_dev,
+                                       int32_t ptab_stride, int32_t max_new, int32_t max_len, int32_t layer,
+                                       int32_t num_layers, int32_t num_heads, int32_t num_kv_heads,
+                                       int32_t head_dim, float *out_dev, int64_t ld_out, void *workspace_dev,
+                                       int64_t workspace_bytes);
+
+/* One token per row of logits_dev [rows][ld] (vocab_size values each) from
+ * uniform_dev [rows] in [0, 1).  Per row, arrays or NULL for off: temperature
+ * (0 = the maximum, first index; NULL = 1), then the prefixes of the order by
+ * descending value, equal values by index: top_k (<= 0 off), top_p of the mass
+ * that top_k leaves (>= 1 off), and the weights of at least min_p times the
+ * largest (<= 0 off).  The token is the first kept index whose running mass
+ * exceeds uniform times the kept mass.  prob_dev and entropy_dev (NULL or
+ * [rows]) get the token's probability and the entropy (nats) of the kept
+ * distribution, as TokenOutput has them.  NaN counts as -inf; a row with
+ * nothing above -inf gets token -1, probability and entropy 0.  The order of
+ * the steps is not tb_runner_set_sampler's, which follows the reference: there
+ * the temperature comes last, top_p applies only without top_k, and there is
+ * no min_p. */
+tb_status tb_sample_rows_dev(void *stream, const float *logits_dev, int64_t ld, int32_t rows, int32_t vocab_size,
+                             const float *temperature_dev, const int32_t *top_k_dev, const float *top_p_dev,
+                             const float *min_p_dev, const float *uniform_dev, int32_t *token_dev, float *prob_dev,
+                             float *entropy_dev);
+
 /* ---------------------------------------------------------------- model -- */
 typedef enum { TB_ARCH_LLAMA = 0, TB_ARCH_TOY = 1 } tb_architecture;
 typedef enum {

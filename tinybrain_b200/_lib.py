@@ -89,6 +89,14 @@ SIGNATURES = {
     "tb_paged_attention_dev": [_P, _P, _I32, _P, _P, _I32, _P, _I32, _I32, _I32, _I32, _I32, _I32, _P],
     "tb_paged_attention_dev_noalloc": [_P, _P, _I32, _P, _P, _I32, _P, _I32, _I32, _I32, _I32, _I32, _I32, _P],
     "tb_paged_attention_noalloc_status": [_P, _I32],
+    "tb_page_tables_build_dev": [_P, _P, _P, _I32, _P, _I32, _P, _I32, _I32, _P, _P, _P, _P, _P, _P],
+    "tb_rope_table": [_I32, _I32, _P],
+    "tb_rope_append_paged_dev": [_P, _P, _I64, _P, _I64, _P, _I64, _I32, _P, _P, _P, _P, _I32, _I32, _I32, _I32, _I32,
+                                 _I32, _P, _I32, _P, _I64],
+    "tb_paged_attention_chunk_workspace": [_I32, _I32, _I32, _I32, _I32, _I32, _I32, _PI64],
+    "tb_paged_attention_chunk_dev": [_P, _P, _I64, _I32, _P, _P, _I32, _P, _I32, _P, _I32, _I32, _I32, _I32, _I32,
+                                     _I32, _I32, _I32, _P, _I64, _P, _I64],
+    "tb_sample_rows_dev": [_P, _P, _I64, _I32, _I32, _P, _P, _P, _P, _P, _P, _P, _P],
     "tb_model_create": [_P, C.POINTER(ModelConfigC), C.POINTER(_P)],
     "tb_model_free": [_P],
     "tb_tp_unique_id": [_P],

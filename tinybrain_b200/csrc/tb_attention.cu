@@ -23,6 +23,7 @@
 #include "../../include/tinybrain_cuda.h"
 #include "tb_common.cuh"
 #include "tb_kernels.h"
+#include "tb_stream_entry.h"
 
 #include <cuda.h>
 #include <cudaTypedefs.h>
@@ -1559,8 +1560,13 @@ cudaError_t noalloc_setup(int dev) {
     int sms = 0;
     cudaError_t e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
     if (e != cudaSuccess) return e;
+    // the symbol's first use may load the module, which a capturing thread may
+    // only do in relaxed mode
+    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+    cudaThreadExchangeStreamCaptureMode(&mode);
     void* ptr = nullptr;
     e = cudaGetSymbolAddress(&ptr, g_noalloc_err);
+    cudaThreadExchangeStreamCaptureMode(&mode);
     if (e != cudaSuccess) return e;
     g_noalloc_err_dev[dev] = static_cast<int*>(ptr);
     g_noalloc_sms[dev] = sms;
@@ -1587,6 +1593,15 @@ int noalloc_device(tb_status* st) {
     return dev;
 }
 }  // namespace
+
+cudaError_t stream_entry_state(int dev, int* num_sms, int** err) {
+    if (dev < 0 || dev >= kMaxDevices) return cudaErrorInvalidDevice;
+    cudaError_t e = noalloc_setup(dev);
+    if (e != cudaSuccess) return e;
+    *num_sms = g_noalloc_sms[dev];
+    *err = g_noalloc_err_dev[dev];
+    return cudaSuccess;
+}
 
 }  // namespace tb
 
@@ -1645,5 +1660,9 @@ extern "C" tb_status tb_paged_attention_noalloc_status(void* stream, int32_t cle
     if (v == 0) return TB_OK;
     if (v == kDevWaitTimeout)
         return (tb_status)report_error(TB_ERR_DEVICE_TIMEOUT, "a device-side wait exceeded its time limit");
+    if (v == kDevBadPage)
+        return (tb_status)report_error(TB_ERR_STATE, "a page or slot lies outside the KV pool or the page table");
+    if (v == kDevBadPosition)
+        return (tb_status)report_error(TB_ERR_STATE, "a token's position has no row in the RoPE table");
     return (tb_status)report_error(TB_ERR_STATE, "device error code %d", v);
 }

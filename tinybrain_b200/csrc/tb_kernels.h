@@ -3,6 +3,8 @@
 // the public C ABI (include/tinybrain_cuda.h).
 #pragma once
 
+#include <algorithm>
+#include <cmath>
 #include <cstddef>
 #include <cstdint>
 #include <cuda_runtime.h>
@@ -16,6 +18,7 @@ enum DeviceError : int {
     kDevBadPage = 2,          // KV append found no page mapped for a position
     kDevBadToken = 3,         // token id outside [0, vocab)
     kDevBadSmem = 4,          // a shared-memory buffer is not aligned as its layout requires
+    kDevBadPosition = 5,      // a token's position has no row in the RoPE table
 };
 
 // ----------------------------------------------------------------------------
@@ -357,6 +360,15 @@ cudaError_t launch_sample(const SampleParams& p, cudaStream_t stream, bool pdl);
 // -- so the wait runs out and records kDevWaitTimeout in *err.  `word` is one
 // zeroed 64-bit device word.
 cudaError_t launch_wait_probe(int which, const unsigned long long* word, int* err, cudaStream_t stream);
+
+// (cos, sin) of the pair (i, i + 1) of head_dim d at position pos, with the
+// reference's fp32 formula (ModelRunner.swift:478-486).
+inline void rope_angle(int pos, int i, int d, float* cos_sin) {
+    const float theta = powf(10000.0f, -((float)i / (float)d));
+    const float angle = (float)pos * theta;
+    cos_sin[0] = cosf(angle);
+    cos_sin[1] = sinf(angle);
+}
 
 // Record the calling thread's last-error message (tb_last_error); returns status.
 int report_error(int status, const char* fmt, ...);

@@ -1753,12 +1753,7 @@ extern "C" tb_status tb_runner_create(tb_model* m, int32_t max_batch, int32_t ma
     {
         std::vector<float2> tab((size_t)r->max_positions * (d / 2));
         for (int pos = 0; pos < r->max_positions; ++pos)
-            for (int i = 0; i < d; i += 2) {
-                const float freq = (float)i / (float)d;
-                const float theta = powf(10000.0f, -freq);
-                const float angle = (float)pos * theta;
-                tab[(size_t)pos * (d / 2) + i / 2] = make_float2(cosf(angle), sinf(angle));
-            }
+            for (int i = 0; i < d; i += 2) rope_angle(pos, i, d, &tab[(size_t)pos * (d / 2) + i / 2].x);
         TB_CUDA(r->rope.alloc(tab.size() * sizeof(float2)));
         TB_CUDA(cudaMemcpy(r->rope.p, tab.data(), tab.size() * sizeof(float2), cudaMemcpyHostToDevice));
     }

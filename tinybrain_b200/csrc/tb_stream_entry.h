@@ -1,0 +1,72 @@
+// tb_stream_entry.h -- what the stream-level C entries share (the entries that
+// take a cudaStream_t and device pointers, and no context): they run on the
+// device that holds the caller's memory, whatever device is current, and their
+// kernels report into that device's error word
+// (tb_paged_attention_noalloc_status).
+#pragma once
+
+#include "../../include/tinybrain_cuda.h"
+#include "tb_kernels.h"
+
+namespace tb {
+
+// SM count and address of the stream-level entries' error word on device
+// `dev`, which must be current.  Safe inside a stream capture.
+cudaError_t stream_entry_state(int dev, int* num_sms, int** err);
+
+// Makes the device of `mem` (device memory of the caller) current for the
+// lifetime of the object.  `status` is not TB_OK, with the message set, if
+// `mem` is not device memory.
+class StreamEntry {
+public:
+    explicit StreamEntry(const void* mem, const char* what) {
+        cudaPointerAttributes a{};
+        cudaError_t e = cudaPointerGetAttributes(&a, mem);
+        if (e != cudaSuccess) {
+            cudaGetLastError();  // not left behind for the caller's next check
+            status = (tb_status)report_error(e == cudaErrorNoDevice ? TB_ERR_NO_DEVICE : TB_ERR_CUDA, "%s: %s", what,
+                                             cudaGetErrorString(e));
+            return;
+        }
+        if (a.type != cudaMemoryTypeDevice && a.type != cudaMemoryTypeManaged) {
+            status = (tb_status)report_error(TB_ERR_INVALID_ARGUMENT, "%s is not device memory", what);
+            return;
+        }
+        e = cudaGetDevice(&prev_);
+        if (e == cudaSuccess && prev_ != a.device) {
+            e = cudaSetDevice(a.device);
+            if (e == cudaSuccess) switched_ = true;
+        }
+        if (e == cudaSuccess) e = stream_entry_state(a.device, &num_sms, &err);
+        if (e != cudaSuccess)
+            status = (tb_status)report_error(TB_ERR_CUDA, "selecting device %d: %s", a.device, cudaGetErrorString(e));
+    }
+    ~StreamEntry() {
+        if (switched_) cudaSetDevice(prev_);
+    }
+    StreamEntry(const StreamEntry&) = delete;
+    StreamEntry& operator=(const StreamEntry&) = delete;
+
+    tb_status status = TB_OK;
+    int num_sms = 0;
+    int* err = nullptr;
+
+private:
+    int prev_ = 0;
+    bool switched_ = false;
+};
+
+#define TB_ENTRY_CHECK(cond, ...)                                                             \
+    do {                                                                                      \
+        if (!(cond)) return (tb_status)::tb::report_error(TB_ERR_INVALID_ARGUMENT, __VA_ARGS__); \
+    } while (0)
+
+inline tb_status launch_status(cudaError_t e, const char* what) {
+    if (e == cudaSuccess) return TB_OK;
+    return (tb_status)report_error(e == cudaErrorNotSupported ? TB_ERR_UNSUPPORTED : TB_ERR_CUDA, "%s: %s", what,
+                                   cudaGetErrorString(e));
+}
+
+inline bool aligned_to(const void* p, size_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
+
+}  // namespace tb
