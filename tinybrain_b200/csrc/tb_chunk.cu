@@ -120,17 +120,21 @@ struct RowSum {
 // several CTAs hold leaves partial sums in the workspace; chunk_combine_kernel
 // adds them in the order of the CTAs.
 //
-// Roles (14 warps of 16):
+// Roles (16 warps):
 //   producer   one lane per page of a tile: page table, then a bulk copy of the
 //              page's K or V rows of this head into a ring of fp32 pages;
-//   converters (8 warps) one page at a time: the page's largest magnitude gives
+//   converters (6 warps) one page at a time: the page's largest magnitude gives
 //              a power-of-two scale, the halves go to the K and V operand rings;
 //   issuer     one thread: S(i + 1) before P V(i), so the softmax of a tile runs
 //              while the tensor cores do the next S and the last P V;
-//   softmax    (4 warps, a row a thread) base-2 softmax over the tile, P as
-//              halves over S in tensor memory, and the last tile's P V added to
-//              the row's sums in registers, which are rescaled only where the
-//              running maximum grew by more than 2^8.
+//   softmax    two warpgroups, one for even and one for odd tiles, a row a
+//              thread: base-2 softmax over the tile, P as halves over S in tensor
+//              memory, and the P V of the warpgroup's last tile added to the row's
+//              sums in registers, which are rescaled only where its running
+//              maximum grew by more than 2^8.  Each keeps its own maximum and
+//              sums; at a unit's end the odd one hands its to the even one, which
+//              writes the unit.  (One warpgroup took 6300 cycles a tile: one warp
+//              per scheduler waits for each of its own instructions.)
 //
 // With c the row's scale times the page's, a score is c S and a weighted value
 // 2^(c S - M) v = 2^(c S + e - M) (v 2^-e): the page's value exponent e enters
@@ -141,17 +145,23 @@ struct RowSum {
 // rows of the tile), nor have scores beyond 2^20: the unit's rows are then summed
 // in fp32 on the CUDA cores.
 // ---------------------------------------------------------------------------
-constexpr int kSoftmaxWarps = 4, kConvertWarps = 8;
-constexpr int kIssueWarp = kSoftmaxWarps + kConvertWarps, kLoadWarp = kIssueWarp + 1;
-constexpr int kChunkThreads = 512;  // four warpgroups, the last one with two idle warps
-// registers of a thread: 128 at launch, then the softmax warpgroup (a tile's
-// row of S and the row's sums) takes what the other three leave
-constexpr int kLaunchRegs = 128, kSoftmaxRegs = 224, kOtherRegs = 96;
-static_assert(kSoftmaxRegs + 3 * kOtherRegs == 4 * kLaunchRegs, "registers");
+constexpr int kSoftmaxWarps = 8;  // a warpgroup of 4 per tile parity
+// The roles' warps, and the registers of a thread: the launch's, then what the
+// softmax warpgroups (with the rows' sums) take and the others keep.
+template <bool PRE>
+struct Roles {
+    static constexpr int kConvertWarps = PRE ? 0 : 6;
+    static constexpr int kIssueWarp = kSoftmaxWarps + kConvertWarps, kLoadWarp = kIssueWarp + 1;
+    static constexpr int kThreads = PRE ? 384 : 512;
+    static constexpr int kLaunchRegs = PRE ? 168 : 128, kSoftmaxRegs = PRE ? 208 : 192, kOtherRegs = PRE ? 88 : 64;
+    static_assert(2 * 128 * kSoftmaxRegs + (kThreads - 256) * kOtherRegs == kThreads * kLaunchRegs, "registers");
+    static_assert(kLoadWarp < kThreads / 32, "warps");
+};
 constexpr int kChunkCtas = 148;   // most CTAs of a launch (the workspace's size)
 constexpr int kTileRows = 128;
-constexpr int kStages = 2;        // K and V operand tiles each
-constexpr int kScaleRing = 4;     // tiles whose page scales are kept
+constexpr int kScaleRing = 8;     // tiles whose page scales are kept, at least two more than operand tiles
+constexpr int kUnitRing = 4;      // units whose queries' scales are kept: with units of one tile, one
+                                  // softmax warpgroup can be two units ahead of the other
 constexpr uint32_t kWildBits = (127u + 20u) << 23;    // a K or V value of 2^20
 constexpr uint32_t kWildQueryBits = (127u + 40u) << 23;
 constexpr float kPShift = 6.0f;   // P = 2^(6 + score - M), M within 2^8 of the maximum: at most 2^14
@@ -165,8 +175,12 @@ struct Shape {
     static constexpr int PG = NT / kPageTokens;        // its pages
     static constexpr int kPageBytes = kPageTokens * D * 4;
     static constexpr int kHalf = NT * D * 2;           // bytes of one operand half
-    static constexpr int kSlots = D == 128 ? 12 : D == 64 ? 24 : 32;
-    static constexpr size_t kSmem = (size_t)kStages * 4 * kHalf + (size_t)kSlots * kPageBytes;
+    static constexpr int kSlots = D == 128 ? 10 : D == 64 ? 20 : 32;  // fp32 pages, at least a tile's
+    // K and V operand tiles each, and the bytes of shared memory
+    template <bool PRE>
+    static constexpr int kStages = PRE ? 3 : 2;
+    template <bool PRE>
+    static constexpr size_t kSmem = (size_t)kStages<PRE> * 4 * kHalf + (PRE ? 0 : (size_t)kSlots * kPageBytes);
     // tensor memory columns
     static constexpr int kS = 0, kO = 2 * NT, kQ = kO + 2 * D;  // S / P and O twice
     static_assert(kQ + D <= 512, "tensor memory");
@@ -181,10 +195,10 @@ struct Unit {
 
 struct ChunkBars {
     uint64_t slot_full[32], slot_empty[32];
-    uint64_t k_full[kStages], k_empty[kStages], v_full[kStages], v_empty[kStages];
+    uint64_t k_full[3], k_empty[3], v_full[3], v_empty[3];
     uint64_t scales[kScaleRing];
     uint64_t s_full[2], p_full[2];
-    uint64_t pv_done[2], q_full, drained;
+    uint64_t pv_done[2], q_full[kUnitRing], merge_full[4], merge_read[4], drained;
 };
 
 __device__ __forceinline__ int tokens_of_tile(int G) { return kTileRows / G; }
@@ -214,18 +228,51 @@ __device__ __forceinline__ void next_unit(const ChunkParams& p, Unit& u) {
     }
     set_tile<D>(p, u);
 }
+// sum of floor((a i + b) / m) over i < n, for a, b >= 0 and m > 0 (Euclid's
+// algorithm on the lattice points under the line).
+__device__ __forceinline__ long long floor_sum(long long n, long long m, long long a, long long b) {
+    long long sum = 0;
+    while (n > 0) {
+        sum += (a / m) * (n * (n - 1) / 2) + (b / m) * n;
+        a %= m;
+        b %= m;
+        const long long top = a * n + b;
+        if (top < m) break;
+        n = top / m;
+        b = top % m;
+        const long long t = m;
+        m = a;
+        a = t;
+    }
+    return sum;
+}
+// Position tiles of the first `count` row tiles of u's sequence, for one head.
+template <int D>
+__device__ __forceinline__ long long tiles_before(const ChunkParams& p, Unit u, int count) {
+    constexpr int NT = Shape<D>::NT;
+    const int per = tokens_of_tile(p.H / p.Hkv), held = u.len - u.n, all = (u.n + per - 1) / per;
+    if (held >= 0 && u.len <= p.stride * kPageTokens) {
+        // ceil((held + (t + 1) per) / NT) each, but for the last row tile of the sequence
+        const int full = min(count, all - 1);
+        long long sum = floor_sum(full, NT, per, (long long)held + per + NT - 1);
+        if (count == all && all > 0) sum += (u.len + NT - 1) / NT;
+        return sum;
+    }
+    long long sum = 0;  // lengths that do not fit (reported): one by one
+    for (u.tile = 0; u.tile < count; ++u.tile) {
+        set_tile<D>(p, u);
+        sum += u.tiles;
+    }
+    return sum;
+}
 // Tiles of all units of a sequence.
 template <int D>
 __device__ __forceinline__ long long tiles_of_sequence(const ChunkParams& p, int s) {
     Unit u;
     u.s = s;
     set_sequence(p, u);
-    long long sum = 0;
-    for (u.tile = 0; u.tile * tokens_of_tile(p.H / p.Hkv) < u.n; ++u.tile) {
-        set_tile<D>(p, u);
-        sum += u.tiles;
-    }
-    return sum * p.Hkv;
+    const int per = tokens_of_tile(p.H / p.Hkv);
+    return tiles_before<D>(p, u, (u.n + per - 1) / per) * p.Hkv;
 }
 
 // What a CTA leaves for chunk_combine_kernel: its last unit, if that begins
@@ -239,23 +286,53 @@ struct Partial {
     static constexpr size_t kFloats = (size_t)kTileRows * (D + 2);
 };
 
+// Operands made beforehand (chunk_operands_kernel): per sequence, KV head and
+// tile [K high, K low, V high, V low] as the kernel holds them, and the tile's
+// 16 page scales.  tiles = 0: none, the kernel converts pages itself.
+struct Operands {
+    uint8_t* ops;
+    float* scales;
+    int tiles;  // of a sequence
+};
+template <int D>
+__device__ __forceinline__ size_t operand_tile(const ChunkParams& p, const Operands& o, int s, int head, int tile) {
+    return ((size_t)s * p.Hkv + head) * o.tiles + tile;
+}
+
 struct ChunkShared {
     ChunkBars bars;
-    float k_scale[kScaleRing][8], v_exp[kScaleRing][8];
+    alignas(16) float scale[kScaleRing][16];  // of a tile's pages: K factors, then V exponents
     int slot_page[32];
     Unit start;
     int start_tile;
-    long long total, ctas, begin, end;
-    long long scan[kChunkThreads / 32];
+    long long scan[16];
     uint32_t tmem;
+    float q_scale[kUnitRing][kTileRows];              // of the units' rows
+    float merge_m[kTileRows], merge_l[kTileRows];     // the odd warpgroup's
+    float quad_m[kTileRows], quad_l[kTileRows];       // the even warpgroup's warps', in small units
+    float quad_sum[3][32][17];
+    int merge_wild[4], quad_wild[4];
     volatile int dead;  // a wait ran out: nobody waits any more
 };
 
+// Sleeps until the phase completes or a millisecond has passed.  Without the
+// hint the waiting warps poll, and took a third of the issue slots.
+__device__ __forceinline__ bool sleep_on(uint64_t* bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(smem_u32(bar)), "r"(parity), "r"(1000000u)
+        : "memory");
+    return ok != 0;
+}
 __device__ __forceinline__ bool chunk_wait(ChunkShared& sh, uint64_t* bar, uint32_t parity, int* err) {
-    if (mbar_try_wait(bar, parity)) return true;
+    if (sleep_on(bar, parity)) return true;
     const uint64_t t0 = global_timer_ns();
     while (!sh.dead) {
-        if (mbar_try_wait(bar, parity)) return true;
+        if (sleep_on(bar, parity)) return true;
         if (global_timer_ns() - t0 > kWaitLimitNs) {
             record_error(err, kDevWaitTimeout);
             sh.dead = 1;
@@ -268,50 +345,51 @@ __device__ __forceinline__ void warp_wait(ChunkShared& sh, uint64_t* bar, uint32
     __syncwarp();
 }
 
-// Largest magnitude of the warp's values, as bits.
-__device__ __forceinline__ uint32_t warp_max_bits(uint32_t m) { return __reduce_max_sync(0xffffffffu, m); }
+// Exponent of a page's block from the lanes' largest magnitudes (all lanes get it).
+__device__ __forceinline__ uint32_t warp_max_bits(float m) {
+    return __reduce_max_sync(0xffffffffu, __float_as_uint(m) & 0x7fffffffu);
+}
+__device__ __forceinline__ void split4(const float4& a, float s, uint2& hi, uint2& lo) {
+    const float2 ss = make_float2(s, s);
+    const float2 x = __fmul2_rn(make_float2(a.x, a.y), ss), y = __fmul2_rn(make_float2(a.z, a.w), ss);
+    split_pair(x.x, x.y, hi.x, lo.x);
+    split_pair(y.x, y.y, hi.y, lo.y);
+}
 
-// K page -> rows `page * 16 ..` of the K operand.  A lane takes 8 consecutive
-// dims of a token; the dims are staggered over the tokens so that eight lanes'
-// reads (rows of D floats) and writes (16-byte rows of a core matrix) both fall
-// into different banks.
+// K page -> rows `page * 16 ..` of the K operand, four dims of a token at a
+// time.  Lane (r, q) of a step takes dims 4 g .. of token r + 8 (q & 1) with g
+// staggered over the lanes, so that the reads (rows of D floats, 16 bytes a
+// lane) and the writes (8 bytes of a core matrix's 16-byte rows) fall into
+// different banks.  The page is read twice, for its largest magnitude and for
+// its halves, which costs less than the registers to keep it.
 template <int D>
 __device__ __forceinline__ void convert_k(const float* src, int valid, uint8_t* hi, uint8_t* lo, int page,
                                           float* scale_out) {
-    constexpr int C = D / 8, kTasks = C / 2;
-    const int lane = threadIdx.x & 31, l7 = lane & 7, swap = (lane >> 2) & 1;
-    const int r = l7 + 8 * ((lane >> 3) & 1), c0 = l7 + (lane >> 4) * kTasks;
-    float4 x[kTasks][2];
-    uint32_t m = 0;
+    constexpr int C = D / 4, kTasks = C / 2;  // 16-byte columns of a token, steps of a lane
+    const int lane = threadIdx.x & 31, r = lane & 15;
+    const int g0 = (lane & 7) + ((lane >> 3) & 1) + (lane >> 4) * kTasks;
+    const float* row = src + r * D;
+    const bool in = r < valid;
+    float m = 0.0f;
+    if (in) {
 #pragma unroll
-    for (int t = 0; t < kTasks; ++t) {
-        const float* at = src + r * D + ((c0 + t) % C) * 8;
-        float4 a = make_float4(0, 0, 0, 0), b = a;
-        if (r < valid) {
-            a = lds128f(at + 4 * swap);
-            b = lds128f(at + 4 * (swap ^ 1));
+        for (int t = 0; t < kTasks; ++t) {
+            const float4 a = lds128f(row + ((g0 + t) % C) * 4);
+            m = max_abs(max_abs(m, a.x, a.y), a.z, a.w);
         }
-        x[t][0] = swap ? b : a;
-        x[t][1] = swap ? a : b;
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-            m = max(max(m, max(abs_bits(x[t][h].x), abs_bits(x[t][h].y))),
-                    max(abs_bits(x[t][h].z), abs_bits(x[t][h].w)));
     }
-    m = warp_max_bits(m);
-    const int e = block_exponent(m);
+    const uint32_t bits = warp_max_bits(m);
+    const int e = block_exponent(bits);
     const float s = exp2_int(-e);
-    if (lane == 0) *scale_out = m >= kWildBits ? kWildMark : exp2_int(e);
-#pragma unroll
+    if (lane == 0) *scale_out = bits >= kWildBits ? kWildMark : exp2_int(e);
+    const int at0 = (page * 2 + (r >> 3)) * (D * 16) + (r & 7) * 16;
+#pragma unroll 4
     for (int t = 0; t < kTasks; ++t) {
-        uint4 h, l;
-        split_pair(x[t][0].x * s, x[t][0].y * s, h.x, l.x);
-        split_pair(x[t][0].z * s, x[t][0].w * s, h.y, l.y);
-        split_pair(x[t][1].x * s, x[t][1].y * s, h.z, l.z);
-        split_pair(x[t][1].z * s, x[t][1].w * s, h.w, l.w);
-        const int row = page * kPageTokens + r, at = (row >> 3) * (C * 128) + ((c0 + t) % C) * 128 + (row & 7) * 16;
-        *reinterpret_cast<uint4*>(hi + at) = h;
-        *reinterpret_cast<uint4*>(lo + at) = l;
+        const int g = (g0 + t) % C, at = at0 + (g >> 1) * 128 + (g & 1) * 8;
+        uint2 h, l;
+        split4(in ? lds128f(row + g * 4) : make_float4(0, 0, 0, 0), s, h, l);
+        *reinterpret_cast<uint2*>(hi + at) = h;
+        *reinterpret_cast<uint2*>(lo + at) = l;
     }
 }
 
@@ -322,32 +400,36 @@ __device__ __forceinline__ void convert_v(const float* src, int valid, uint8_t* 
                                           float* exp_out) {
     constexpr int NT = Shape<D>::NT, kTasks = D / 16;
     const int lane = threadIdx.x & 31;
-    float x[kTasks][8];
-    uint32_t m = 0;
+    float m = 0.0f;
 #pragma unroll
-    for (int t = 0; t < kTasks; ++t) {
-        const int task = lane + 32 * t, n = task % D, kc = task / D;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            x[t][j] = kc * 8 + j < valid ? src[(kc * 8 + j) * D + n] : 0.0f;
-            m = max(m, abs_bits(x[t][j]));
+    for (int t = 0; t < 2 * kTasks; ++t) {  // any order will do for the maximum
+        const int item = lane + 32 * t;
+        if (item / (D / 4) < valid) {
+            const float4 a = lds128f(src + item * 4);
+            m = max_abs(max_abs(m, a.x, a.y), a.z, a.w);
         }
     }
-    m = warp_max_bits(m);
-    const int e = block_exponent(m);
+    const uint32_t bits = warp_max_bits(m);
+    const int e = block_exponent(bits);
     const float s = exp2_int(-e);
-    if (lane == 0) *exp_out = m >= kWildBits ? kWildMark : (float)e;
-#pragma unroll
+    if (lane == 0) *exp_out = bits >= kWildBits ? kWildMark : (float)e;
+#pragma unroll 2
     for (int t = 0; t < kTasks; ++t) {
         const int task = lane + 32 * t, n = task % D, kc = task / D;
-        uint4 h, l;
-        split_pair(x[t][0] * s, x[t][1] * s, h.x, l.x);
-        split_pair(x[t][2] * s, x[t][3] * s, h.y, l.y);
-        split_pair(x[t][4] * s, x[t][5] * s, h.z, l.z);
-        split_pair(x[t][6] * s, x[t][7] * s, h.w, l.w);
+        float x[8];
+        if (valid == kPageTokens) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) x[j] = src[(kc * 8 + j) * D + n];
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) x[j] = kc * 8 + j < valid ? src[(kc * 8 + j) * D + n] : 0.0f;
+        }
+        uint2 h0, l0, h1, l1;
+        split4(make_float4(x[0], x[1], x[2], x[3]), s, h0, l0);
+        split4(make_float4(x[4], x[5], x[6], x[7]), s, h1, l1);
         const int at = (n >> 3) * (NT * 16) + (page * 2 + kc) * 128 + (n & 7) * 16;
-        *reinterpret_cast<uint4*>(hi + at) = h;
-        *reinterpret_cast<uint4*>(lo + at) = l;
+        *reinterpret_cast<uint4*>(hi + at) = make_uint4(h0.x, h0.y, h1.x, h1.y);
+        *reinterpret_cast<uint4*>(lo + at) = make_uint4(l0.x, l0.y, l1.x, l1.y);
     }
 }
 
@@ -366,13 +448,16 @@ __device__ __forceinline__ void load_row4(const float* q, bool wide, int i, floa
 template <int D>
 __device__ __forceinline__ float load_queries(const ChunkParams& p, const float* q, bool valid, bool wide,
                                               uint32_t tq) {
-    uint32_t m = 0;
-    if (valid)
+    float top = 0.0f;
+    if (valid) {
+#pragma unroll 8
         for (int i = 0; i < D; i += 4) {
             float x[4];
             load_row4<D>(q, wide, i, x);
-            m = max(max(m, max(abs_bits(x[0]), abs_bits(x[1]))), max(abs_bits(x[2]), abs_bits(x[3])));
+            top = max_abs(max_abs(top, x[0], x[1]), x[2], x[3]);
         }
+    }
+    const uint32_t m = __float_as_uint(top) & 0x7fffffffu;
     const int e = m < kWildQueryBits ? block_exponent(m) : 0;
     const float s = exp2_int(-e);
     constexpr int W = D < 32 ? D : 32;
@@ -401,7 +486,7 @@ __device__ __forceinline__ float load_queries(const ChunkParams& p, const float*
 template <int D>
 __device__ __noinline__ void rows_without_operands(const ChunkParams& p, const Unit& u, int t0, int t1, float* partial) {
     const int G = p.H / p.Hkv, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    for (int r = warp * 32; r < warp * 32 + 32; ++r) {
+    for (int r = warp * 32; r < warp * 32 + 32; ++r) {  // the even warpgroup's warps 0 to 3
         const int token = u.tile * tokens_of_tile(G) + r / G;
         if (r >= tokens_of_tile(G) * G || token >= u.n) break;
         const int h = u.head * G + r % G;
@@ -424,30 +509,41 @@ __device__ __noinline__ void rows_without_operands(const ChunkParams& p, const U
     }
 }
 
-template <int D>
-__global__ void __launch_bounds__(kChunkThreads, 1) chunk_tiles_kernel(ChunkParams p, float* partials,
-                                                                        ChunkSplit* splits, bool wide_q, bool wide_out) {
+template <int D, bool PRE>
+__global__ void __launch_bounds__(Roles<PRE>::kThreads, 1)
+    chunk_tiles_kernel(ChunkParams p, float* partials, ChunkSplit* splits, Operands pre, bool wide_q, bool wide_out) {
     using S = Shape<D>;
-    constexpr int NT = S::NT, PG = S::PG;
+    using R = Roles<PRE>;
+    constexpr int NT = S::NT, PG = S::PG, kStages = S::template kStages<PRE>, kChunkThreads = R::kThreads;
+    constexpr int kIssueWarp = R::kIssueWarp, kLoadWarp = R::kLoadWarp, kConvertWarps = R::kConvertWarps;
+    constexpr int kSoftmaxRegs = R::kSoftmaxRegs, kOtherRegs = R::kOtherRegs;
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ ChunkShared sh;
-    static_assert(S::kSmem + sizeof(ChunkShared) <= 227 * 1024, "shared memory");
+    static_assert(S::template kSmem<PRE> + sizeof(ChunkShared) <= 227 * 1024, "shared memory");
+    static_assert(kScaleRing >= kStages + 2 && S::kSlots >= 2 * PG && S::kSlots > kConvertWarps, "rings");
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     uint8_t* k_ops = smem;                                // [stage][hi, lo]
     uint8_t* v_ops = smem + kStages * 2 * S::kHalf;
     uint8_t* pages = smem + kStages * 4 * S::kHalf;
     ChunkBars& b = sh.bars;
 
-    // the CTA's share: tiles [total c / C, total (c + 1) / C) of all units' tiles
-    long long sum = 0;
-    for (int s = tid; s < p.batch; s += kChunkThreads) {
-        sum += tiles_of_sequence<D>(p, s);
+    // the CTA's share: tiles [total c / C, total (c + 1) / C) of all units'
+    // tiles; a thread counts those of a run of sequences
+    const int run = (p.batch + kChunkThreads - 1) / kChunkThreads;
+    const int s0 = min(tid * run, p.batch), s1 = min(s0 + run, p.batch);
+    long long mine = 0;
+    for (int s = s0; s < s1; ++s) {
+        mine += tiles_of_sequence<D>(p, s);
         int first, n;
         rows_of(p, s, first, n);
         if (n && p.total_lens[s] > p.stride * kPageTokens) record_error(p.err, kDevBadPage);
     }
-    for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    if (lane == 0) sh.scan[warp] = sum;
+    long long incl = mine;
+    for (int o = 1; o < 32; o <<= 1) {
+        const long long t = __shfl_up_sync(0xffffffffu, incl, o);
+        if (lane >= o) incl += t;
+    }
+    if (lane == 31) sh.scan[warp] = incl;
     if (tid == 0) {
         sh.dead = 0;
         for (int i = 0; i < S::kSlots; ++i) {
@@ -455,70 +551,55 @@ __global__ void __launch_bounds__(kChunkThreads, 1) chunk_tiles_kernel(ChunkPara
             mbar_init(b.slot_empty + i, 1);
         }
         for (int i = 0; i < kStages; ++i) {
-            mbar_init(b.k_full + i, PG);
-            mbar_init(b.v_full + i, PG);
+            mbar_init(b.k_full + i, PRE ? 1 : PG);
+            mbar_init(b.v_full + i, PRE ? 1 : PG);
             mbar_init(b.k_empty + i, 1);
             mbar_init(b.v_empty + i, 1);
         }
-        for (int i = 0; i < kScaleRing; ++i) mbar_init(b.scales + i, 2 * PG);
+        for (int i = 0; i < kScaleRing; ++i) mbar_init(b.scales + i, PRE ? 1 : 2 * PG);
         for (int i = 0; i < 2; ++i) {
             mbar_init(b.s_full + i, 1);
-            mbar_init(b.p_full + i, kSoftmaxWarps);
+            mbar_init(b.p_full + i, 4);
             mbar_init(b.pv_done + i, 1);
         }
+        for (int i = 0; i < kUnitRing; ++i) mbar_init(b.q_full + i, 4);
+        for (int i = 0; i < 4; ++i) {
+            mbar_init(b.merge_full + i, 1);
+            mbar_init(b.merge_read + i, 1);
+        }
         mbar_init(&b.drained, 1);
-        mbar_init(&b.q_full, kSoftmaxWarps);
         fence_barrier_init();
         fence_proxy_async_shared();
     }
     __syncthreads();
-    if (tid == 0) {
-        long long total = 0;
-        for (int w = 0; w < kChunkThreads / 32; ++w) total += sh.scan[w];
-        const long long c = blockIdx.x, ctas = min((long long)gridDim.x, total);  // every share has a tile
-        sh.total = total;
-        sh.ctas = ctas;
-        sh.begin = c < ctas ? total * c / ctas : 0;
-        sh.end = c < ctas ? total * (c + 1) / ctas : 0;
-        sh.start.s = -1;
+    long long before = incl - mine, total = 0;
+    for (int w = 0; w < kChunkThreads / 32; ++w) {
+        if (w < warp) before += sh.scan[w];
+        total += sh.scan[w];
     }
-    __syncthreads();
-    const long long begin = sh.begin, count = sh.end - begin;
-    if (count > 0) {
-        long long carry = 0;
-        for (int base = 0; base < p.batch; base += kChunkThreads) {
-            const int s = base + tid;
-            const long long mine = s < p.batch ? tiles_of_sequence<D>(p, s) : 0;
-            long long incl = mine;
-            for (int o = 1; o < 32; o <<= 1) {
-                const long long t = __shfl_up_sync(0xffffffffu, incl, o);
-                if (lane >= o) incl += t;
-            }
-            __syncthreads();
-            if (lane == 31) sh.scan[warp] = incl;
-            __syncthreads();
-            long long before = carry + incl - mine;
-            for (int w = 0; w < kChunkThreads / 32; ++w) {
-                if (w < warp) before += sh.scan[w];
-                carry += sh.scan[w];
-            }
-            if (mine > 0 && before <= begin && begin < before + mine) {
-                Unit u;
-                u.s = s;
-                u.head = 0;
-                set_sequence(p, u);
-                long long at = begin - before;
-                for (u.tile = 0;; ++u.tile) {
-                    set_tile<D>(p, u);
-                    if (at < (long long)u.tiles * p.Hkv) break;
-                    at -= (long long)u.tiles * p.Hkv;
-                }
-                u.head = (int)(at / u.tiles);
-                sh.start = u;
-                sh.start_tile = (int)(at % u.tiles);
-            }
-            if (carry > begin) break;
+    const long long ctas = min((long long)gridDim.x, total), cta = blockIdx.x;  // every share has a tile
+    const long long begin = cta < ctas ? total * cta / ctas : 0, end = cta < ctas ? total * (cta + 1) / ctas : 0;
+    const long long count = end - begin;
+    if (count > 0 && mine > 0 && before <= begin && begin < before + mine) {
+        Unit u;
+        long long at = begin - before;
+        for (u.s = s0;; ++u.s) {
+            const long long here = tiles_of_sequence<D>(p, u.s);
+            if (at < here) break;
+            at -= here;
         }
+        set_sequence(p, u);
+        int lo = 0, hi = (u.n + tokens_of_tile(p.H / p.Hkv) - 1) / tokens_of_tile(p.H / p.Hkv);
+        while (hi - lo > 1) {  // the last row tile that begins at or before `at`
+            const int mid = (lo + hi) / 2;
+            if (tiles_before<D>(p, u, mid) * p.Hkv <= at) lo = mid; else hi = mid;
+        }
+        at -= tiles_before<D>(p, u, lo) * p.Hkv;
+        u.tile = lo;
+        set_tile<D>(p, u);
+        u.head = (int)(at / u.tiles);
+        sh.start = u;
+        sh.start_tile = (int)(at % u.tiles);
     }
     if (warp == kIssueWarp) tmem_alloc(&sh.tmem, 512);
     tc_fence_before();
@@ -533,16 +614,44 @@ __global__ void __launch_bounds__(kChunkThreads, 1) chunk_tiles_kernel(ChunkPara
     if (count > 0 && warp == kLoadWarp) {
         // ---- producer ----
         set_registers_down<kOtherRegs>();
-        long long job0 = 0;
+        if constexpr (PRE) {
+            int i = 0;
+            if (lane == 0) {
+                for (long long left = count; left > 0 && !sh.dead; at = 0) {
+                    const int take = (int)min((long long)(u.tiles - at), left);
+                    for (int j = at; j < at + take; ++j, ++i) {
+                        const int st = i % kStages, ring = i % kScaleRing;
+                        const bool made = u.len <= pre.tiles * NT;  // a longer one goes without operands
+                        const size_t t = made ? operand_tile<D>(p, pre, u.s, u.head, j) : 0;
+                        const uint8_t* src = pre.ops + t * (4 * S::kHalf);
+                        if (!chunk_wait(sh, b.k_empty + st, (uint32_t)(i / kStages & 1) ^ 1, p.err)) break;
+                        mbar_arrive_expect_tx(b.scales + ring, 64);
+                        bulk_g2s(sh.scale[ring], pre.scales + t * 16, 64, b.scales + ring);
+                        mbar_arrive_expect_tx(b.k_full + st, 2 * S::kHalf);
+                        bulk_g2s(k_ops + st * 2 * S::kHalf, src, 2 * S::kHalf, b.k_full + st);
+                        if (!chunk_wait(sh, b.v_empty + st, (uint32_t)(i / kStages & 1) ^ 1, p.err)) break;
+                        mbar_arrive_expect_tx(b.v_full + st, 2 * S::kHalf);
+                        bulk_g2s(v_ops + st * 2 * S::kHalf, src + 2 * S::kHalf, 2 * S::kHalf, b.v_full + st);
+                    }
+                    left -= take;
+                    if (left > 0) next_unit<D>(p, u);
+                }
+                if (sh.dead) {  // copies still in flight must land before the CTA ends: a second is ample
+                    const uint64_t t0 = global_timer_ns();
+                    while (global_timer_ns() - t0 < kWaitLimitNs / 2) {
+                    }
+                }
+            }
+            __syncwarp();
+        } else {
+        int jobs = 0, slot = lane, fill = 0;  // the lane's page slot, and how often it was filled before
         for (long long left = count; left > 0 && !sh.dead; at = 0) {
             const int take = (int)min((long long)(u.tiles - at), left);
-            for (int j = at; j < at + take; ++j, job0 += 2 * PG) {
+            for (int j = at; j < at + take; ++j, jobs += 2 * PG) {
                 if (lane < 2 * PG) {
                     const int kv = lane / PG, pos = j * NT + (lane % PG) * kPageTokens;
                     const int page = pos < u.limit ? page_at(p, u.s, pos) : -1;
-                    const long long job = job0 + lane;
-                    const int slot = (int)(job % S::kSlots);
-                    if (chunk_wait(sh, b.slot_empty + slot, (uint32_t)(job / S::kSlots & 1) ^ 1, p.err)) {
+                    if (chunk_wait(sh, b.slot_empty + slot, (uint32_t)(fill & 1) ^ 1, p.err)) {
                         sh.slot_page[slot] = page;
                         if (page >= 0) {
                             mbar_arrive_expect_tx(b.slot_full + slot, S::kPageBytes);
@@ -551,6 +660,11 @@ __global__ void __launch_bounds__(kChunkThreads, 1) chunk_tiles_kernel(ChunkPara
                         } else {
                             mbar_arrive(b.slot_full + slot);
                         }
+                    }
+                    slot += 2 * PG;
+                    if (slot >= S::kSlots) {
+                        slot -= S::kSlots;
+                        ++fill;
                     }
                 }
                 __syncwarp();
@@ -561,22 +675,22 @@ __global__ void __launch_bounds__(kChunkThreads, 1) chunk_tiles_kernel(ChunkPara
         if (sh.dead) {  // copies still in flight must land before the CTA ends
             const uint64_t t0 = global_timer_ns();
             for (int s = lane; s < S::kSlots; s += 32) {
-                // the slot's last fill, counted in jobs
-                const long long fills = (job0 - 1 - s >= 0) ? (job0 - 1 - s) / S::kSlots + 1 : 0;
+                const int fills = jobs > s ? (jobs - 1 - s) / S::kSlots + 1 : 0;
                 while (fills && !mbar_try_wait(b.slot_full + s, (uint32_t)(fills - 1) & 1) &&
                        global_timer_ns() - t0 < kWaitLimitNs) {
                 }
             }
         }
+        }
     } else if (count > 0 && warp == kIssueWarp) {
         // ---- issuer ----
         set_registers_down<kOtherRegs>();
-        if (lane == 0) {
+        if (elect_one()) {
             const uint32_t k0 = smem_u32(k_ops), v0 = smem_u32(v_ops);
-            long long i = 0, unit = 0;
-            const auto issue_s = [&](long long item, bool first, long long un) {
-                const int st = (int)(item % kStages);
-                if (first) chunk_wait(sh, &b.q_full, (uint32_t)(un & 1), p.err);
+            int i = 0, unit = 0;
+            const auto issue_s = [&](int item, bool first, int un) {
+                const int st = item % kStages;
+                if (first) chunk_wait(sh, b.q_full + un % kUnitRing, (uint32_t)(un / kUnitRing & 1), p.err);
                 chunk_wait(sh, b.k_full + st, (uint32_t)(item / kStages & 1), p.err);
                 tc_fence_after();
                 const uint32_t kb = k0 + st * 2 * S::kHalf;
@@ -590,7 +704,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) chunk_tiles_kernel(ChunkPara
                 issue_s(i, true, unit);
                 for (int j = 0; j < take; ++j, ++i) {
                     if (j + 1 < take) issue_s(i + 1, false, unit);
-                    const int st = (int)(i % kStages);
+                    const int st = i % kStages;
                     chunk_wait(sh, b.v_full + st, (uint32_t)(i / kStages & 1), p.err);
                     chunk_wait(sh, b.p_full + (i & 1), (uint32_t)(i / 2 & 1), p.err);
                     tc_fence_after();
@@ -613,30 +727,28 @@ __global__ void __launch_bounds__(kChunkThreads, 1) chunk_tiles_kernel(ChunkPara
             }
         }
         __syncwarp();
-    } else if (count > 0 && warp >= kSoftmaxWarps && warp < kIssueWarp) {
-        // ---- converters ----
+    } else if (!PRE && count > 0 && warp >= kSoftmaxWarps && warp < kIssueWarp) {
+        // ---- converters: the CTA's pages in order, each warp every sixth ----
         set_registers_down<kOtherRegs>();
-        const int cw = warp - kSoftmaxWarps;
-        long long i = 0;
+        int i = 0, jj = warp - kSoftmaxWarps;
+        int slot = jj, fill = 0;  // page slot, and how often it was filled before
         for (long long left = count; left > 0; at = 0) {
             const int take = (int)min((long long)(u.tiles - at), left);
-            for (int j = at; j < at + take; ++j, ++i) {
-                const int st = (int)(i % kStages), ring = (int)(i % kScaleRing);
-                for (int jj = cw; jj < 2 * PG; jj += kConvertWarps) {
+            for (int j = at; j < at + take; ++j, ++i, jj -= 2 * PG) {
+                const int st = i % kStages, ring = i % kScaleRing;
+                for (; jj < 2 * PG; jj += PRE ? 2 * PG : kConvertWarps) {
                     const bool is_v = jj >= PG;
                     const int page = jj % PG;
-                    const long long job = i * (2 * PG) + jj;
-                    const int slot = (int)(job % S::kSlots);
-                    warp_wait(sh, b.slot_full + slot, (uint32_t)(job / S::kSlots & 1), p.err);
+                    warp_wait(sh, b.slot_full + slot, (uint32_t)fill & 1, p.err);
                     const int left_here = u.limit - (j * NT + page * kPageTokens);
                     const int valid = sh.slot_page[slot] < 0 ? 0 : max(0, min(left_here, kPageTokens));
                     warp_wait(sh, (is_v ? b.v_empty : b.k_empty) + st, (uint32_t)(i / kStages & 1) ^ 1, p.err);
                     const float* src = reinterpret_cast<const float*>(pages + slot * S::kPageBytes);
                     uint8_t* op = (is_v ? v_ops : k_ops) + st * 2 * S::kHalf;
                     if (is_v)
-                        convert_v<D>(src, valid, op, op + S::kHalf, page, &sh.v_exp[ring][page]);
+                        convert_v<D>(src, valid, op, op + S::kHalf, page, &sh.scale[ring][8 + page]);
                     else
-                        convert_k<D>(src, valid, op, op + S::kHalf, page, &sh.k_scale[ring][page]);
+                        convert_k<D>(src, valid, op, op + S::kHalf, page, &sh.scale[ring][page]);
                     fence_proxy_async_shared();
                     __syncwarp();
                     if (lane == 0) {
@@ -644,193 +756,333 @@ __global__ void __launch_bounds__(kChunkThreads, 1) chunk_tiles_kernel(ChunkPara
                         mbar_arrive(b.slot_empty + slot);
                         mbar_arrive(b.scales + ring);
                     }
+                    slot += kConvertWarps;
+                    if (slot >= S::kSlots) {
+                        slot -= S::kSlots;
+                        ++fill;
+                    }
                 }
             }
             left -= take;
             if (left > 0) next_unit<D>(p, u);
         }
     } else if (count > 0 && warp < kSoftmaxWarps) {
-        // ---- softmax ----
+        // ---- softmax: warpgroup `odd` takes the tiles of its parity ----
         set_registers_up<kSoftmaxRegs>();
-        const uint32_t lanes = (uint32_t)(warp * 32) << 16;
+        const int odd = warp >> 2, quad = warp & 3;
+        const uint32_t lanes = (uint32_t)(quad * 32) << 16;
         const int G = p.H / p.Hkv, per = tokens_of_tile(G);
-        const int row = tid, tok = row / G, sub = row % G;
-        long long i = 0;
+        const uint32_t ts = tmem + S::kS + (uint32_t)odd * NT + lanes, to = tmem + S::kO + (uint32_t)odd * D + lanes;
         ChunkSplit split{0, 0, 0, -1};
-        const auto queries = [&](const Unit& w) {
-            const int token = w.tile * per + tok;
+        // A unit of at most 32 rows would leave three of a warpgroup's four warps
+        // idle: its rows stand in all four lane groups, each of which takes a
+        // quarter of a tile's positions (P is zero elsewhere).
+        const auto small_unit = [&](const Unit& w) { return min(per, w.n - w.tile * per) * G <= 32; };
+        const auto queries = [&](const Unit& w, int unit) {
+            const int row = small_unit(w) ? lane : quad * 32 + lane;
+            const int token = w.tile * per + row / G;
             const bool valid = row < per * G && token < w.n;
-            float f = 1.0f;
             if (__any_sync(0xffffffffu, valid)) {
-                f = load_queries<D>(p, p.q + (w.first + (valid ? token : 0)) * p.ld_q + (size_t)(w.head * G + sub) * D, valid,
-                                    wide_q, tmem + S::kQ + lanes);
+                sh.q_scale[unit % kUnitRing][quad * 32 + lane] = load_queries<D>(
+                    p, p.q + (w.first + (valid ? token : 0)) * p.ld_q + (size_t)(w.head * G + row % G) * D, valid,
+                    wide_q, tmem + S::kQ + lanes);
                 tmem_st_wait();
             }
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive(&b.q_full);
-            return f;
+            if (lane == 0) mbar_arrive(b.q_full + unit % kUnitRing);
         };
-        float c = queries(u);
-        for (long long left = count; left > 0;) {
+        int i = 0, unit = 0, merges = 0;
+        if (!odd) queries(u, 0);
+        for (long long left = count; left > 0; ++unit) {
             const int take = (int)min((long long)(u.tiles - at), left);
-            const int token = u.tile * per + tok;
+            const bool small = small_unit(u);
+            const int row = small ? lane : quad * 32 + lane, sub = row % G;
+            const int token = u.tile * per + row / G;
             const bool valid = row < per * G && token < u.n;
+            // the warp's positions of a tile: [from_col, to_col)
+            const int from_col = small ? quad * (NT / 4) : 0, to_col = small ? from_col + NT / 4 : NT;
             const bool busy = __any_sync(0xffffffffu, valid);
             const int sees = min(u.len - u.n + token + 1, u.limit);  // the row's own limit, may be <= 0
             const int first_sees = __shfl_sync(0xffffffffu, sees, 0);  // tokens ascend with the lanes
-            bool wild = __any_sync(0xffffffffu, valid && c < 0.0f);
-            bool huge = false;
+            warp_wait(sh, b.q_full + unit % kUnitRing, (uint32_t)(unit / kUnitRing & 1), p.err);
+            const float c = busy ? sh.q_scale[unit % kUnitRing][quad * 32 + lane] : 1.0f;
+            bool wild = __any_sync(0xffffffffu, valid && c < 0.0f) || (PRE && u.len > pre.tiles * NT), huge = false;
             float M = -INFINITY, l = 0.0f;
             float2 acc[D / 2];
 #pragma unroll
             for (int x = 0; x < D / 2; ++x) acc[x] = make_float2(0.0f, 0.0f);
-            // adds P V of tile `item`, whose scale the sums still have
-            const auto collect = [&](long long item) {
-                warp_wait(sh, b.pv_done + (item & 1), (uint32_t)(item / 2 & 1), p.err);
+            // adds P V of the warpgroup's tile `item`, whose scale the sums still have
+            const auto collect = [&](int item) {
+                warp_wait(sh, b.pv_done + odd, (uint32_t)(item / 2 & 1), p.err);
                 tc_fence_after();
-                const uint32_t to = tmem + S::kO + (uint32_t)(item & 1) * D + lanes;
-                if constexpr (D == 16) {
+#pragma unroll
+                for (int o = 0; o < D; o += 16) {
                     int v[16];
-                    tmem_ld16(to, v);
+                    tmem_ld16(to + o, v);
                     tmem_ld_wait();
 #pragma unroll
                     for (int x = 0; x < 8; ++x)
-                        acc[x] = __fadd2_rn(acc[x], make_float2(__int_as_float(v[2 * x]), __int_as_float(v[2 * x + 1])));
-                } else {
-#pragma unroll
-                    for (int o = 0; o < D; o += 32) {
-                        int v[32];
-                        tmem_ld32(to + o, v);
-                        tmem_ld_wait();
-#pragma unroll
-                        for (int x = 0; x < 16; ++x)
-                            acc[o / 2 + x] = __fadd2_rn(acc[o / 2 + x], make_float2(__int_as_float(v[2 * x]),
-                                                                                     __int_as_float(v[2 * x + 1])));
-                    }
+                        acc[o / 2 + x] = __fadd2_rn(
+                            acc[o / 2 + x], make_float2(__int_as_float(v[2 * x]), __int_as_float(v[2 * x + 1])));
                 }
             };
-            for (int j = at; j < at + take; ++j, ++i) {
-                const uint32_t ts = tmem + S::kS + (uint32_t)(i & 1) * NT + lanes;
-                const int ring = (int)(i % kScaleRing);
+            const int i0 = i, first = (i0 & 1) == odd ? i0 : i0 + 1;  // this warpgroup's first tile of the unit
+            for (i = first; i < i0 + take; i += 2) {
+                const int j = at + (i - i0), ring = i % kScaleRing;
                 warp_wait(sh, b.scales + ring, (uint32_t)(i / kScaleRing & 1), p.err);
-                warp_wait(sh, b.s_full + (i & 1), (uint32_t)(i / 2 & 1), p.err);
+                warp_wait(sh, b.s_full + odd, (uint32_t)(i / 2 & 1), p.err);
                 tc_fence_after();
-                float r = 1.0f;
                 if (busy) {
-                    const float *ks = sh.k_scale[ring], *ve = sh.v_exp[ring];
-                    int v[NT / 32][32];
-#pragma unroll
-                    for (int g = 0; g < NT / 32; ++g) tmem_ld32(ts + 32 * g, v[g]);
-                    tmem_ld_wait();
-                    if (first_sees < (j + 1) * NT) {  // some row does not see all of the tile
-                        const int room = sees - j * NT;
-#pragma unroll
-                        for (int x = 0; x < NT; ++x)
-                            if (x >= room) v[x / 32][x % 32] = __float_as_int(-INFINITY);
-                    }
+                    const float *ks = sh.scale[ring], *ve = ks + 8;
+                    const int room = sees - j * NT;                 // columns below it are seen
+                    const bool masked = first_sees < (j + 1) * NT;  // some row does not see all of the tile
                     // the row's maximum of score + value exponent: per page the largest S decides
                     float top = -INFINITY;
+#pragma unroll 1
+                    for (int g = from_col / 32; g * 32 < to_col; ++g) {
+                        int v[32];
+                        tmem_ld32(ts + 32 * g, v);
+                        tmem_ld_wait();
+                        if (masked) {
 #pragma unroll
-                    for (int g = 0; g < PG; ++g) {
-                        float m0 = __int_as_float(v[g / 2][g % 2 * 16]), m1 = __int_as_float(v[g / 2][g % 2 * 16 + 1]);
-#pragma unroll
-                        for (int x = 2; x < 16; x += 2) {
-                            m0 = fmaxf(m0, __int_as_float(v[g / 2][g % 2 * 16 + x]));
-                            m1 = fmaxf(m1, __int_as_float(v[g / 2][g % 2 * 16 + x + 1]));
+                            for (int x = 0; x < 32; ++x)
+                                if (32 * g + x >= room) v[x] = __float_as_int(-INFINITY);
                         }
-                        wild |= ks[g] == kWildMark || ve[g] == kWildMark;
-                        top = fmaxf(top, fmaf(fmaxf(m0, m1), c * ks[g], ve[g]));
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            float m0 = __int_as_float(v[16 * h]), m1 = __int_as_float(v[16 * h + 1]);
+#pragma unroll
+                            for (int x = 16 * h + 2; x < 16 * h + 14; x += 4) {
+                                m0 = max3(m0, __int_as_float(v[x]), __int_as_float(v[x + 1]));
+                                m1 = max3(m1, __int_as_float(v[x + 2]), __int_as_float(v[x + 3]));
+                            }
+                            m0 = max3(m0, __int_as_float(v[16 * h + 14]), __int_as_float(v[16 * h + 15]));
+                            const int page = 2 * g + h;
+                            if (NT / 4 >= 32 || (page * 16 >= from_col && page * 16 < to_col)) {
+                                wild |= ks[page] == kWildMark || ve[page] == kWildMark;
+                                top = fmaxf(top, fmaf(fmaxf(m0, m1), c * ks[page], ve[page]));
+                            }
+                        }
                     }
                     huge |= valid && top > -INFINITY && fabsf(top) > kHuge;
+                    float r = 1.0f;
                     if (top > M + kLazy || (M == -INFINITY && top > -INFINITY)) {
                         r = M == -INFINITY ? 0.0f : ex2(M - top);
                         M = top;
                         l *= r;
                     }
                     const float shift = kPShift - (M == -INFINITY ? 0.0f : M);
-#pragma unroll
+#pragma unroll 1
                     for (int g = 0; g < NT / 32; ++g) {
                         uint32_t hi[16], lo[16];
+                        if (32 * g + 32 <= from_col || 32 * g >= to_col) {  // another warp's positions
 #pragma unroll
-                        for (int h = 0; h < 2; ++h) {
-                            const float e = ve[2 * g + h];
-                            const float2 kk = make_float2(c * ks[2 * g + h], c * ks[2 * g + h]);
-                            const float2 bb = make_float2(e + shift, e + shift);
-                            float2 sum = make_float2(0.0f, 0.0f);
+                            for (int x = 0; x < 16; ++x) hi[x] = lo[x] = 0;
+                        } else {
+                            int v[32];
+                            tmem_ld32(ts + 32 * g, v);
+                            const float e0 = ve[2 * g], e1 = ve[2 * g + 1];
+                            const float k0 = c * ks[2 * g], k1 = c * ks[2 * g + 1];
+                            // where a warp's quarter is one page, the other page of the 32 gets no weight
+                            const float off0 = NT / 4 >= 32 || 32 * g >= from_col ? shift : -INFINITY;
+                            const float off1 = NT / 4 >= 32 || 32 * g + 16 < to_col ? shift : -INFINITY;
+                            tmem_ld_wait();
+                            if (masked) {
 #pragma unroll
-                            for (int x = 16 * h; x < 16 * h + 16; x += 2) {
-                                const float2 t = __ffma2_rn(
-                                    make_float2(__int_as_float(v[g][x]), __int_as_float(v[g][x + 1])), kk, bb);
-                                const float2 w = make_float2(ex2(t.x), ex2(t.y));
-                                sum = __fadd2_rn(sum, w);
-                                split_pair(w.x, w.y, hi[x / 2], lo[x / 2]);
+                                for (int x = 0; x < 32; ++x)
+                                    if (32 * g + x >= room) v[x] = __float_as_int(-INFINITY);
                             }
-                            l = fmaf(sum.x + sum.y, ex2(-e), l);
+#pragma unroll
+                            for (int h = 0; h < 2; ++h) {
+                                const float2 kk = h ? make_float2(k1, k1) : make_float2(k0, k0);
+                                const float2 bb = h ? make_float2(e1 + off1, e1 + off1)
+                                                    : make_float2(e0 + off0, e0 + off0);
+                                float2 sum = make_float2(0.0f, 0.0f);
+#pragma unroll
+                                for (int x = 16 * h; x < 16 * h + 16; x += 2) {
+                                    const float2 t = __ffma2_rn(
+                                        make_float2(__int_as_float(v[x]), __int_as_float(v[x + 1])), kk, bb);
+                                    const float2 w = make_float2(ex2(t.x), ex2(t.y));
+                                    sum = __fadd2_rn(sum, w);
+                                    split_pair(w.x, w.y, hi[x / 2], lo[x / 2]);
+                                }
+                                l = fmaf(sum.x + sum.y, ex2(h ? -e1 : -e0), l);
+                            }
                         }
                         tmem_st16(ts + 32 * g, hi);
                         tmem_st16(ts + 32 * g + 16, lo);
                     }
                     tmem_st_wait();
-                }
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(b.p_full + (i & 1));
-                if (busy) {
-                    if (j > at) collect(i - 1);
+                    if (i > first) collect(i - 2);
                     if (__any_sync(0xffffffffu, r != 1.0f)) {
 #pragma unroll
                         for (int x = 0; x < D / 2; ++x) acc[x] = __fmul2_rn(acc[x], make_float2(r, r));
                     }
                 }
+                // the odd sums of the last unit still stand where P V of this tile goes
+                if (odd && i == first && merges > 0)
+                    warp_wait(sh, b.merge_read + quad, (uint32_t)(merges - 1) & 1, p.err);
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(b.p_full + odd);
             }
+            i = i0 + take;
             const Unit done = u;
             const int from = at;
             left -= take;
-            if (left > 0) {  // the next unit's queries, while the last products run
+            at = 0;
+            if (left > 0) {
                 next_unit<D>(p, u);
-                c = queries(u);
+                // the warpgroup of the unit's last tile knows that its queries are read
+                if (((i - 1) & 1) == odd) queries(u, unit + 1);
+            }
+            if (busy && first < i) collect(((i - 1) & 1) == odd ? i - 1 : i - 2);
+            wild |= __any_sync(0xffffffffu, huge);
+            const bool merge = (i0 & 1) || take > 1;  // the odd warpgroup had a tile
+            if (odd) {
+                if (merge) {
+                    if (busy) {
+#pragma unroll
+                        for (int o = 0; o < D; o += 16) {
+                            uint32_t w[16];
+#pragma unroll
+                            for (int x = 0; x < 8; ++x) {
+                                w[2 * x] = __float_as_uint(acc[o / 2 + x].x);
+                                w[2 * x + 1] = __float_as_uint(acc[o / 2 + x].y);
+                            }
+                            tmem_st16(to + o, w);
+                        }
+                        sh.merge_m[quad * 32 + lane] = M;
+                        sh.merge_l[quad * 32 + lane] = l;
+                        if (lane == 0) sh.merge_wild[quad] = wild;
+                        tmem_st_wait();
+                    }
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(b.merge_full + quad);
+                    ++merges;
+                }
+                continue;
             }
             const bool whole = from == 0 && take == done.tiles;
             float* part = nullptr;
             if (!whole) {
                 part = partials + ((size_t)blockIdx.x * 2 + (from == 0)) * Partial<D>::kFloats;
                 if (from == 0) {  // goes on in the next CTAs: up to the one that holds its last tile
-                    const long long last = sh.end + (done.tiles - take) - 1;
+                    const long long last = end + (done.tiles - take) - 1;
                     int more = 0;
-                    while (sh.total * (blockIdx.x + more + 2) / sh.ctas <= last) ++more;
+                    while (total * (cta + more + 2) / ctas <= last) ++more;
                     split = ChunkSplit{done.s, done.tile, done.head, more + 1};
                 }
             }
-            if (busy) collect(i - 1);
-            wild |= __any_sync(0xffffffffu, huge);
-            if (valid && !wild) {
-                float* dst = part ? part + (size_t)row * D
-                                  : p.out + (done.first + token) * p.ld_out + (size_t)(done.head * G + sub) * D;
-                const float inv = part ? 1.0f : sees > 0 ? 1.0f / l : 0.0f;
-                if (part || wide_out) {
+            float w0 = 1.0f, w1 = 0.0f;
+            if (merge) {
+                warp_wait(sh, b.merge_full + quad, (uint32_t)merges & 1, p.err);
+                tc_fence_after();
+                ++merges;
+                if (busy) {
+                    const float m1 = sh.merge_m[quad * 32 + lane], both = fmaxf(M, m1);
+                    const float off = both == -INFINITY ? 0.0f : both;
+                    w0 = ex2(M - off);
+                    w1 = ex2(m1 - off);
+                    M = both;
+                    l = l * w0 + sh.merge_l[quad * 32 + lane] * w1;
+                    wild |= sh.merge_wild[quad] != 0;
+                }
+            }
+            if (small) {  // the four warps' sums share a maximum and a row sum
+                sh.quad_m[quad * 32 + lane] = M;
+                sh.quad_l[quad * 32 + lane] = l;
+                if (lane == 0) sh.quad_wild[quad] = wild;
+                named_bar_sync(1, 128);
+                float top = -INFINITY;
+                for (int k = 0; k < 4; ++k) {
+                    top = fmaxf(top, sh.quad_m[k * 32 + lane]);
+                    wild |= sh.quad_wild[k] != 0;
+                }
+                const float off = top == -INFINITY ? 0.0f : top, w = ex2(M - off);
+                w0 *= w;
+                w1 *= w;
+                M = top;
+                l = 0.0f;
+                for (int k = 0; k < 4; ++k) l = fmaf(ex2(sh.quad_m[k * 32 + lane] - off), sh.quad_l[k * 32 + lane], l);
+            }
+            if (!part) {
+                const float inv = sees > 0 ? 1.0f / l : 0.0f;
+                w0 = sees > 0 ? w0 * inv : 0.0f;
+                w1 = sees > 0 ? w1 * inv : 0.0f;
+            }
+            float* dst = part ? part + (size_t)row * D
+                              : p.out + (done.first + (valid ? token : 0)) * p.ld_out +
+                                    (size_t)(done.head * G + sub) * D;
+            const bool writes = valid && !wild && (!small || quad == 0);
+            if (busy) {
 #pragma unroll
-                    for (int x = 0; x < D / 2; x += 2)
-                        *reinterpret_cast<float4*>(dst + 2 * x) = make_float4(acc[x].x * inv, acc[x].y * inv,
-                                                                              acc[x + 1].x * inv, acc[x + 1].y * inv);
-                } else {
+                for (int o = 0; o < D; o += 16) {
+                    int v[16];
+                    if (merge) {
+                        tmem_ld16(to + D + o, v);
+                        tmem_ld_wait();
+                    }
 #pragma unroll
-                    for (int x = 0; x < D / 2; ++x) {
-                        dst[2 * x] = acc[x].x * inv;
-                        dst[2 * x + 1] = acc[x].y * inv;
+                    for (int x = 0; x < 8; ++x) {
+                        float2 y = __fmul2_rn(acc[o / 2 + x], make_float2(w0, w0));
+                        if (merge)
+                            y = __ffma2_rn(make_float2(__int_as_float(v[2 * x]), __int_as_float(v[2 * x + 1])),
+                                           make_float2(w1, w1), y);
+                        acc[o / 2 + x] = y;
+                    }
+                    if (small) {  // the first warp adds the others', 16 dims at a time
+                        if (o) named_bar_sync(1, 128);
+                        if (quad) {
+#pragma unroll
+                            for (int x = 0; x < 8; ++x) {
+                                sh.quad_sum[quad - 1][lane][2 * x] = acc[o / 2 + x].x;
+                                sh.quad_sum[quad - 1][lane][2 * x + 1] = acc[o / 2 + x].y;
+                            }
+                        }
+                        named_bar_sync(1, 128);
+                        if (!quad) {
+#pragma unroll
+                            for (int x = 0; x < 8; ++x)
+#pragma unroll
+                                for (int k = 0; k < 3; ++k)
+                                    acc[o / 2 + x] = __fadd2_rn(
+                                        acc[o / 2 + x], make_float2(sh.quad_sum[k][lane][2 * x],
+                                                                    sh.quad_sum[k][lane][2 * x + 1]));
+                        }
+                    }
+                    if (!writes) continue;
+                    if (part || wide_out) {
+#pragma unroll
+                        for (int x = o / 2; x < o / 2 + 8; x += 2)
+                            *reinterpret_cast<float4*>(dst + 2 * x) =
+                                make_float4(acc[x].x, acc[x].y, acc[x + 1].x, acc[x + 1].y);
+                    } else {
+#pragma unroll
+                        for (int x = o / 2; x < o / 2 + 8; ++x) {
+                            dst[2 * x] = acc[x].x;
+                            dst[2 * x + 1] = acc[x].y;
+                        }
                     }
                 }
-                if (part) {
+                if (part && writes) {
                     part[kTileRows * D + row] = M;
                     part[kTileRows * (D + 1) + row] = l;
                 }
+                if (small) named_bar_sync(1, 128);  // the sums' buffer is free again
+            }
+            if (merge) {
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(b.merge_read + quad);
             }
             if (busy && wild) rows_without_operands<D>(p, done, from * NT, (from + take) * NT, part);
-            at = 0;
         }
         if (tid == 0) splits[blockIdx.x] = split;
     } else if (count > 0) {
-        set_registers_down<kOtherRegs>();
+        set_registers_down<kOtherRegs>();  // idle
     } else if (tid == 0) {
         splits[blockIdx.x] = ChunkSplit{0, 0, 0, -1};
     }
@@ -842,71 +1094,179 @@ __global__ void __launch_bounds__(kChunkThreads, 1) chunk_tiles_kernel(ChunkPara
     }
 }
 
-// Block c: the unit that begins in CTA c and goes on in the next ones.
-constexpr int kCombineThreads = 256;
+// Block (c, y): 16 rows of the unit that begins in CTA c and goes on in the
+// next ones.  A warp a row forms the parts' weights, then the threads sum.
+constexpr int kCombineThreads = 256, kCombineRows = 16;
 template <int D>
 __global__ void __launch_bounds__(kCombineThreads) chunk_combine_kernel(ChunkParams p, const float* partials,
                                                                          const ChunkSplit* splits) {
+    __shared__ float weight[kCombineRows][kChunkCtas], norm[kCombineRows];
     pdl_wait();
     const ChunkSplit s = splits[blockIdx.x];
     if (s.more < 0) return;
     Unit u;
     u.s = s.s, u.tile = s.tile, u.head = s.head;
     set_sequence(p, u);
-    set_tile<D>(p, u);
-    const int G = p.H / p.Hkv, per = tokens_of_tile(G);
-    const int rows = min(per, u.n - u.tile * per) * G;
+    const int G = p.H / p.Hkv, per = tokens_of_tile(G), r0 = blockIdx.y * kCombineRows;
+    const int rows = min(min(per, u.n - u.tile * per) * G - r0, kCombineRows);
+    if (rows <= 0) return;
     const auto part = [&](int k) {
         return partials + ((size_t)(blockIdx.x + k) * 2 + (k == 0)) * Partial<D>::kFloats;
     };
-    for (int e = threadIdx.x; e < rows * D; e += kCombineThreads) {
-        const int row = e / D, token = u.tile * per + row / G;
-        float top = -INFINITY;
-        for (int k = 0; k <= s.more; ++k) top = fmaxf(top, part(k)[kTileRows * D + row]);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    for (int r = warp; r < rows; r += kCombineThreads / 32) {
+        float top = -INFINITY, l = 0.0f;
+        for (int k = lane; k <= s.more; k += 32) top = fmaxf(top, part(k)[kTileRows * D + r0 + r]);
+        for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
         const float off = top == -INFINITY ? 0.0f : top;
-        float o = 0.0f, l = 0.0f;
-        for (int k = 0; k <= s.more; ++k) {
-            const float* x = part(k);
-            const float w = exp2f(x[kTileRows * D + row] - off);
-            o = fmaf(w, x[e], o);
-            l = fmaf(w, x[kTileRows * (D + 1) + row], l);
+        for (int k = lane; k <= s.more; k += 32) {
+            const float w = exp2f(part(k)[kTileRows * D + r0 + r] - off);
+            weight[r][k] = w;
+            l = fmaf(w, part(k)[kTileRows * (D + 1) + r0 + r], l);
         }
-        p.out[(u.first + token) * p.ld_out + (size_t)(u.head * G + row % G) * D + e % D] =
-            u.len - u.n + token >= 0 ? o / l : 0.0f;
+        for (int o = 16; o; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+        const int token = u.tile * per + (r0 + r) / G;
+        if (lane == 0) norm[r] = u.len - u.n + token >= 0 ? 1.0f / l : 0.0f;
+    }
+    __syncthreads();
+    for (int e = threadIdx.x; e < rows * (D / 4); e += kCombineThreads) {
+        const int r = e / (D / 4), d4 = e % (D / 4) * 4, token = u.tile * per + (r0 + r) / G;
+        float4 o = make_float4(0, 0, 0, 0);
+#pragma unroll 4
+        for (int k = 0; k <= s.more; ++k) {
+            const float4 x = *reinterpret_cast<const float4*>(part(k) + (size_t)(r0 + r) * D + d4);
+            const float w = weight[r][k];
+            o.x = fmaf(w, x.x, o.x), o.y = fmaf(w, x.y, o.y), o.z = fmaf(w, x.z, o.z), o.w = fmaf(w, x.w, o.w);
+        }
+        float* dst = p.out + (u.first + token) * p.ld_out + (size_t)(u.head * G + (r0 + r) % G) * D + d4;
+        const float inv = norm[r];
+        const bool none = inv == 0.0f && u.len - u.n + token < 0;  // zeros, whatever the parts hold
+        dst[0] = none ? 0.0f : o.x * inv;
+        dst[1] = none ? 0.0f : o.y * inv;
+        dst[2] = none ? 0.0f : o.z * inv;
+        dst[3] = none ? 0.0f : o.w * inv;
     }
 }
 
-// CTAs of a launch: one per tile of work that the caller's bounds allow, at
-// most one per SM.
-int chunk_ctas(long long rows, long long batch, long long max_new, long long max_len, int H, int Hkv, int d) {
-    const long long G = H / Hkv, per = kTileRows / G, nt = d == 128 ? 64 : 128;
-    const long long units = std::min(batch * ((std::min(max_new, rows) + per - 1) / per), batch + rows / per) * Hkv;
-    const long long tiles = units * ((max_len + nt - 1) / nt);
-    return (int)std::max<long long>(1, std::min<long long>(tiles, kChunkCtas));
+// Operands of one tile of one KV head: a CTA of 8 warps, one or two pages each.
+constexpr int kOperandThreads = 256;
+template <int D>
+__global__ void __launch_bounds__(kOperandThreads) chunk_operands_kernel(ChunkParams p, Operands pre) {
+    using S = Shape<D>;
+    constexpr int PG = S::PG;
+    extern __shared__ __align__(128) uint8_t smem[];
+    __shared__ uint64_t bar[kOperandThreads / 32];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, tile = blockIdx.x, head = blockIdx.y;
+    int first, n;
+    const int s = blockIdx.z;
+    rows_of(p, s, first, n);
+    const int len = p.total_lens[s], limit = min(len, p.stride * kPageTokens);
+    if (n == 0 || tile * S::NT >= limit || len > pre.tiles * S::NT) return;
+    const size_t t = operand_tile<D>(p, pre, s, head, tile);
+    if (lane == 0) {
+        mbar_init(bar + warp, 1);
+        fence_barrier_init();
+        fence_proxy_async_shared();
+    }
+    __syncwarp();
+    int phase = 0;
+    float* src = reinterpret_cast<float*>(smem + 4 * S::kHalf + warp * S::kPageBytes);
+    for (int j = warp; j < 2 * PG; j += kOperandThreads / 32) {
+        const int page = j % PG, pos = tile * S::NT + page * kPageTokens;
+        const int id = pos < limit ? page_at(p, s, pos) : -1;
+        if (id >= 0) {
+            if (lane == 0) {
+                mbar_arrive_expect_tx(bar + warp, S::kPageBytes);
+                bulk_g2s(src, head_rows<D>(p, id, j / PG, head), S::kPageBytes, bar + warp);
+            }
+            mbar_wait(bar + warp, phase, p.err);
+            phase ^= 1;
+        }
+        const int valid = id >= 0 ? min(limit - pos, kPageTokens) : 0;
+        if (j < PG)
+            convert_k<D>(src, valid, smem, smem + S::kHalf, page, pre.scales + t * 16 + page);
+        else
+            convert_v<D>(src, valid, smem + 2 * S::kHalf, smem + 3 * S::kHalf, page, pre.scales + t * 16 + 8 + page);
+        fence_proxy_async_shared();  // the page's buffer takes the next copy
+        __syncwarp();
+    }
+    __syncthreads();
+    const uint4* from = reinterpret_cast<const uint4*>(smem);
+    uint4* to = reinterpret_cast<uint4*>(pre.ops + t * (4 * S::kHalf));
+    for (int i = threadIdx.x; i < 4 * S::kHalf / 16; i += kOperandThreads) to[i] = from[i];
 }
-size_t chunk_workspace(int ctas, int d) {
-    return (size_t)ctas * (2 * (size_t)kTileRows * (d + 2) * sizeof(float) + sizeof(ChunkSplit));
+
+// The launch for a call's bounds, and its workspace: partial sums, what is
+// split, and the operands where they are made beforehand.
+struct ChunkPlan {
+    int ctas;           // one per tile of work that the bounds allow, at most one per SM
+    int operand_tiles;  // of a sequence, 0: converted by the CTAs that read them
+    size_t splits, operands, scales, bytes;  // offsets, and all of it
+};
+ChunkPlan chunk_plan(long long rows, long long batch, long long max_new, long long max_len, int H, int Hkv, int d) {
+    const long long G = H / Hkv, per = kTileRows / G, nt = d == 128 ? 64 : 128, len_tiles = (max_len + nt - 1) / nt;
+    const long long row_tiles = std::min(batch * ((std::min(max_new, rows) + per - 1) / per), batch + rows / per);
+    ChunkPlan c{};
+    const auto most = [](long long n) { return std::min<long long>(n, kChunkCtas); };
+    c.ctas = (int)std::max<long long>(1, most(most(row_tiles) * most(Hkv) * most(len_tiles)));
+    // Made beforehand where every K and V tile is read by kPreReuse row tiles or
+    // more (as far as the bounds tell) and the operands fit kPreBytes.
+    constexpr long long kPreReuse = 8, kPreBytes = 1ll << 30;
+    const long long tile_bytes = 8 * nt * d + 64;
+    const bool fits = batch <= 65535 && len_tiles <= (1 << 24) && batch * Hkv * len_tiles <= kPreBytes / tile_bytes;
+    if (fits && rows / per >= kPreReuse * batch) c.operand_tiles = (int)len_tiles;
+    const long long all_tiles = batch * Hkv * c.operand_tiles;
+    const auto up = [](size_t n) { return (n + 127) & ~(size_t)127; };
+    c.splits = (size_t)c.ctas * 2 * kTileRows * (d + 2) * sizeof(float);
+    c.operands = up(c.splits + (size_t)c.ctas * sizeof(ChunkSplit));
+    c.scales = c.operands + (size_t)all_tiles * 8 * nt * d;
+    c.bytes = c.scales + (size_t)all_tiles * 64;
+    return c;
+}
+
+template <class K>
+cudaError_t chunk_kernel_attributes(K kernel, size_t smem, int regs) {
+    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (e != cudaSuccess || !regs) return e;
+    // setmaxnreg moves registers within what the CTA was launched with: with
+    // fewer than planned the softmax warps would wait for them
+    cudaFuncAttributes a{};
+    e = cudaFuncGetAttributes(&a, kernel);
+    return e == cudaSuccess && a.numRegs != regs ? cudaErrorNotSupported : e;
+}
+
+template <int D, bool PRE>
+cudaError_t launch_tiles(const ChunkParams& p, const ChunkPlan& plan, float* partials, ChunkSplit* splits,
+                         const Operands& pre, cudaStream_t stream) {
+    const bool wide_q = p.ld_q % 4 == 0 && aligned_to(p.q, 16), wide_out = p.ld_out % 4 == 0 && aligned_to(p.out, 16);
+    cudaError_t e = chunk_kernel_attributes(chunk_tiles_kernel<D, PRE>, Shape<D>::template kSmem<PRE>, Roles<PRE>::kLaunchRegs);
+    if (e != cudaSuccess) return e;
+    chunk_tiles_kernel<D, PRE><<<plan.ctas, Roles<PRE>::kThreads, Shape<D>::template kSmem<PRE>, stream>>>(p, partials, splits, pre,
+                                                                                               wide_q, wide_out);
+    return cudaGetLastError();
 }
 
 template <int D>
-cudaError_t launch_chunk(const ChunkParams& p, int ctas, void* workspace, cudaStream_t stream) {
-    float* partials = static_cast<float*>(workspace);
-    ChunkSplit* splits = reinterpret_cast<ChunkSplit*>(partials + (size_t)ctas * 2 * Partial<D>::kFloats);
-    const bool wide_q = p.ld_q % 4 == 0 && aligned_to(p.q, 16), wide_out = p.ld_out % 4 == 0 && aligned_to(p.out, 16);
-    cudaError_t e = cudaFuncSetAttribute(chunk_tiles_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                         (int)Shape<D>::kSmem);
-    if (e != cudaSuccess) return e;
-    // setmaxnreg moves registers within what the CTA was launched with: with
-    // fewer than planned the softmax warps would wait for them
-    cudaFuncAttributes attr_regs{};
-    e = cudaFuncGetAttributes(&attr_regs, chunk_tiles_kernel<D>);
-    if (e != cudaSuccess) return e;
-    if (attr_regs.numRegs != kLaunchRegs) return cudaErrorNotSupported;
-    chunk_tiles_kernel<D><<<ctas, kChunkThreads, Shape<D>::kSmem, stream>>>(p, partials, splits, wide_q, wide_out);
-    e = cudaGetLastError();
+cudaError_t launch_chunk(const ChunkParams& p, const ChunkPlan& plan, void* workspace, cudaStream_t stream) {
+    uint8_t* w = static_cast<uint8_t*>(workspace);
+    float* partials = reinterpret_cast<float*>(w);
+    ChunkSplit* splits = reinterpret_cast<ChunkSplit*>(w + plan.splits);
+    const Operands pre{w + plan.operands, reinterpret_cast<float*>(w + plan.scales), plan.operand_tiles};
+    cudaError_t e;
+    if (plan.operand_tiles) {
+        const size_t smem = 4 * Shape<D>::kHalf + (kOperandThreads / 32) * Shape<D>::kPageBytes;
+        e = chunk_kernel_attributes(chunk_operands_kernel<D>, smem, 0);
+        if (e != cudaSuccess) return e;
+        chunk_operands_kernel<D><<<dim3((unsigned)plan.operand_tiles, (unsigned)p.Hkv, (unsigned)p.batch),
+                                   kOperandThreads, smem, stream>>>(p, pre);
+        e = cudaGetLastError();
+        if (e == cudaSuccess) e = launch_tiles<D, true>(p, plan, partials, splits, pre, stream);
+    } else {
+        e = launch_tiles<D, false>(p, plan, partials, splits, pre, stream);
+    }
     if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3((unsigned)ctas);
+    cfg.gridDim = dim3((unsigned)plan.ctas, kTileRows / kCombineRows);
     cfg.blockDim = dim3(kCombineThreads);
     cfg.stream = stream;
     cudaLaunchAttribute attr[1];
@@ -924,7 +1284,7 @@ using namespace tb;
 
 static tb_status check_chunk(int rows, int batch, int max_new, int max_len, int H, int Hkv, int d) {
     TB_ENTRY_CHECK(rows >= 0 && batch >= 1 && max_new >= 1 && max_len >= 1, "bad rows / batch / lengths");
-    TB_ENTRY_CHECK(H >= 1 && Hkv >= 1 && H % Hkv == 0, "heads must divide: H %d, Hkv %d", H, Hkv);
+    TB_ENTRY_CHECK(H >= 1 && Hkv >= 1 && H % Hkv == 0 && Hkv <= 65535, "heads must divide: H %d, Hkv %d", H, Hkv);
     if ((d != 16 && d != 32 && d != 64 && d != 128) || H / Hkv > kTileRows)
         return (tb_status)report_error(TB_ERR_UNSUPPORTED,
                                        "head dimension %d is not 16, 32, 64 or 128, or %d query heads share a KV head "
@@ -939,7 +1299,7 @@ extern "C" tb_status tb_paged_attention_chunk_workspace(int32_t rows, int32_t ba
     *bytes = 0;
     tb_status st = check_chunk(rows, batch, max_new, max_len, H, Hkv, d);
     if (st == TB_OK && rows > 0)
-        *bytes = (int64_t)chunk_workspace(chunk_ctas(rows, batch, max_new, max_len, H, Hkv, d), d);
+        *bytes = (int64_t)chunk_plan(rows, batch, max_new, max_len, H, Hkv, d).bytes;
     return st;
 }
 
@@ -958,17 +1318,17 @@ extern "C" tb_status tb_paged_attention_chunk_dev(void* stream, const float* q, 
     TB_ENTRY_CHECK(ld_q >= (int64_t)H * d && ld_out >= (int64_t)H * d, "a row stride is shorter than its row");
     TB_ENTRY_CHECK(aligned_to(pool, 16), "kv_pool must be 16-byte aligned");
     if (rows == 0) return TB_OK;
-    const int ctas = chunk_ctas(rows, batch, max_new, max_len, H, Hkv, d);
-    TB_ENTRY_CHECK(workspace && aligned_to(workspace, 16) && workspace_bytes >= (int64_t)chunk_workspace(ctas, d),
-                   "the workspace must be 16-byte aligned and hold %lld bytes", (long long)chunk_workspace(ctas, d));
+    const ChunkPlan plan = chunk_plan(rows, batch, max_new, max_len, H, Hkv, d);
+    TB_ENTRY_CHECK(workspace && aligned_to(workspace, 16) && workspace_bytes >= (int64_t)plan.bytes,
+                   "the workspace must be 16-byte aligned and hold %lld bytes", (long long)plan.bytes);
     StreamEntry entry(pool, "kv_pool");
     if (entry.status != TB_OK) return entry.status;
     ChunkParams p{q, ld_q, row_offsets, total_lens, batch, rows, pool, num_pages, table, stride, layer, num_layers, H,
                   Hkv, out, ld_out, entry.err};
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    cudaError_t e = d == 16   ? launch_chunk<16>(p, ctas, workspace, s)
-                    : d == 32 ? launch_chunk<32>(p, ctas, workspace, s)
-                    : d == 64 ? launch_chunk<64>(p, ctas, workspace, s)
-                              : launch_chunk<128>(p, ctas, workspace, s);
+    cudaError_t e = d == 16   ? launch_chunk<16>(p, plan, workspace, s)
+                    : d == 32 ? launch_chunk<32>(p, plan, workspace, s)
+                    : d == 64 ? launch_chunk<64>(p, plan, workspace, s)
+                              : launch_chunk<128>(p, plan, workspace, s);
     return launch_status(e, "chunk attention launch");
 }

@@ -90,7 +90,26 @@ __device__ __forceinline__ int block_exponent(uint32_t max_bits) {
     return max_bits ? max((int)(max_bits >> 23) - 127 - 14, -100) : 0;
 }
 __device__ __forceinline__ float exp2_int(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }  // |e| <= 126
-__device__ __forceinline__ uint32_t abs_bits(float x) { return __float_as_uint(x) & 0x7fffffffu; }
+// Largest magnitude of three, NaN if one is (one instruction).
+__device__ __forceinline__ float max_abs(float a, float b, float c) {
+    float y;
+    asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
+    return y;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float y;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
+    return y;
+}
+// One thread of a converged warp.  The tensor-core instructions take their
+// operands from uniform registers: in a branch that the compiler knows to hold
+// one thread they issue back to back (64 cycles for N = 128, as fast as they
+// run); under `lane == 0` each took more than 120.
+__device__ __forceinline__ bool elect_one() {
+    uint32_t p;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
+    return p != 0;
+}
 // Moves the executing warpgroup's share of the CTA's registers to R a thread.
 template <int R>
 __device__ __forceinline__ void set_registers_up() {
