@@ -38,14 +38,16 @@ __device__ __forceinline__ void rows_of(const ChunkParams& p, int s, int& first,
     count = max(min(p.row_offsets[s + 1], p.rows) - first, 0);
 }
 
-// Pool page of a position, -1 where there is none (evicted, or reported as bad).
-__device__ __forceinline__ int page_at(const ChunkParams& p, int s, int pos) {
-    const int page = p.table[(size_t)s * p.stride + pos / kPageTokens];
+// Pool page of a table entry, -1 where there is none (evicted, or reported as bad).
+__device__ __forceinline__ int checked_page(const ChunkParams& p, int page) {
     if (page >= p.num_pages) {
         record_error(p.err, kDevBadPage);
         return -1;
     }
     return page;
+}
+__device__ __forceinline__ int page_at(const ChunkParams& p, int s, int pos) {
+    return checked_page(p, p.table[(size_t)s * p.stride + pos / kPageTokens]);
 }
 
 template <int D>
@@ -120,21 +122,22 @@ struct RowSum {
 // several CTAs hold leaves partial sums in the workspace; chunk_combine_kernel
 // adds them in the order of the CTAs.
 //
-// Roles (16 warps):
+// Roles:
 //   producer   one lane per page of a tile: page table, then a bulk copy of the
 //              page's K or V rows of this head into a ring of fp32 pages;
-//   converters (6 warps) one page at a time: the page's largest magnitude gives
+//   converters (10 warps) one page at a time: the page's largest magnitude gives
 //              a power-of-two scale, the halves go to the K and V operand rings;
 //   issuer     one thread: S(i + 1) before P V(i), so the softmax of a tile runs
 //              while the tensor cores do the next S and the last P V;
-//   softmax    two warpgroups, one for even and one for odd tiles, a row a
-//              thread: base-2 softmax over the tile, P as halves over S in tensor
-//              memory, and the P V of the warpgroup's last tile added to the row's
-//              sums in registers, which are rescaled only where its running
-//              maximum grew by more than 2^8.  Each keeps its own maximum and
-//              sums; at a unit's end the odd one hands its to the even one, which
-//              writes the unit.  (One warpgroup took 6300 cycles a tile: one warp
-//              per scheduler waits for each of its own instructions.)
+//   softmax    a warpgroup, a row a thread: base-2 softmax over the tile, P as
+//              halves over S in tensor memory, and the P V of the last tile added
+//              to the row's sums in registers, which are rescaled only where the
+//              running maximum grew by more than 2^8.
+// Where the operands are made beforehand (long prompts) there are no converters;
+// the producer copies operand tiles, and a second softmax warpgroup takes the
+// odd tiles: one warp per scheduler waits for its own instructions, two fill
+// each other's gaps.  Each keeps its own maximum and sums, and at a unit's end
+// the odd one hands its to the even one, which writes the unit.
 //
 // With c the row's scale times the page's, a score is c S and a weighted value
 // 2^(c S - M) v = 2^(c S + e - M) (v 2^-e): the page's value exponent e enters
@@ -145,21 +148,26 @@ struct RowSum {
 // rows of the tile), nor have scores beyond 2^20: the unit's rows are then summed
 // in fp32 on the CUDA cores.
 // ---------------------------------------------------------------------------
-constexpr int kSoftmaxWarps = 8;  // a warpgroup of 4 per tile parity
 // The roles' warps, and the registers of a thread: the launch's, then what the
 // softmax warpgroups (with the rows' sums) take and the others keep.
 template <bool PRE>
 struct Roles {
-    static constexpr int kConvertWarps = PRE ? 0 : 6;
+    static constexpr int kGroups = PRE ? 2 : 1;  // softmax warpgroups
+    static constexpr int kSoftmaxWarps = 4 * kGroups, kConvertWarps = PRE ? 0 : 10;
     static constexpr int kIssueWarp = kSoftmaxWarps + kConvertWarps, kLoadWarp = kIssueWarp + 1;
     static constexpr int kThreads = PRE ? 384 : 512;
-    static constexpr int kLaunchRegs = PRE ? 168 : 128, kSoftmaxRegs = PRE ? 208 : 192, kOtherRegs = PRE ? 88 : 64;
-    static_assert(2 * 128 * kSoftmaxRegs + (kThreads - 256) * kOtherRegs == kThreads * kLaunchRegs, "registers");
+    static constexpr int kLaunchRegs = PRE ? 168 : 128, kSoftmaxRegs = PRE ? 208 : 224, kOtherRegs = PRE ? 88 : 96;
+    static_assert(kGroups * 128 * kSoftmaxRegs + (kThreads - kGroups * 128) * kOtherRegs == kThreads * kLaunchRegs,
+                  "registers");
     static_assert(kLoadWarp < kThreads / 32, "warps");
 };
 constexpr int kChunkCtas = 148;   // most CTAs of a launch (the workspace's size)
 constexpr int kTileRows = 128;
 constexpr int kScaleRing = 8;     // tiles whose page scales are kept, at least two more than operand tiles
+// Barriers that free the operand tiles, more than there are tiles: a converter
+// warp may have no K (or V) page in a tile, and a phase two back on the same
+// barrier would then look like the one it waits for.
+constexpr int kEmptyRing = 4;
 constexpr int kUnitRing = 4;      // units whose queries' scales are kept: with units of one tile, one
                                   // softmax warpgroup can be two units ahead of the other
 constexpr uint32_t kWildBits = (127u + 20u) << 23;    // a K or V value of 2^20
@@ -175,12 +183,18 @@ struct Shape {
     static constexpr int PG = NT / kPageTokens;        // its pages
     static constexpr int kPageBytes = kPageTokens * D * 4;
     static constexpr int kHalf = NT * D * 2;           // bytes of one operand half
-    static constexpr int kSlots = D == 128 ? 10 : D == 64 ? 20 : 32;  // fp32 pages, at least a tile's
-    // K and V operand tiles each, and the bytes of shared memory
+    // fp32 pages on their way: a page takes about 3 us under load, so what streams
+    // from HBM is bound by the bytes in flight (80 KB: 3.7 TB/s)
+    static constexpr int kSlots = D == 128 ? 14 : D == 64 ? 28 : 64;
+    // K and V operand tiles, and the bytes of shared memory.  K is free once S is
+    // done, V only after P V, one softmax later.
     template <bool PRE>
-    static constexpr int kStages = PRE ? 3 : 2;
+    static constexpr int kKStages = PRE ? 3 : 1;
     template <bool PRE>
-    static constexpr size_t kSmem = (size_t)kStages<PRE> * 4 * kHalf + (PRE ? 0 : (size_t)kSlots * kPageBytes);
+    static constexpr int kVStages = PRE ? 3 : 2;
+    template <bool PRE>
+    static constexpr size_t kSmem = (size_t)(kKStages<PRE> + kVStages<PRE>) * 2 * kHalf +
+                                    (PRE ? 0 : (size_t)kSlots * kPageBytes);
     // tensor memory columns
     static constexpr int kS = 0, kO = 2 * NT, kQ = kO + 2 * D;  // S / P and O twice
     static_assert(kQ + D <= 512, "tensor memory");
@@ -194,8 +208,9 @@ struct Unit {
 };
 
 struct ChunkBars {
-    uint64_t slot_full[32], slot_empty[32];
-    uint64_t k_full[3], k_empty[3], v_full[3], v_empty[3];
+    uint64_t slot_full[64], slot_empty[64];
+    uint64_t k_full[3], v_full[3];
+    uint64_t k_empty[kEmptyRing], v_empty[kEmptyRing];  // by tile, see kEmptyRing
     uint64_t scales[kScaleRing];
     uint64_t s_full[2], p_full[2];
     uint64_t pv_done[2], q_full[kUnitRing], merge_full[4], merge_read[4], drained;
@@ -251,14 +266,14 @@ template <int D>
 __device__ __forceinline__ long long tiles_before(const ChunkParams& p, Unit u, int count) {
     constexpr int NT = Shape<D>::NT;
     const int per = tokens_of_tile(p.H / p.Hkv), held = u.len - u.n, all = (u.n + per - 1) / per;
-    if (held >= 0 && u.len <= p.stride * kPageTokens) {
+    if (count > 4 && held >= 0 && u.len <= p.stride * kPageTokens) {
         // ceil((held + (t + 1) per) / NT) each, but for the last row tile of the sequence
         const int full = min(count, all - 1);
         long long sum = floor_sum(full, NT, per, (long long)held + per + NT - 1);
         if (count == all && all > 0) sum += (u.len + NT - 1) / NT;
         return sum;
     }
-    long long sum = 0;  // lengths that do not fit (reported): one by one
+    long long sum = 0;  // a few, or lengths that do not fit (reported): one by one
     for (u.tile = 0; u.tile < count; ++u.tile) {
         set_tile<D>(p, u);
         sum += u.tiles;
@@ -302,9 +317,10 @@ __device__ __forceinline__ size_t operand_tile(const ChunkParams& p, const Opera
 struct ChunkShared {
     ChunkBars bars;
     alignas(16) float scale[kScaleRing][16];  // of a tile's pages: K factors, then V exponents
-    int slot_page[32];
+    int slot_page[64];
     Unit start;
     int start_tile;
+    long long start_at;
     long long scan[16];
     uint32_t tmem;
     float q_scale[kUnitRing][kTileRows];              // of the units' rows
@@ -340,6 +356,12 @@ __device__ __forceinline__ bool chunk_wait(ChunkShared& sh, uint64_t* bar, uint3
     }
     return false;
 }
+// Whether the operand tile that position tile i goes to is free: its last user,
+// `stages` tiles before, has been read.
+__device__ __forceinline__ bool wait_free(ChunkShared& sh, uint64_t* ring, int i, int stages, int* err) {
+    const int last = i - stages;
+    return last < 0 || chunk_wait(sh, ring + last % kEmptyRing, (uint32_t)(last / kEmptyRing & 1), err);
+}
 __device__ __forceinline__ void warp_wait(ChunkShared& sh, uint64_t* bar, uint32_t parity, int* err) {
     if ((threadIdx.x & 31) == 0) chunk_wait(sh, bar, parity, err);
     __syncwarp();
@@ -360,8 +382,7 @@ __device__ __forceinline__ void split4(const float4& a, float s, uint2& hi, uint
 // time.  Lane (r, q) of a step takes dims 4 g .. of token r + 8 (q & 1) with g
 // staggered over the lanes, so that the reads (rows of D floats, 16 bytes a
 // lane) and the writes (8 bytes of a core matrix's 16-byte rows) fall into
-// different banks.  The page is read twice, for its largest magnitude and for
-// its halves, which costs less than the registers to keep it.
+// different banks.
 template <int D>
 __device__ __forceinline__ void convert_k(const float* src, int valid, uint8_t* hi, uint8_t* lo, int page,
                                           float* scale_out) {
@@ -369,25 +390,23 @@ __device__ __forceinline__ void convert_k(const float* src, int valid, uint8_t* 
     const int lane = threadIdx.x & 31, r = lane & 15;
     const int g0 = (lane & 7) + ((lane >> 3) & 1) + (lane >> 4) * kTasks;
     const float* row = src + r * D;
-    const bool in = r < valid;
-    float m = 0.0f;
-    if (in) {
+    float4 x[kTasks];
 #pragma unroll
-        for (int t = 0; t < kTasks; ++t) {
-            const float4 a = lds128f(row + ((g0 + t) % C) * 4);
-            m = max_abs(max_abs(m, a.x, a.y), a.z, a.w);
-        }
-    }
+    for (int t = 0; t < kTasks; ++t)
+        x[t] = r < valid ? lds128f(row + ((g0 + t) % C) * 4) : make_float4(0, 0, 0, 0);
+    float m = 0.0f;
+#pragma unroll
+    for (int t = 0; t < kTasks; ++t) m = max_abs(max_abs(m, x[t].x, x[t].y), x[t].z, x[t].w);
     const uint32_t bits = warp_max_bits(m);
     const int e = block_exponent(bits);
     const float s = exp2_int(-e);
     if (lane == 0) *scale_out = bits >= kWildBits ? kWildMark : exp2_int(e);
     const int at0 = (page * 2 + (r >> 3)) * (D * 16) + (r & 7) * 16;
-#pragma unroll 4
+#pragma unroll
     for (int t = 0; t < kTasks; ++t) {
         const int g = (g0 + t) % C, at = at0 + (g >> 1) * 128 + (g & 1) * 8;
         uint2 h, l;
-        split4(in ? lds128f(row + g * 4) : make_float4(0, 0, 0, 0), s, h, l);
+        split4(x[t], s, h, l);
         *reinterpret_cast<uint2*>(hi + at) = h;
         *reinterpret_cast<uint2*>(lo + at) = l;
     }
@@ -400,33 +419,28 @@ __device__ __forceinline__ void convert_v(const float* src, int valid, uint8_t* 
                                           float* exp_out) {
     constexpr int NT = Shape<D>::NT, kTasks = D / 16;
     const int lane = threadIdx.x & 31;
+    float x[kTasks][8];
     float m = 0.0f;
 #pragma unroll
-    for (int t = 0; t < 2 * kTasks; ++t) {  // any order will do for the maximum
-        const int item = lane + 32 * t;
-        if (item / (D / 4) < valid) {
-            const float4 a = lds128f(src + item * 4);
-            m = max_abs(max_abs(m, a.x, a.y), a.z, a.w);
-        }
+    for (int t = 0; t < kTasks; ++t) {
+        const int task = lane + 32 * t, n = task % D, kc = task / D;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[t][j] = kc * 8 + j < valid ? src[(kc * 8 + j) * D + n] : 0.0f;
     }
+#pragma unroll
+    for (int t = 0; t < kTasks; ++t)
+#pragma unroll
+        for (int j = 0; j < 8; j += 2) m = max_abs(m, x[t][j], x[t][j + 1]);
     const uint32_t bits = warp_max_bits(m);
     const int e = block_exponent(bits);
     const float s = exp2_int(-e);
     if (lane == 0) *exp_out = bits >= kWildBits ? kWildMark : (float)e;
-#pragma unroll 2
+#pragma unroll
     for (int t = 0; t < kTasks; ++t) {
         const int task = lane + 32 * t, n = task % D, kc = task / D;
-        float x[8];
-        if (valid == kPageTokens) {
-#pragma unroll
-            for (int j = 0; j < 8; ++j) x[j] = src[(kc * 8 + j) * D + n];
-        } else {
-#pragma unroll
-            for (int j = 0; j < 8; ++j) x[j] = kc * 8 + j < valid ? src[(kc * 8 + j) * D + n] : 0.0f;
-        }
         uint2 h0, l0, h1, l1;
-        split4(make_float4(x[0], x[1], x[2], x[3]), s, h0, l0);
-        split4(make_float4(x[4], x[5], x[6], x[7]), s, h1, l1);
+        split4(make_float4(x[t][0], x[t][1], x[t][2], x[t][3]), s, h0, l0);
+        split4(make_float4(x[t][4], x[t][5], x[t][6], x[t][7]), s, h1, l1);
         const int at = (n >> 3) * (NT * 16) + (page * 2 + kc) * 128 + (n & 7) * 16;
         *reinterpret_cast<uint4*>(hi + at) = make_uint4(h0.x, h0.y, h1.x, h1.y);
         *reinterpret_cast<uint4*>(lo + at) = make_uint4(l0.x, l0.y, l1.x, l1.y);
@@ -514,17 +528,19 @@ __global__ void __launch_bounds__(Roles<PRE>::kThreads, 1)
     chunk_tiles_kernel(ChunkParams p, float* partials, ChunkSplit* splits, Operands pre, bool wide_q, bool wide_out) {
     using S = Shape<D>;
     using R = Roles<PRE>;
-    constexpr int NT = S::NT, PG = S::PG, kStages = S::template kStages<PRE>, kChunkThreads = R::kThreads;
+    constexpr int NT = S::NT, PG = S::PG, kChunkThreads = R::kThreads;
+    constexpr int kKStages = S::template kKStages<PRE>, kVStages = S::template kVStages<PRE>;
     constexpr int kIssueWarp = R::kIssueWarp, kLoadWarp = R::kLoadWarp, kConvertWarps = R::kConvertWarps;
-    constexpr int kSoftmaxRegs = R::kSoftmaxRegs, kOtherRegs = R::kOtherRegs;
+    constexpr int kSoftmaxRegs = R::kSoftmaxRegs, kOtherRegs = R::kOtherRegs, kSoftmaxWarps = R::kSoftmaxWarps;
+    constexpr int kGroups = R::kGroups;
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ ChunkShared sh;
     static_assert(S::template kSmem<PRE> + sizeof(ChunkShared) <= 227 * 1024, "shared memory");
-    static_assert(kScaleRing >= kStages + 2 && S::kSlots >= 2 * PG && S::kSlots > kConvertWarps, "rings");
+    static_assert(S::kSlots <= 64 && kScaleRing >= kVStages + 2 && S::kSlots >= 2 * PG && S::kSlots >= kConvertWarps, "rings");
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     uint8_t* k_ops = smem;                                // [stage][hi, lo]
-    uint8_t* v_ops = smem + kStages * 2 * S::kHalf;
-    uint8_t* pages = smem + kStages * 4 * S::kHalf;
+    uint8_t* v_ops = smem + kKStages * 2 * S::kHalf;
+    uint8_t* pages = v_ops + kVStages * 2 * S::kHalf;
     ChunkBars& b = sh.bars;
 
     // the CTA's share: tiles [total c / C, total (c + 1) / C) of all units'
@@ -550,9 +566,11 @@ __global__ void __launch_bounds__(Roles<PRE>::kThreads, 1)
             mbar_init(b.slot_full + i, 1);
             mbar_init(b.slot_empty + i, 1);
         }
-        for (int i = 0; i < kStages; ++i) {
+        for (int i = 0; i < 3; ++i) {
             mbar_init(b.k_full + i, PRE ? 1 : PG);
             mbar_init(b.v_full + i, PRE ? 1 : PG);
+        }
+        for (int i = 0; i < kEmptyRing; ++i) {
             mbar_init(b.k_empty + i, 1);
             mbar_init(b.v_empty + i, 1);
         }
@@ -580,26 +598,52 @@ __global__ void __launch_bounds__(Roles<PRE>::kThreads, 1)
     const long long ctas = min((long long)gridDim.x, total), cta = blockIdx.x;  // every share has a tile
     const long long begin = cta < ctas ? total * cta / ctas : 0, end = cta < ctas ? total * (cta + 1) / ctas : 0;
     const long long count = end - begin;
+    const int per_tile = tokens_of_tile(p.H / p.Hkv);
     if (count > 0 && mine > 0 && before <= begin && begin < before + mine) {
         Unit u;
         long long at = begin - before;
-        for (u.s = s0;; ++u.s) {
+        for (u.s = s0; s1 - s0 > 1; ++u.s) {
             const long long here = tiles_of_sequence<D>(p, u.s);
             if (at < here) break;
             at -= here;
         }
         set_sequence(p, u);
-        int lo = 0, hi = (u.n + tokens_of_tile(p.H / p.Hkv) - 1) / tokens_of_tile(p.H / p.Hkv);
-        while (hi - lo > 1) {  // the last row tile that begins at or before `at`
-            const int mid = (lo + hi) / 2;
-            if (tiles_before<D>(p, u, mid) * p.Hkv <= at) lo = mid; else hi = mid;
-        }
-        at -= tiles_before<D>(p, u, lo) * p.Hkv;
-        u.tile = lo;
-        set_tile<D>(p, u);
-        u.head = (int)(at / u.tiles);
+        u.head = u.tile = 0;
         sh.start = u;
-        sh.start_tile = (int)(at % u.tiles);
+        sh.start_at = at;
+    }
+    __syncthreads();
+    if (count > 0) {  // its row tile: a run of row tiles a thread
+        Unit u = sh.start;
+        const int all = (u.n + per_tile - 1) / per_tile, each = (all + kChunkThreads - 1) / kChunkThreads;
+        const int t0 = min(tid * each, all), t1 = min(t0 + each, all);
+        long long here = 0;
+        for (u.tile = t0; u.tile < t1; ++u.tile) {
+            set_tile<D>(p, u);
+            here += (long long)u.tiles * p.Hkv;
+        }
+        long long upto = here;
+        if (all > each) {
+            for (int o = 1; o < 32; o <<= 1) {
+                const long long t = __shfl_up_sync(0xffffffffu, upto, o);
+                if (lane >= o) upto += t;
+            }
+            if (lane == 31) sh.scan[warp] = upto;
+            __syncthreads();
+            for (int w = 0; w < warp; ++w) upto += sh.scan[w];
+        }
+        long long at = sh.start_at - (upto - here);
+        __syncthreads();
+        if (here > 0 && at >= 0 && at < here) {
+            for (u.tile = t0;; ++u.tile) {
+                set_tile<D>(p, u);
+                if (at < (long long)u.tiles * p.Hkv) break;
+                at -= (long long)u.tiles * p.Hkv;
+            }
+            u.head = (int)(at / u.tiles);
+            sh.start = u;
+            sh.start_tile = (int)(at % u.tiles);
+        }
     }
     if (warp == kIssueWarp) tmem_alloc(&sh.tmem, 512);
     tc_fence_before();
@@ -620,18 +664,18 @@ __global__ void __launch_bounds__(Roles<PRE>::kThreads, 1)
                 for (long long left = count; left > 0 && !sh.dead; at = 0) {
                     const int take = (int)min((long long)(u.tiles - at), left);
                     for (int j = at; j < at + take; ++j, ++i) {
-                        const int st = i % kStages, ring = i % kScaleRing;
+                        const int sk = i % kKStages, sv = i % kVStages, ring = i % kScaleRing;
                         const bool made = u.len <= pre.tiles * NT;  // a longer one goes without operands
                         const size_t t = made ? operand_tile<D>(p, pre, u.s, u.head, j) : 0;
                         const uint8_t* src = pre.ops + t * (4 * S::kHalf);
-                        if (!chunk_wait(sh, b.k_empty + st, (uint32_t)(i / kStages & 1) ^ 1, p.err)) break;
+                        if (!wait_free(sh, b.k_empty, i, kKStages, p.err)) break;
                         mbar_arrive_expect_tx(b.scales + ring, 64);
                         bulk_g2s(sh.scale[ring], pre.scales + t * 16, 64, b.scales + ring);
-                        mbar_arrive_expect_tx(b.k_full + st, 2 * S::kHalf);
-                        bulk_g2s(k_ops + st * 2 * S::kHalf, src, 2 * S::kHalf, b.k_full + st);
-                        if (!chunk_wait(sh, b.v_empty + st, (uint32_t)(i / kStages & 1) ^ 1, p.err)) break;
-                        mbar_arrive_expect_tx(b.v_full + st, 2 * S::kHalf);
-                        bulk_g2s(v_ops + st * 2 * S::kHalf, src + 2 * S::kHalf, 2 * S::kHalf, b.v_full + st);
+                        mbar_arrive_expect_tx(b.k_full + sk, 2 * S::kHalf);
+                        bulk_g2s(k_ops + sk * 2 * S::kHalf, src, 2 * S::kHalf, b.k_full + sk);
+                        if (!wait_free(sh, b.v_empty, i, kVStages, p.err)) break;
+                        mbar_arrive_expect_tx(b.v_full + sv, 2 * S::kHalf);
+                        bulk_g2s(v_ops + sv * 2 * S::kHalf, src + 2 * S::kHalf, 2 * S::kHalf, b.v_full + sv);
                     }
                     left -= take;
                     if (left > 0) next_unit<D>(p, u);
@@ -644,33 +688,56 @@ __global__ void __launch_bounds__(Roles<PRE>::kThreads, 1)
             }
             __syncwarp();
         } else {
+        // Table entries are read a tile ahead: their latency would otherwise stand
+        // in front of every tile's copies.
         int jobs = 0, slot = lane, fill = 0;  // the lane's page slot, and how often it was filled before
-        for (long long left = count; left > 0 && !sh.dead; at = 0) {
-            const int take = (int)min((long long)(u.tiles - at), left);
-            for (int j = at; j < at + take; ++j, jobs += 2 * PG) {
-                if (lane < 2 * PG) {
-                    const int kv = lane / PG, pos = j * NT + (lane % PG) * kPageTokens;
-                    const int page = pos < u.limit ? page_at(p, u.s, pos) : -1;
-                    if (chunk_wait(sh, b.slot_empty + slot, (uint32_t)(fill & 1) ^ 1, p.err)) {
-                        sh.slot_page[slot] = page;
-                        if (page >= 0) {
-                            mbar_arrive_expect_tx(b.slot_full + slot, S::kPageBytes);
-                            bulk_g2s(pages + slot * S::kPageBytes, head_rows<D>(p, page, kv, u.head), S::kPageBytes,
-                                     b.slot_full + slot);
-                        } else {
-                            mbar_arrive(b.slot_full + slot);
-                        }
-                    }
-                    slot += 2 * PG;
-                    if (slot >= S::kSlots) {
-                        slot -= S::kSlots;
-                        ++fill;
+        const bool mine = lane < 2 * PG;
+        const int kv = lane / PG, in_tile = lane % PG * kPageTokens;
+        const auto entry = [&](int j) {
+            const int pos = j * NT + in_tile;
+            return mine && pos < u.limit ? p.table[(size_t)u.s * p.stride + pos / kPageTokens] : -1;
+        };
+        long long left = count;
+        int j = at, end_j = at + (int)min((long long)(u.tiles - at), left), page = entry(j);
+        while (left > 0 && !sh.dead) {
+            const int now = page, head = u.head;
+            --left;
+            if (left > 0) {
+                if (++j == end_j) {
+                    next_unit<D>(p, u);
+                    j = 0;
+                    end_j = (int)min((long long)u.tiles, left);
+                }
+                page = entry(j);
+            }
+            // Four pages at a time: one by one, sixteen lanes' branches in turn took
+            // longer than the copies, and all together waited for the last slot.
+            const int id = mine ? checked_page(p, now) : -1;
+            for (int g = 0; g < 2 * PG; g += 4) {
+                const bool turn = lane >= g && lane < g + 4;
+                bool ready = !turn;
+                while (!__all_sync(0xffffffffu, ready))
+                    if (!ready)
+                        ready = chunk_wait(sh, b.slot_empty + slot, (uint32_t)(fill & 1) ^ 1, p.err) || sh.dead;
+                if (turn && !sh.dead) {
+                    sh.slot_page[slot] = id;
+                    if (id >= 0) {
+                        mbar_arrive_expect_tx(b.slot_full + slot, S::kPageBytes);
+                        bulk_g2s(pages + slot * S::kPageBytes, head_rows<D>(p, id, kv, head), S::kPageBytes,
+                                 b.slot_full + slot);
+                    } else {
+                        mbar_arrive(b.slot_full + slot);
                     }
                 }
                 __syncwarp();
             }
-            left -= take;
-            if (left > 0) next_unit<D>(p, u);
+            slot += 2 * PG;
+            if (slot >= S::kSlots) {
+                slot -= S::kSlots;
+                ++fill;
+            }
+            __syncwarp();
+            jobs += 2 * PG;
         }
         if (sh.dead) {  // copies still in flight must land before the CTA ends
             const uint64_t t0 = global_timer_ns();
@@ -689,23 +756,23 @@ __global__ void __launch_bounds__(Roles<PRE>::kThreads, 1)
             const uint32_t k0 = smem_u32(k_ops), v0 = smem_u32(v_ops);
             int i = 0, unit = 0;
             const auto issue_s = [&](int item, bool first, int un) {
-                const int st = item % kStages;
+                const int st = item % kKStages;
                 if (first) chunk_wait(sh, b.q_full + un % kUnitRing, (uint32_t)(un / kUnitRing & 1), p.err);
-                chunk_wait(sh, b.k_full + st, (uint32_t)(item / kStages & 1), p.err);
+                chunk_wait(sh, b.k_full + st, (uint32_t)(item / kKStages & 1), p.err);
                 tc_fence_after();
                 const uint32_t kb = k0 + st * 2 * S::kHalf;
                 tc_mma_split<NT, D>(tmem + S::kS + (uint32_t)(item & 1) * NT, tmem + S::kQ,
                                     [](int s) { return 8 * s; }, D / 2, kb, kb + S::kHalf);
                 tc_commit(b.s_full + (item & 1));
-                tc_commit(b.k_empty + st);
+                tc_commit(b.k_empty + item % kEmptyRing);
             };
             for (long long left = count; left > 0; at = 0) {
                 const int take = (int)min((long long)(u.tiles - at), left);
                 issue_s(i, true, unit);
                 for (int j = 0; j < take; ++j, ++i) {
                     if (j + 1 < take) issue_s(i + 1, false, unit);
-                    const int st = i % kStages;
-                    chunk_wait(sh, b.v_full + st, (uint32_t)(i / kStages & 1), p.err);
+                    const int st = i % kVStages;
+                    chunk_wait(sh, b.v_full + st, (uint32_t)(i / kVStages & 1), p.err);
                     chunk_wait(sh, b.p_full + (i & 1), (uint32_t)(i / 2 & 1), p.err);
                     tc_fence_after();
                     const uint32_t vb = v0 + st * 2 * S::kHalf;
@@ -713,7 +780,7 @@ __global__ void __launch_bounds__(Roles<PRE>::kThreads, 1)
                     // tiles before was read before P of this one arrived.
                     tc_mma_split<D, NT>(tmem + S::kO + (uint32_t)(i & 1) * D, tmem + S::kS + (uint32_t)(i & 1) * NT,
                                         [](int s) { return 32 * (s / 2) + 8 * (s % 2); }, 16, vb, vb + S::kHalf);
-                    tc_commit(b.v_empty + st);
+                    tc_commit(b.v_empty + i % kEmptyRing);
                     tc_commit(b.pv_done + (i & 1));
                 }
                 left -= take;
@@ -735,14 +802,16 @@ __global__ void __launch_bounds__(Roles<PRE>::kThreads, 1)
         for (long long left = count; left > 0; at = 0) {
             const int take = (int)min((long long)(u.tiles - at), left);
             for (int j = at; j < at + take; ++j, ++i, jj -= 2 * PG) {
-                const int st = i % kStages, ring = i % kScaleRing;
+                const int ring = i % kScaleRing;
                 for (; jj < 2 * PG; jj += PRE ? 2 * PG : kConvertWarps) {
                     const bool is_v = jj >= PG;
                     const int page = jj % PG;
                     warp_wait(sh, b.slot_full + slot, (uint32_t)fill & 1, p.err);
                     const int left_here = u.limit - (j * NT + page * kPageTokens);
                     const int valid = sh.slot_page[slot] < 0 ? 0 : max(0, min(left_here, kPageTokens));
-                    warp_wait(sh, (is_v ? b.v_empty : b.k_empty) + st, (uint32_t)(i / kStages & 1) ^ 1, p.err);
+                    const int st = is_v ? i % kVStages : i % kKStages;
+                    if (lane == 0) wait_free(sh, is_v ? b.v_empty : b.k_empty, i, is_v ? kVStages : kKStages, p.err);
+                    __syncwarp();
                     const float* src = reinterpret_cast<const float*>(pages + slot * S::kPageBytes);
                     uint8_t* op = (is_v ? v_ops : k_ops) + st * 2 * S::kHalf;
                     if (is_v)
@@ -767,12 +836,12 @@ __global__ void __launch_bounds__(Roles<PRE>::kThreads, 1)
             if (left > 0) next_unit<D>(p, u);
         }
     } else if (count > 0 && warp < kSoftmaxWarps) {
-        // ---- softmax: warpgroup `odd` takes the tiles of its parity ----
+        // ---- softmax: of two warpgroups each takes the tiles of its parity ----
         set_registers_up<kSoftmaxRegs>();
-        const int odd = warp >> 2, quad = warp & 3;
+        const int group = warp >> 2, quad = warp & 3;
         const uint32_t lanes = (uint32_t)(quad * 32) << 16;
         const int G = p.H / p.Hkv, per = tokens_of_tile(G);
-        const uint32_t ts = tmem + S::kS + (uint32_t)odd * NT + lanes, to = tmem + S::kO + (uint32_t)odd * D + lanes;
+        const uint32_t s0_addr = tmem + S::kS + lanes, o0_addr = tmem + S::kO + lanes;
         ChunkSplit split{0, 0, 0, -1};
         // A unit of at most 32 rows would leave three of a warpgroup's four warps
         // idle: its rows stand in all four lane groups, each of which takes a
@@ -793,15 +862,13 @@ __global__ void __launch_bounds__(Roles<PRE>::kThreads, 1)
             if (lane == 0) mbar_arrive(b.q_full + unit % kUnitRing);
         };
         int i = 0, unit = 0, merges = 0;
-        if (!odd) queries(u, 0);
+        if (group == 0) queries(u, 0);
         for (long long left = count; left > 0; ++unit) {
             const int take = (int)min((long long)(u.tiles - at), left);
             const bool small = small_unit(u);
             const int row = small ? lane : quad * 32 + lane, sub = row % G;
             const int token = u.tile * per + row / G;
             const bool valid = row < per * G && token < u.n;
-            // the warp's positions of a tile: [from_col, to_col)
-            const int from_col = small ? quad * (NT / 4) : 0, to_col = small ? from_col + NT / 4 : NT;
             const bool busy = __any_sync(0xffffffffu, valid);
             const int sees = min(u.len - u.n + token + 1, u.limit);  // the row's own limit, may be <= 0
             const int first_sees = __shfl_sync(0xffffffffu, sees, 0);  // tokens ascend with the lanes
@@ -814,118 +881,157 @@ __global__ void __launch_bounds__(Roles<PRE>::kThreads, 1)
             for (int x = 0; x < D / 2; ++x) acc[x] = make_float2(0.0f, 0.0f);
             // adds P V of the warpgroup's tile `item`, whose scale the sums still have
             const auto collect = [&](int item) {
-                warp_wait(sh, b.pv_done + odd, (uint32_t)(item / 2 & 1), p.err);
+                warp_wait(sh, b.pv_done + (item & 1), (uint32_t)(item / 2 & 1), p.err);
                 tc_fence_after();
-#pragma unroll
-                for (int o = 0; o < D; o += 16) {
+                const uint32_t to = o0_addr + (uint32_t)(item & 1) * D;
+                if constexpr (D == 16) {
                     int v[16];
-                    tmem_ld16(to + o, v);
+                    tmem_ld16(to, v);
                     tmem_ld_wait();
 #pragma unroll
                     for (int x = 0; x < 8; ++x)
-                        acc[o / 2 + x] = __fadd2_rn(
-                            acc[o / 2 + x], make_float2(__int_as_float(v[2 * x]), __int_as_float(v[2 * x + 1])));
+                        acc[x] = __fadd2_rn(acc[x],
+                                            make_float2(__int_as_float(v[2 * x]), __int_as_float(v[2 * x + 1])));
+                } else {
+#pragma unroll
+                    for (int o = 0; o < D; o += 64) {
+                        int v[2][32];
+                        tmem_ld32(to + o, v[0]);
+                        if (o + 32 < D) tmem_ld32(to + o + 32, v[1]);
+                        tmem_ld_wait();
+#pragma unroll
+                        for (int h = 0; h < 2 && o + 32 * h < D; ++h)
+#pragma unroll
+                            for (int x = 0; x < 16; ++x)
+                                acc[o / 2 + 16 * h + x] = __fadd2_rn(
+                                    acc[o / 2 + 16 * h + x], make_float2(__int_as_float(v[h][2 * x]),
+                                                                         __int_as_float(v[h][2 * x + 1])));
+                    }
                 }
             };
-            const int i0 = i, first = (i0 & 1) == odd ? i0 : i0 + 1;  // this warpgroup's first tile of the unit
-            for (i = first; i < i0 + take; i += 2) {
+            const int i0 = i;  // then this warpgroup's first tile of the unit:
+            const int first = kGroups == 1 || (i0 & 1) == group ? i0 : i0 + 1;
+            for (i = first; i < i0 + take; i += kGroups) {
+                const uint32_t ts = s0_addr + (uint32_t)(i & 1) * NT;
                 const int j = at + (i - i0), ring = i % kScaleRing;
                 warp_wait(sh, b.scales + ring, (uint32_t)(i / kScaleRing & 1), p.err);
-                warp_wait(sh, b.s_full + odd, (uint32_t)(i / 2 & 1), p.err);
+                warp_wait(sh, b.s_full + (i & 1), (uint32_t)(i / 2 & 1), p.err);
                 tc_fence_after();
                 if (busy) {
                     const float *ks = sh.scale[ring], *ve = ks + 8;
                     const int room = sees - j * NT;                 // columns below it are seen
                     const bool masked = first_sees < (j + 1) * NT;  // some row does not see all of the tile
-                    // the row's maximum of score + value exponent: per page the largest S decides
-                    float top = -INFINITY;
-#pragma unroll 1
-                    for (int g = from_col / 32; g * 32 < to_col; ++g) {
-                        int v[32];
-                        tmem_ld32(ts + 32 * g, v);
-                        tmem_ld_wait();
-                        if (masked) {
+                    // A block of W positions: -inf where the row does not see one, the largest
+                    // score + value exponent (per page the largest S decides), and the weights.
+                    const auto mask = [&](auto& v, int col) {
+                        constexpr int W = sizeof(v) / 4;
 #pragma unroll
-                            for (int x = 0; x < 32; ++x)
-                                if (32 * g + x >= room) v[x] = __float_as_int(-INFINITY);
+                        for (int x = 0; x < W; ++x)
+                            if (col + x >= room) v[x] = __float_as_int(-INFINITY);
+                    };
+                    const auto page_top = [&](const int* v, int page) {
+                        float m0 = __int_as_float(v[0]), m1 = __int_as_float(v[1]);
+#pragma unroll
+                        for (int x = 2; x < 14; x += 4) {
+                            m0 = max3(m0, __int_as_float(v[x]), __int_as_float(v[x + 1]));
+                            m1 = max3(m1, __int_as_float(v[x + 2]), __int_as_float(v[x + 3]));
                         }
+                        m0 = max3(m0, __int_as_float(v[14]), __int_as_float(v[15]));
+                        wild |= ks[page] == kWildMark || ve[page] == kWildMark;
+                        return fmaf(fmaxf(m0, m1), c * ks[page], ve[page]);
+                    };
+                    const auto page_weights = [&](const int* v, int page, float shift, uint32_t* hi, uint32_t* lo) {
+                        const float e = ve[page], k = c * ks[page];
+                        const float2 kk = make_float2(k, k), bb = make_float2(e + shift, e + shift);
+                        float2 sum = make_float2(0.0f, 0.0f);
 #pragma unroll
-                        for (int h = 0; h < 2; ++h) {
-                            float m0 = __int_as_float(v[16 * h]), m1 = __int_as_float(v[16 * h + 1]);
-#pragma unroll
-                            for (int x = 16 * h + 2; x < 16 * h + 14; x += 4) {
-                                m0 = max3(m0, __int_as_float(v[x]), __int_as_float(v[x + 1]));
-                                m1 = max3(m1, __int_as_float(v[x + 2]), __int_as_float(v[x + 3]));
-                            }
-                            m0 = max3(m0, __int_as_float(v[16 * h + 14]), __int_as_float(v[16 * h + 15]));
-                            const int page = 2 * g + h;
-                            if (NT / 4 >= 32 || (page * 16 >= from_col && page * 16 < to_col)) {
-                                wild |= ks[page] == kWildMark || ve[page] == kWildMark;
-                                top = fmaxf(top, fmaf(fmaxf(m0, m1), c * ks[page], ve[page]));
-                            }
+                        for (int x = 0; x < 16; x += 2) {
+                            const float2 t =
+                                __ffma2_rn(make_float2(__int_as_float(v[x]), __int_as_float(v[x + 1])), kk, bb);
+                            const float2 w = make_float2(ex2(t.x), ex2(t.y));
+                            sum = __fadd2_rn(sum, w);
+                            split_pair(w.x, w.y, hi[x / 2], lo[x / 2]);
                         }
-                    }
-                    huge |= valid && top > -INFINITY && fabsf(top) > kHuge;
+                        l = fmaf(sum.x + sum.y, ex2(-e), l);
+                    };
                     float r = 1.0f;
-                    if (top > M + kLazy || (M == -INFINITY && top > -INFINITY)) {
-                        r = M == -INFINITY ? 0.0f : ex2(M - top);
-                        M = top;
-                        l *= r;
-                    }
-                    const float shift = kPShift - (M == -INFINITY ? 0.0f : M);
-#pragma unroll 1
-                    for (int g = 0; g < NT / 32; ++g) {
-                        uint32_t hi[16], lo[16];
-                        if (32 * g + 32 <= from_col || 32 * g >= to_col) {  // another warp's positions
+                    // takes the block's maximum into the reference; the result is P's shift
+                    const auto refer = [&](float top) {
+                        huge |= valid && top > -INFINITY && fabsf(top) > kHuge;
+                        if (top > M + kLazy || (M == -INFINITY && top > -INFINITY)) {
+                            r = M == -INFINITY ? 0.0f : ex2(M - top);
+                            M = top;
+                            l *= r;
+                        }
+                        return kPShift - (M == -INFINITY ? 0.0f : M);
+                    };
+                    if (small) {  // the warp's quarter, kept in registers; zeros elsewhere
+                        constexpr int W = NT / 4;
+                        const int col = quad * W, g = col / 32;
+                        int v[W];
+                        if constexpr (W == 32)
+                            tmem_ld32(ts + col, v);
+                        else
+                            tmem_ld16(ts + col, v);
+                        tmem_ld_wait();
+                        uint32_t zero[32];
 #pragma unroll
-                            for (int x = 0; x < 16; ++x) hi[x] = lo[x] = 0;
+                        for (int x = 0; x < 32; ++x) zero[x] = 0;
+#pragma unroll
+                        for (int k = 0; k < NT / 32; ++k)
+                            if (W == 16 || k != g) tmem_st32(ts + 32 * k, zero);
+                        if (masked) mask(v, col);
+                        float top = page_top(v, col / 16);
+                        if constexpr (W == 32) top = fmaxf(top, page_top(v + 16, col / 16 + 1));
+                        const float shift = refer(top);
+                        uint32_t hi[W / 2], lo[W / 2];
+                        page_weights(v, col / 16, shift, hi, lo);
+                        if constexpr (W == 32) {
+                            page_weights(v + 16, col / 16 + 1, shift, hi + 8, lo + 8);
+                            tmem_st16(ts + 32 * g, hi);
+                            tmem_st16(ts + 32 * g + 16, lo);
                         } else {
+                            tmem_st_wait();  // over the zeros
+                            tmem_st8(ts + 32 * g + col % 32 / 2, hi);
+                            tmem_st8(ts + 32 * g + 16 + col % 32 / 2, lo);
+                        }
+                    } else {
+                        float top = -INFINITY;
+#pragma unroll 1
+                        for (int g = 0; g < NT / 32; ++g) {
                             int v[32];
                             tmem_ld32(ts + 32 * g, v);
-                            const float e0 = ve[2 * g], e1 = ve[2 * g + 1];
-                            const float k0 = c * ks[2 * g], k1 = c * ks[2 * g + 1];
-                            // where a warp's quarter is one page, the other page of the 32 gets no weight
-                            const float off0 = NT / 4 >= 32 || 32 * g >= from_col ? shift : -INFINITY;
-                            const float off1 = NT / 4 >= 32 || 32 * g + 16 < to_col ? shift : -INFINITY;
                             tmem_ld_wait();
-                            if (masked) {
-#pragma unroll
-                                for (int x = 0; x < 32; ++x)
-                                    if (32 * g + x >= room) v[x] = __float_as_int(-INFINITY);
-                            }
-#pragma unroll
-                            for (int h = 0; h < 2; ++h) {
-                                const float2 kk = h ? make_float2(k1, k1) : make_float2(k0, k0);
-                                const float2 bb = h ? make_float2(e1 + off1, e1 + off1)
-                                                    : make_float2(e0 + off0, e0 + off0);
-                                float2 sum = make_float2(0.0f, 0.0f);
-#pragma unroll
-                                for (int x = 16 * h; x < 16 * h + 16; x += 2) {
-                                    const float2 t = __ffma2_rn(
-                                        make_float2(__int_as_float(v[x]), __int_as_float(v[x + 1])), kk, bb);
-                                    const float2 w = make_float2(ex2(t.x), ex2(t.y));
-                                    sum = __fadd2_rn(sum, w);
-                                    split_pair(w.x, w.y, hi[x / 2], lo[x / 2]);
-                                }
-                                l = fmaf(sum.x + sum.y, ex2(h ? -e1 : -e0), l);
-                            }
+                            if (masked) mask(v, 32 * g);
+                            top = max3(top, page_top(v, 2 * g), page_top(v + 16, 2 * g + 1));
                         }
-                        tmem_st16(ts + 32 * g, hi);
-                        tmem_st16(ts + 32 * g + 16, lo);
+                        const float shift = refer(top);
+#pragma unroll 1
+                        for (int g = 0; g < NT / 32; ++g) {
+                            int v[32];
+                            uint32_t hi[16], lo[16];
+                            tmem_ld32(ts + 32 * g, v);
+                            tmem_ld_wait();
+                            if (masked) mask(v, 32 * g);
+                            page_weights(v, 2 * g, shift, hi, lo);
+                            page_weights(v + 16, 2 * g + 1, shift, hi + 8, lo + 8);
+                            tmem_st16(ts + 32 * g, hi);
+                            tmem_st16(ts + 32 * g + 16, lo);
+                        }
                     }
                     tmem_st_wait();
-                    if (i > first) collect(i - 2);
+                    if (i > first) collect(i - kGroups);
                     if (__any_sync(0xffffffffu, r != 1.0f)) {
 #pragma unroll
                         for (int x = 0; x < D / 2; ++x) acc[x] = __fmul2_rn(acc[x], make_float2(r, r));
                     }
                 }
                 // the odd sums of the last unit still stand where P V of this tile goes
-                if (odd && i == first && merges > 0)
+                if (group == 1 && i == first && merges > 0)
                     warp_wait(sh, b.merge_read + quad, (uint32_t)(merges - 1) & 1, p.err);
                 tc_fence_before();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(b.p_full + odd);
+                if (lane == 0) mbar_arrive(b.p_full + (i & 1));
             }
             i = i0 + take;
             const Unit done = u;
@@ -935,12 +1041,12 @@ __global__ void __launch_bounds__(Roles<PRE>::kThreads, 1)
             if (left > 0) {
                 next_unit<D>(p, u);
                 // the warpgroup of the unit's last tile knows that its queries are read
-                if (((i - 1) & 1) == odd) queries(u, unit + 1);
+                if (kGroups == 1 || ((i - 1) & 1) == group) queries(u, unit + 1);
             }
-            if (busy && first < i) collect(((i - 1) & 1) == odd ? i - 1 : i - 2);
+            if (busy && first < i) collect(kGroups == 1 || ((i - 1) & 1) == group ? i - 1 : i - 2);
             wild |= __any_sync(0xffffffffu, huge);
-            const bool merge = (i0 & 1) || take > 1;  // the odd warpgroup had a tile
-            if (odd) {
+            const bool merge = kGroups == 2 && ((i0 & 1) || take > 1);  // the odd warpgroup had a tile
+            if (group == 1) {
                 if (merge) {
                     if (busy) {
 #pragma unroll
@@ -951,7 +1057,7 @@ __global__ void __launch_bounds__(Roles<PRE>::kThreads, 1)
                                 w[2 * x] = __float_as_uint(acc[o / 2 + x].x);
                                 w[2 * x + 1] = __float_as_uint(acc[o / 2 + x].y);
                             }
-                            tmem_st16(to + o, w);
+                            tmem_st16(o0_addr + D + o, w);
                         }
                         sh.merge_m[quad * 32 + lane] = M;
                         sh.merge_l[quad * 32 + lane] = l;
@@ -1022,7 +1128,7 @@ __global__ void __launch_bounds__(Roles<PRE>::kThreads, 1)
                 for (int o = 0; o < D; o += 16) {
                     int v[16];
                     if (merge) {
-                        tmem_ld16(to + D + o, v);
+                        tmem_ld16(o0_addr + D + o, v);
                         tmem_ld_wait();
                     }
 #pragma unroll

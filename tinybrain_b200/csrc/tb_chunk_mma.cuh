@@ -45,7 +45,7 @@ template <int N, int K, class Step>
 __device__ __forceinline__ void tc_mma_split(uint32_t d, uint32_t a, Step step, uint32_t lo_at, uint32_t b_hi,
                                              uint32_t b_lo) {
     constexpr uint32_t idesc = tc_idesc_f16(N);
-#pragma unroll
+#pragma unroll 1
     for (int product = 0; product < 3; ++product) {
         const uint32_t half = product == 0 ? lo_at : 0, b = product == 1 ? b_lo : b_hi;
 #pragma unroll
