@@ -123,10 +123,11 @@ struct RowSum {
 // adds them in the order of the CTAs.
 //
 // Roles:
-//   producer   one lane per page of a tile: page table, then a bulk copy of the
-//              page's K or V rows of this head into a ring of fp32 pages;
-//   converters (10 warps) one page at a time: the page's largest magnitude gives
-//              a power-of-two scale, the halves go to the K and V operand rings;
+//   producers  (2 warps: K, V) a lane per page of a tile: page table, then a bulk
+//              copy of the page's rows of this head into a ring of fp32 pages;
+//   converters (8 warps) the K and the V page of 16 tokens at a time: a page's
+//              largest magnitude gives a power-of-two scale, the halves go to the
+//              operand tiles;
 //   issuer     one thread: S(i + 1) before P V(i), so the softmax of a tile runs
 //              while the tensor cores do the next S and the last P V;
 //   softmax    a warpgroup, a row a thread: base-2 softmax over the tile, P as
@@ -153,13 +154,14 @@ struct RowSum {
 template <bool PRE>
 struct Roles {
     static constexpr int kGroups = PRE ? 2 : 1;  // softmax warpgroups
-    static constexpr int kSoftmaxWarps = 4 * kGroups, kConvertWarps = PRE ? 0 : 10;
+    static constexpr int kSoftmaxWarps = 4 * kGroups, kConvertWarps = PRE ? 0 : 8;
     static constexpr int kIssueWarp = kSoftmaxWarps + kConvertWarps, kLoadWarp = kIssueWarp + 1;
+    static constexpr int kLoadWarps = PRE ? 1 : 2;  // K pages, V pages
     static constexpr int kThreads = PRE ? 384 : 512;
     static constexpr int kLaunchRegs = PRE ? 168 : 128, kSoftmaxRegs = PRE ? 208 : 224, kOtherRegs = PRE ? 88 : 96;
     static_assert(kGroups * 128 * kSoftmaxRegs + (kThreads - kGroups * 128) * kOtherRegs == kThreads * kLaunchRegs,
                   "registers");
-    static_assert(kLoadWarp < kThreads / 32, "warps");
+    static_assert(kLoadWarp + kLoadWarps <= kThreads / 32, "warps");
 };
 constexpr int kChunkCtas = 148;   // most CTAs of a launch (the workspace's size)
 constexpr int kTileRows = 128;
@@ -356,12 +358,21 @@ __device__ __forceinline__ bool chunk_wait(ChunkShared& sh, uint64_t* bar, uint3
     }
     return false;
 }
-// Whether the operand tile that position tile i goes to is free: its last user,
-// `stages` tiles before, has been read.
-__device__ __forceinline__ bool wait_free(ChunkShared& sh, uint64_t* ring, int i, int stages, int* err) {
-    const int last = i - stages;
-    return last < 0 || chunk_wait(sh, ring + last % kEmptyRing, (uint32_t)(last / kEmptyRing & 1), err);
+// The same for several barriers at once: every lane with one of its own (bar not
+// null) waits for it, all return together.  With the roles' code spread over the
+// instruction cache a wait costs some 300 cycles even where nothing is missing.
+__device__ __forceinline__ void lanes_wait(ChunkShared& sh, uint64_t* bar, uint32_t parity, int* err) {
+    bool ok = !bar || sleep_on(bar, parity);
+    if (__all_sync(0xffffffffu, ok)) return;
+    if (!ok) chunk_wait(sh, bar, parity, err);
+    __syncwarp();
 }
+// What frees the operand tile that position tile i goes to: the product with its
+// last user, `stages` tiles before.
+__device__ __forceinline__ uint64_t* free_bar(uint64_t* ring, int i, int stages) {
+    return i < stages ? nullptr : ring + (i - stages) % kEmptyRing;
+}
+__device__ __forceinline__ uint32_t free_parity(int i, int stages) { return (uint32_t)((i - stages) / kEmptyRing & 1); }
 __device__ __forceinline__ void warp_wait(ChunkShared& sh, uint64_t* bar, uint32_t parity, int* err) {
     if ((threadIdx.x & 31) == 0) chunk_wait(sh, bar, parity, err);
     __syncwarp();
@@ -536,7 +547,7 @@ __global__ void __launch_bounds__(Roles<PRE>::kThreads, 1)
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ ChunkShared sh;
     static_assert(S::template kSmem<PRE> + sizeof(ChunkShared) <= 227 * 1024, "shared memory");
-    static_assert(S::kSlots <= 64 && kScaleRing >= kVStages + 2 && S::kSlots >= 2 * PG && S::kSlots >= kConvertWarps, "rings");
+    static_assert(S::kSlots <= 64 && kScaleRing >= kVStages + 2 && S::kSlots >= 2 * PG && PG <= 8, "rings");
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     uint8_t* k_ops = smem;                                // [stage][hi, lo]
     uint8_t* v_ops = smem + kKStages * 2 * S::kHalf;
@@ -597,7 +608,7 @@ __global__ void __launch_bounds__(Roles<PRE>::kThreads, 1)
     }
     const long long ctas = min((long long)gridDim.x, total), cta = blockIdx.x;  // every share has a tile
     const long long begin = cta < ctas ? total * cta / ctas : 0, end = cta < ctas ? total * (cta + 1) / ctas : 0;
-    const long long count = end - begin;
+    const int count = (int)(end - begin);
     const int per_tile = tokens_of_tile(p.H / p.Hkv);
     if (count > 0 && mine > 0 && before <= begin && begin < before + mine) {
         Unit u;
@@ -655,25 +666,25 @@ __global__ void __launch_bounds__(Roles<PRE>::kThreads, 1)
     int at = sh.start_tile;
 
     // (a warpgroup's warps all move the same way, each in its own role)
-    if (count > 0 && warp == kLoadWarp) {
+    if (count > 0 && warp >= kLoadWarp && warp < kLoadWarp + R::kLoadWarps) {
         // ---- producer ----
         set_registers_down<kOtherRegs>();
         if constexpr (PRE) {
             int i = 0;
             if (lane == 0) {
-                for (long long left = count; left > 0 && !sh.dead; at = 0) {
-                    const int take = (int)min((long long)(u.tiles - at), left);
+                for (int left = count; left > 0 && !sh.dead; at = 0) {
+                    const int take = min(u.tiles - at, left);
                     for (int j = at; j < at + take; ++j, ++i) {
                         const int sk = i % kKStages, sv = i % kVStages, ring = i % kScaleRing;
                         const bool made = u.len <= pre.tiles * NT;  // a longer one goes without operands
                         const size_t t = made ? operand_tile<D>(p, pre, u.s, u.head, j) : 0;
                         const uint8_t* src = pre.ops + t * (4 * S::kHalf);
-                        if (!wait_free(sh, b.k_empty, i, kKStages, p.err)) break;
+                        if (i >= kKStages && !chunk_wait(sh, free_bar(b.k_empty, i, kKStages), free_parity(i, kKStages), p.err)) break;
                         mbar_arrive_expect_tx(b.scales + ring, 64);
                         bulk_g2s(sh.scale[ring], pre.scales + t * 16, 64, b.scales + ring);
                         mbar_arrive_expect_tx(b.k_full + sk, 2 * S::kHalf);
                         bulk_g2s(k_ops + sk * 2 * S::kHalf, src, 2 * S::kHalf, b.k_full + sk);
-                        if (!wait_free(sh, b.v_empty, i, kVStages, p.err)) break;
+                        if (i >= kVStages && !chunk_wait(sh, free_bar(b.v_empty, i, kVStages), free_parity(i, kVStages), p.err)) break;
                         mbar_arrive_expect_tx(b.v_full + sv, 2 * S::kHalf);
                         bulk_g2s(v_ops + sv * 2 * S::kHalf, src + 2 * S::kHalf, 2 * S::kHalf, b.v_full + sv);
                     }
@@ -689,45 +700,36 @@ __global__ void __launch_bounds__(Roles<PRE>::kThreads, 1)
             __syncwarp();
         } else {
         // Table entries are read a tile ahead: their latency would otherwise stand
-        // in front of every tile's copies.
-        int jobs = 0, slot = lane, fill = 0;  // the lane's page slot, and how often it was filled before
-        const bool mine = lane < 2 * PG;
-        const int kv = lane / PG, in_tile = lane % PG * kPageTokens;
+        // in front of every tile's copies.  Four pages go at a time: one by one the
+        // lanes' branches take longer than the copies, and a whole tile would wait
+        // for its last slot.
+        const int kv = warp - kLoadWarp;
+        int jobs = 0, slot = kv * PG + lane, fill = 0;  // the lane's page slot, and its fills before
+        const bool mine = lane < PG;
         const auto entry = [&](int j) {
-            const int pos = j * NT + in_tile;
+            const int pos = j * NT + lane * kPageTokens;
             return mine && pos < u.limit ? p.table[(size_t)u.s * p.stride + pos / kPageTokens] : -1;
         };
-        long long left = count;
-        int j = at, end_j = at + (int)min((long long)(u.tiles - at), left), page = entry(j);
+        int left = count, j = at, end_j = at + min(u.tiles - at, left), page = entry(j);
         while (left > 0 && !sh.dead) {
-            const int now = page, head = u.head;
-            --left;
-            if (left > 0) {
+            const int id = checked_page(p, page);
+            const float* src = head_rows<D>(p, max(id, 0), kv, u.head);
+            if (--left > 0) {
                 if (++j == end_j) {
                     next_unit<D>(p, u);
                     j = 0;
-                    end_j = (int)min((long long)u.tiles, left);
+                    end_j = min(u.tiles, left);
                 }
                 page = entry(j);
             }
-            // Four pages at a time: one by one, sixteen lanes' branches in turn took
-            // longer than the copies, and all together waited for the last slot.
-            const int id = mine ? checked_page(p, now) : -1;
-            for (int g = 0; g < 2 * PG; g += 4) {
+#pragma unroll 1
+            for (int g = 0; g < PG; g += 4) {
                 const bool turn = lane >= g && lane < g + 4;
-                bool ready = !turn;
-                while (!__all_sync(0xffffffffu, ready))
-                    if (!ready)
-                        ready = chunk_wait(sh, b.slot_empty + slot, (uint32_t)(fill & 1) ^ 1, p.err) || sh.dead;
+                lanes_wait(sh, turn ? b.slot_empty + slot : nullptr, (uint32_t)(fill & 1) ^ 1, p.err);
                 if (turn && !sh.dead) {
                     sh.slot_page[slot] = id;
-                    if (id >= 0) {
-                        mbar_arrive_expect_tx(b.slot_full + slot, S::kPageBytes);
-                        bulk_g2s(pages + slot * S::kPageBytes, head_rows<D>(p, id, kv, head), S::kPageBytes,
-                                 b.slot_full + slot);
-                    } else {
-                        mbar_arrive(b.slot_full + slot);
-                    }
+                    mbar_arrive_expect_tx(b.slot_full + slot, id >= 0 ? S::kPageBytes : 0);
+                    if (id >= 0) bulk_g2s(pages + slot * S::kPageBytes, src, S::kPageBytes, b.slot_full + slot);
                 }
                 __syncwarp();
             }
@@ -736,12 +738,11 @@ __global__ void __launch_bounds__(Roles<PRE>::kThreads, 1)
                 slot -= S::kSlots;
                 ++fill;
             }
-            __syncwarp();
             jobs += 2 * PG;
         }
         if (sh.dead) {  // copies still in flight must land before the CTA ends
             const uint64_t t0 = global_timer_ns();
-            for (int s = lane; s < S::kSlots; s += 32) {
+            for (int s = lane; s < S::kSlots; s += 32) {  // (a slot of the other producer's counts too)
                 const int fills = jobs > s ? (jobs - 1 - s) / S::kSlots + 1 : 0;
                 while (fills && !mbar_try_wait(b.slot_full + s, (uint32_t)(fills - 1) & 1) &&
                        global_timer_ns() - t0 < kWaitLimitNs) {
@@ -766,8 +767,8 @@ __global__ void __launch_bounds__(Roles<PRE>::kThreads, 1)
                 tc_commit(b.s_full + (item & 1));
                 tc_commit(b.k_empty + item % kEmptyRing);
             };
-            for (long long left = count; left > 0; at = 0) {
-                const int take = (int)min((long long)(u.tiles - at), left);
+            for (int left = count; left > 0; at = 0) {
+                const int take = min(u.tiles - at, left);
                 issue_s(i, true, unit);
                 for (int j = 0; j < take; ++j, ++i) {
                     if (j + 1 < take) issue_s(i + 1, false, unit);
@@ -795,41 +796,42 @@ __global__ void __launch_bounds__(Roles<PRE>::kThreads, 1)
         }
         __syncwarp();
     } else if (!PRE && count > 0 && warp >= kSoftmaxWarps && warp < kIssueWarp) {
-        // ---- converters: the CTA's pages in order, each warp every sixth ----
+        // ---- converters: a warp takes the same pages of every tile (of every second one where a
+        //      tile has only four) ----
         set_registers_down<kOtherRegs>();
-        int i = 0, jj = warp - kSoftmaxWarps;
-        int slot = jj, fill = 0;  // page slot, and how often it was filled before
-        for (long long left = count; left > 0; at = 0) {
-            const int take = (int)min((long long)(u.tiles - at), left);
-            for (int j = at; j < at + take; ++j, ++i, jj -= 2 * PG) {
-                const int ring = i % kScaleRing;
-                for (; jj < 2 * PG; jj += PRE ? 2 * PG : kConvertWarps) {
-                    const bool is_v = jj >= PG;
-                    const int page = jj % PG;
-                    warp_wait(sh, b.slot_full + slot, (uint32_t)fill & 1, p.err);
-                    const int left_here = u.limit - (j * NT + page * kPageTokens);
-                    const int valid = sh.slot_page[slot] < 0 ? 0 : max(0, min(left_here, kPageTokens));
-                    const int st = is_v ? i % kVStages : i % kKStages;
-                    if (lane == 0) wait_free(sh, is_v ? b.v_empty : b.k_empty, i, is_v ? kVStages : kKStages, p.err);
-                    __syncwarp();
+        constexpr int kStep = 8 / PG;
+        const int cw = warp - kSoftmaxWarps, page = cw % PG;
+        int i = 0, mine = cw / PG;  // the CTA's tile, and the warp's next one
+        int left = count;
+        for (; left > 0; at = 0) {
+            const int take = min(u.tiles - at, left);
+            for (int j = at; j < at + take; ++j, ++i) {
+                if (i != mine) continue;
+                mine += kStep;
+                const int ring = i % kScaleRing, valid_here = u.limit - (j * NT + page * kPageTokens);
+                const int job = i * (2 * PG) + page;
+                for (int kv = 0; kv < 2; ++kv) {
+                    const int slot = (job + kv * PG) % S::kSlots, fill = (job + kv * PG) / S::kSlots;
+                    const int st = kv ? i % kVStages : i % kKStages, stages = kv ? kVStages : kKStages;
+                    // lane 0: the page, lane 1: its place in the operand tile
+                    lanes_wait(sh,
+                               lane == 0   ? b.slot_full + slot
+                               : lane == 1 ? free_bar(kv ? b.v_empty : b.k_empty, i, stages)
+                                           : nullptr,
+                               lane == 0 ? (uint32_t)fill & 1 : free_parity(i, stages), p.err);
+                    const int valid = sh.slot_page[slot] < 0 ? 0 : max(0, min(valid_here, kPageTokens));
                     const float* src = reinterpret_cast<const float*>(pages + slot * S::kPageBytes);
-                    uint8_t* op = (is_v ? v_ops : k_ops) + st * 2 * S::kHalf;
-                    if (is_v)
+                    uint8_t* op = (kv ? v_ops : k_ops) + st * 2 * S::kHalf;
+                    if (kv)
                         convert_v<D>(src, valid, op, op + S::kHalf, page, &sh.scale[ring][8 + page]);
                     else
                         convert_k<D>(src, valid, op, op + S::kHalf, page, &sh.scale[ring][page]);
                     fence_proxy_async_shared();
                     __syncwarp();
-                    if (lane == 0) {
-                        mbar_arrive((is_v ? b.v_full : b.k_full) + st);
-                        mbar_arrive(b.slot_empty + slot);
-                        mbar_arrive(b.scales + ring);
-                    }
-                    slot += kConvertWarps;
-                    if (slot >= S::kSlots) {
-                        slot -= S::kSlots;
-                        ++fill;
-                    }
+                    if (lane < 3)
+                        mbar_arrive(lane == 0   ? (kv ? b.v_full : b.k_full) + st
+                                    : lane == 1 ? b.slot_empty + slot
+                                                : b.scales + ring);
                 }
             }
             left -= take;
@@ -863,8 +865,8 @@ __global__ void __launch_bounds__(Roles<PRE>::kThreads, 1)
         };
         int i = 0, unit = 0, merges = 0;
         if (group == 0) queries(u, 0);
-        for (long long left = count; left > 0; ++unit) {
-            const int take = (int)min((long long)(u.tiles - at), left);
+        for (int left = count; left > 0; ++unit) {
+            const int take = min(u.tiles - at, left);
             const bool small = small_unit(u);
             const int row = small ? lane : quad * 32 + lane, sub = row % G;
             const int token = u.tile * per + row / G;
@@ -914,8 +916,8 @@ __global__ void __launch_bounds__(Roles<PRE>::kThreads, 1)
             for (i = first; i < i0 + take; i += kGroups) {
                 const uint32_t ts = s0_addr + (uint32_t)(i & 1) * NT;
                 const int j = at + (i - i0), ring = i % kScaleRing;
-                warp_wait(sh, b.scales + ring, (uint32_t)(i / kScaleRing & 1), p.err);
-                warp_wait(sh, b.s_full + (i & 1), (uint32_t)(i / 2 & 1), p.err);
+                lanes_wait(sh, lane == 0 ? b.scales + ring : lane == 1 ? b.s_full + (i & 1) : nullptr,
+                           (uint32_t)(lane == 0 ? i / kScaleRing : i / 2) & 1, p.err);
                 tc_fence_after();
                 if (busy) {
                     const float *ks = sh.scale[ring], *ve = ks + 8;
