@@ -7,106 +7,12 @@
 // are in the cache before the call).  Query head h reads KV head h / (H/Hkv).
 // Rows of an evicted page (table entry -1) are zeros, as in the decode
 // attention (ModelRunner.swift:519-579 over KVCache.swift's pages).
-#include <climits>
-
 #include "tb_chunk_mma.cuh"
-#include "tb_common.cuh"
-#include "tb_stream_entry.h"
+#include "tb_chunk_few.cuh"
+#include "tb_chunk_units.cuh"
 
 namespace tb {
 namespace {
-
-struct ChunkParams {
-    const float* q;
-    long long ld_q;
-    const int* row_offsets;
-    const int* total_lens;
-    int batch, rows;
-    const float* pool;
-    int num_pages;
-    const int* table;
-    int stride;
-    int layer, num_layers, H, Hkv;
-    float* out;
-    long long ld_out;
-    int* err;
-};
-
-// The rows of sequence s that the call holds.
-__device__ __forceinline__ void rows_of(const ChunkParams& p, int s, int& first, int& count) {
-    first = min(max(p.row_offsets[s], 0), p.rows);
-    count = max(min(p.row_offsets[s + 1], p.rows) - first, 0);
-}
-
-// Pool page of a table entry, -1 where there is none (evicted, or reported as bad).
-__device__ __forceinline__ int checked_page(const ChunkParams& p, int page) {
-    if (page >= p.num_pages) {
-        record_error(p.err, kDevBadPage);
-        return -1;
-    }
-    return page;
-}
-__device__ __forceinline__ int page_at(const ChunkParams& p, int s, int pos) {
-    return checked_page(p, p.table[(size_t)s * p.stride + pos / kPageTokens]);
-}
-
-template <int D>
-__device__ __forceinline__ const float* head_rows(const ChunkParams& p, int page, int kv, int head) {
-    return p.pool + ((((size_t)page * p.num_layers + p.layer) * 2 + kv) * p.Hkv + head) * (size_t)(kPageTokens * D);
-}
-
-// One query row of one head over positions [t0, t1) by one warp: lane = token
-// for the scores, lane = dim for the sums; fp32 throughout.
-template <int D>
-struct RowSum {
-    float m = -INFINITY, l = 0.0f;
-    float acc[(D + 31) / 32] = {};
-
-    __device__ void add_range(const ChunkParams& p, const float* q, float scale, int s, int head, int t0, int t1) {
-        const int lane = threadIdx.x & 31;
-        for (int base = t0; base < t1; base += 32) {
-            const int t = base + lane;
-            float score = -INFINITY;
-            int page = -1;
-            if (t < t1) {
-                page = page_at(p, s, t);
-                score = 0.0f;
-                if (page >= 0) {
-                    const float4* k = reinterpret_cast<const float4*>(head_rows<D>(p, page, 0, head) +
-                                                                      (t % kPageTokens) * D);
-#pragma unroll 4
-                    for (int i = 0; i < D / 4; ++i) {  // q may be aligned to 4 bytes only
-                        const float4 a = k[i];
-                        score = fmaf(a.x, q[4 * i], fmaf(a.y, q[4 * i + 1],
-                                                         fmaf(a.z, q[4 * i + 2], fmaf(a.w, q[4 * i + 3], score))));
-                    }
-                    score *= scale;
-                }
-            }
-            float mx = score;
-            for (int o = 16; o; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-            mx = fmaxf(mx, m);
-            const float off = mx == -INFINITY ? 0.0f : mx;  // nothing but -inf so far
-            const float w = t < t1 ? expf(score - off) : 0.0f, r = expf(m - off);
-            m = mx;
-            float sum = w;
-            for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-            l = l * r + sum;
-#pragma unroll
-            for (int i = 0; i < (D + 31) / 32; ++i) acc[i] *= r;
-            const int n = min(32, t1 - base);
-            for (int j = 0; j < n; ++j) {
-                const int pg = __shfl_sync(0xffffffffu, page, j);
-                const float wj = __shfl_sync(0xffffffffu, w, j);
-                if (pg < 0) continue;
-                const float* v = head_rows<D>(p, pg, 1, head) + ((base + j) % kPageTokens) * D;
-#pragma unroll
-                for (int i = 0; i < (D + 31) / 32; ++i)
-                    if (lane + 32 * i < D) acc[i] = fmaf(wj, v[lane + 32 * i], acc[i]);
-            }
-        }
-    }
-};
 
 // ---------------------------------------------------------------------------
 // Tiles on the tensor cores.
@@ -163,7 +69,6 @@ struct Roles {
                   "registers");
     static_assert(kLoadWarp + kLoadWarps <= kThreads / 32, "warps");
 };
-constexpr int kChunkCtas = 148;   // most CTAs of a launch (the workspace's size)
 constexpr int kTileRows = 128;
 constexpr int kScaleRing = 8;     // tiles whose page scales are kept, at least two more than operand tiles
 // Barriers that free the operand tiles, more than there are tiles: a converter
@@ -202,13 +107,6 @@ struct Shape {
     static_assert(kQ + D <= 512, "tensor memory");
 };
 
-struct Unit {
-    int s, tile, head;
-    int first, n, len;  // the sequence's first row, rows and length
-    int limit;          // positions that the unit's last row sees
-    int tiles;          // of NT positions, at least one
-};
-
 struct ChunkBars {
     uint64_t slot_full[64], slot_empty[64];
     uint64_t k_full[3], v_full[3];
@@ -216,91 +114,6 @@ struct ChunkBars {
     uint64_t scales[kScaleRing];
     uint64_t s_full[2], p_full[2];
     uint64_t pv_done[2], q_full[kUnitRing], merge_full[4], merge_read[4], drained;
-};
-
-__device__ __forceinline__ int tokens_of_tile(int G) { return kTileRows / G; }
-
-template <int D>
-__device__ __forceinline__ void set_tile(const ChunkParams& p, Unit& u) {
-    const int per = tokens_of_tile(p.H / p.Hkv);
-    const int last = min((u.tile + 1) * per, u.n) - 1;
-    u.limit = min(max(u.len - u.n + last + 1, 0), p.stride * kPageTokens);
-    u.tiles = max(1, (u.limit + Shape<D>::NT - 1) / Shape<D>::NT);
-}
-__device__ __forceinline__ void set_sequence(const ChunkParams& p, Unit& u) {
-    rows_of(p, u.s, u.first, u.n);
-    u.len = p.total_lens[u.s];
-}
-template <int D>
-__device__ __forceinline__ void next_unit(const ChunkParams& p, Unit& u) {
-    if (++u.head < p.Hkv) return;
-    u.head = 0;
-    ++u.tile;
-    if (u.tile * tokens_of_tile(p.H / p.Hkv) >= u.n) {
-        u.tile = 0;
-        do {
-            ++u.s;
-            set_sequence(p, u);
-        } while (u.n == 0 && u.s + 1 < p.batch);
-    }
-    set_tile<D>(p, u);
-}
-// sum of floor((a i + b) / m) over i < n, for a, b >= 0 and m > 0 (Euclid's
-// algorithm on the lattice points under the line).
-__device__ __forceinline__ long long floor_sum(long long n, long long m, long long a, long long b) {
-    long long sum = 0;
-    while (n > 0) {
-        sum += (a / m) * (n * (n - 1) / 2) + (b / m) * n;
-        a %= m;
-        b %= m;
-        const long long top = a * n + b;
-        if (top < m) break;
-        n = top / m;
-        b = top % m;
-        const long long t = m;
-        m = a;
-        a = t;
-    }
-    return sum;
-}
-// Position tiles of the first `count` row tiles of u's sequence, for one head.
-template <int D>
-__device__ __forceinline__ long long tiles_before(const ChunkParams& p, Unit u, int count) {
-    constexpr int NT = Shape<D>::NT;
-    const int per = tokens_of_tile(p.H / p.Hkv), held = u.len - u.n, all = (u.n + per - 1) / per;
-    if (count > 4 && held >= 0 && u.len <= p.stride * kPageTokens) {
-        // ceil((held + (t + 1) per) / NT) each, but for the last row tile of the sequence
-        const int full = min(count, all - 1);
-        long long sum = floor_sum(full, NT, per, (long long)held + per + NT - 1);
-        if (count == all && all > 0) sum += (u.len + NT - 1) / NT;
-        return sum;
-    }
-    long long sum = 0;  // a few, or lengths that do not fit (reported): one by one
-    for (u.tile = 0; u.tile < count; ++u.tile) {
-        set_tile<D>(p, u);
-        sum += u.tiles;
-    }
-    return sum;
-}
-// Tiles of all units of a sequence.
-template <int D>
-__device__ __forceinline__ long long tiles_of_sequence(const ChunkParams& p, int s) {
-    Unit u;
-    u.s = s;
-    set_sequence(p, u);
-    const int per = tokens_of_tile(p.H / p.Hkv);
-    return tiles_before<D>(p, u, (u.n + per - 1) / per) * p.Hkv;
-}
-
-// What a CTA leaves for chunk_combine_kernel: its last unit, if that begins
-// here and goes on in the next `more` CTAs.
-struct ChunkSplit {
-    int s, tile, head, more;
-};
-// Partial sums of one unit in the workspace: O [128][D], then M and l [128].
-template <int D>
-struct Partial {
-    static constexpr size_t kFloats = (size_t)kTileRows * (D + 2);
 };
 
 // Operands made beforehand (chunk_operands_kernel): per sequence, KV head and
@@ -320,10 +133,7 @@ struct ChunkShared {
     ChunkBars bars;
     alignas(16) float scale[kScaleRing][16];  // of a tile's pages: K factors, then V exponents
     int slot_page[64];
-    Unit start;
-    int start_tile;
-    long long start_at;
-    long long scan[16];
+    ShareShared share;
     uint32_t tmem;
     float q_scale[kUnitRing][kTileRows];              // of the units' rows
     float merge_m[kTileRows], merge_l[kTileRows];     // the odd warpgroup's
@@ -333,40 +143,6 @@ struct ChunkShared {
     volatile int dead;  // a wait ran out: nobody waits any more
 };
 
-// Sleeps until the phase completes or a millisecond has passed.  Without the
-// hint the waiting warps poll, and took a third of the issue slots.
-__device__ __forceinline__ bool sleep_on(uint64_t* bar, uint32_t parity) {
-    uint32_t ok;
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
-        "selp.u32 %0, 1, 0, p;\n\t}"
-        : "=r"(ok)
-        : "r"(smem_u32(bar)), "r"(parity), "r"(1000000u)
-        : "memory");
-    return ok != 0;
-}
-__device__ __forceinline__ bool chunk_wait(ChunkShared& sh, uint64_t* bar, uint32_t parity, int* err) {
-    if (sleep_on(bar, parity)) return true;
-    const uint64_t t0 = global_timer_ns();
-    while (!sh.dead) {
-        if (sleep_on(bar, parity)) return true;
-        if (global_timer_ns() - t0 > kWaitLimitNs) {
-            record_error(err, kDevWaitTimeout);
-            sh.dead = 1;
-        }
-    }
-    return false;
-}
-// The same for several barriers at once: every lane with one of its own (bar not
-// null) waits for it, all return together.  With the roles' code spread over the
-// instruction cache a wait costs some 300 cycles even where nothing is missing.
-__device__ __forceinline__ void lanes_wait(ChunkShared& sh, uint64_t* bar, uint32_t parity, int* err) {
-    bool ok = !bar || sleep_on(bar, parity);
-    if (__all_sync(0xffffffffu, ok)) return;
-    if (!ok) chunk_wait(sh, bar, parity, err);
-    __syncwarp();
-}
 // What frees the operand tile that position tile i goes to: the product with its
 // last user, `stages` tiles before.
 __device__ __forceinline__ uint64_t* free_bar(uint64_t* ring, int i, int stages) {
@@ -374,7 +150,7 @@ __device__ __forceinline__ uint64_t* free_bar(uint64_t* ring, int i, int stages)
 }
 __device__ __forceinline__ uint32_t free_parity(int i, int stages) { return (uint32_t)((i - stages) / kEmptyRing & 1); }
 __device__ __forceinline__ void warp_wait(ChunkShared& sh, uint64_t* bar, uint32_t parity, int* err) {
-    if ((threadIdx.x & 31) == 0) chunk_wait(sh, bar, parity, err);
+    if ((threadIdx.x & 31) == 0) chunk_wait(&sh.dead, bar, parity, err);
     __syncwarp();
 }
 
@@ -510,28 +286,9 @@ __device__ __forceinline__ float load_queries(const ChunkParams& p, const float*
 // A unit's rows of one warp in fp32 (pages or queries without fp16 operands).
 template <int D>
 __device__ __noinline__ void rows_without_operands(const ChunkParams& p, const Unit& u, int t0, int t1, float* partial) {
-    const int G = p.H / p.Hkv, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    for (int r = warp * 32; r < warp * 32 + 32; ++r) {  // the even warpgroup's warps 0 to 3
-        const int token = u.tile * tokens_of_tile(G) + r / G;
-        if (r >= tokens_of_tile(G) * G || token >= u.n) break;
-        const int h = u.head * G + r % G;
-        const int sees = min(u.len - u.n + token + 1, u.limit);
-        RowSum<D> sum;
-        sum.add_range(p, p.q + (u.first + token) * p.ld_q + (size_t)h * D, rsqrtf((float)D), u.s, u.head, t0,
-                      min(t1, sees));
-        for (int i = 0; i < (D + 31) / 32; ++i) {
-            const int dim = lane + 32 * i;
-            if (dim >= D) continue;
-            if (partial)
-                partial[(size_t)r * D + dim] = sum.acc[i];
-            else
-                p.out[(u.first + token) * p.ld_out + (size_t)h * D + dim] = sees > 0 ? sum.acc[i] / sum.l : 0.0f;
-        }
-        if (partial && lane == 0) {
-            partial[kTileRows * D + r] = sum.m * 1.4426950408889634f + kPShift;
-            partial[kTileRows * (D + 1) + r] = sum.l;
-        }
-    }
+    const int first = (threadIdx.x >> 5) * 32;
+    for (int r = first; r < first + 32; ++r)  // the even warpgroup's warps 0 to 3
+        if (!row_in_fp32<D, kTileRows>(p, u, r, t0, t1, partial, kPShift)) break;
 }
 
 template <int D, bool PRE>
@@ -554,23 +311,6 @@ __global__ void __launch_bounds__(Roles<PRE>::kThreads, 1)
     uint8_t* pages = v_ops + kVStages * 2 * S::kHalf;
     ChunkBars& b = sh.bars;
 
-    // the CTA's share: tiles [total c / C, total (c + 1) / C) of all units'
-    // tiles; a thread counts those of a run of sequences
-    const int run = (p.batch + kChunkThreads - 1) / kChunkThreads;
-    const int s0 = min(tid * run, p.batch), s1 = min(s0 + run, p.batch);
-    long long mine = 0;
-    for (int s = s0; s < s1; ++s) {
-        mine += tiles_of_sequence<D>(p, s);
-        int first, n;
-        rows_of(p, s, first, n);
-        if (n && p.total_lens[s] > p.stride * kPageTokens) record_error(p.err, kDevBadPage);
-    }
-    long long incl = mine;
-    for (int o = 1; o < 32; o <<= 1) {
-        const long long t = __shfl_up_sync(0xffffffffu, incl, o);
-        if (lane >= o) incl += t;
-    }
-    if (lane == 31) sh.scan[warp] = incl;
     if (tid == 0) {
         sh.dead = 0;
         for (int i = 0; i < S::kSlots; ++i) {
@@ -600,70 +340,16 @@ __global__ void __launch_bounds__(Roles<PRE>::kThreads, 1)
         fence_barrier_init();
         fence_proxy_async_shared();
     }
-    __syncthreads();
-    long long before = incl - mine, total = 0;
-    for (int w = 0; w < kChunkThreads / 32; ++w) {
-        if (w < warp) before += sh.scan[w];
-        total += sh.scan[w];
-    }
-    const long long ctas = min((long long)gridDim.x, total), cta = blockIdx.x;  // every share has a tile
-    const long long begin = cta < ctas ? total * cta / ctas : 0, end = cta < ctas ? total * (cta + 1) / ctas : 0;
-    const int count = (int)(end - begin);
-    const int per_tile = tokens_of_tile(p.H / p.Hkv);
-    if (count > 0 && mine > 0 && before <= begin && begin < before + mine) {
-        Unit u;
-        long long at = begin - before;
-        for (u.s = s0; s1 - s0 > 1; ++u.s) {
-            const long long here = tiles_of_sequence<D>(p, u.s);
-            if (at < here) break;
-            at -= here;
-        }
-        set_sequence(p, u);
-        u.head = u.tile = 0;
-        sh.start = u;
-        sh.start_at = at;
-    }
-    __syncthreads();
-    if (count > 0) {  // its row tile: a run of row tiles a thread
-        Unit u = sh.start;
-        const int all = (u.n + per_tile - 1) / per_tile, each = (all + kChunkThreads - 1) / kChunkThreads;
-        const int t0 = min(tid * each, all), t1 = min(t0 + each, all);
-        long long here = 0;
-        for (u.tile = t0; u.tile < t1; ++u.tile) {
-            set_tile<D>(p, u);
-            here += (long long)u.tiles * p.Hkv;
-        }
-        long long upto = here;
-        if (all > each) {
-            for (int o = 1; o < 32; o <<= 1) {
-                const long long t = __shfl_up_sync(0xffffffffu, upto, o);
-                if (lane >= o) upto += t;
-            }
-            if (lane == 31) sh.scan[warp] = upto;
-            __syncthreads();
-            for (int w = 0; w < warp; ++w) upto += sh.scan[w];
-        }
-        long long at = sh.start_at - (upto - here);
-        __syncthreads();
-        if (here > 0 && at >= 0 && at < here) {
-            for (u.tile = t0;; ++u.tile) {
-                set_tile<D>(p, u);
-                if (at < (long long)u.tiles * p.Hkv) break;
-                at -= (long long)u.tiles * p.Hkv;
-            }
-            u.head = (int)(at / u.tiles);
-            sh.start = u;
-            sh.start_tile = (int)(at % u.tiles);
-        }
-    }
+    const Share share = find_share<NT, kTileRows, kChunkThreads>(p, sh.share);
+    const int count = share.count;
     if (warp == kIssueWarp) tmem_alloc(&sh.tmem, 512);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     pdl_launch_dependents();
     const uint32_t tmem = sh.tmem;
-    Unit u = sh.start;
-    int at = sh.start_tile;
+    Unit u = sh.share.start;
+    int at = sh.share.tile;
 
     // (a warpgroup's warps all move the same way, each in its own role)
     if (count > 0 && warp >= kLoadWarp && warp < kLoadWarp + R::kLoadWarps) {
@@ -679,23 +365,19 @@ __global__ void __launch_bounds__(Roles<PRE>::kThreads, 1)
                         const bool made = u.len <= pre.tiles * NT;  // a longer one goes without operands
                         const size_t t = made ? operand_tile<D>(p, pre, u.s, u.head, j) : 0;
                         const uint8_t* src = pre.ops + t * (4 * S::kHalf);
-                        if (i >= kKStages && !chunk_wait(sh, free_bar(b.k_empty, i, kKStages), free_parity(i, kKStages), p.err)) break;
+                        if (i >= kKStages && !chunk_wait(&sh.dead, free_bar(b.k_empty, i, kKStages), free_parity(i, kKStages), p.err)) break;
                         mbar_arrive_expect_tx(b.scales + ring, 64);
                         bulk_g2s(sh.scale[ring], pre.scales + t * 16, 64, b.scales + ring);
                         mbar_arrive_expect_tx(b.k_full + sk, 2 * S::kHalf);
                         bulk_g2s(k_ops + sk * 2 * S::kHalf, src, 2 * S::kHalf, b.k_full + sk);
-                        if (i >= kVStages && !chunk_wait(sh, free_bar(b.v_empty, i, kVStages), free_parity(i, kVStages), p.err)) break;
+                        if (i >= kVStages && !chunk_wait(&sh.dead, free_bar(b.v_empty, i, kVStages), free_parity(i, kVStages), p.err)) break;
                         mbar_arrive_expect_tx(b.v_full + sv, 2 * S::kHalf);
                         bulk_g2s(v_ops + sv * 2 * S::kHalf, src + 2 * S::kHalf, 2 * S::kHalf, b.v_full + sv);
                     }
                     left -= take;
-                    if (left > 0) next_unit<D>(p, u);
+                    if (left > 0) next_unit<NT, kTileRows>(p, u);
                 }
-                if (sh.dead) {  // copies still in flight must land before the CTA ends: a second is ample
-                    const uint64_t t0 = global_timer_ns();
-                    while (global_timer_ns() - t0 < kWaitLimitNs / 2) {
-                    }
-                }
+                if (sh.dead) land_copies();
             }
             __syncwarp();
         } else {
@@ -704,7 +386,7 @@ __global__ void __launch_bounds__(Roles<PRE>::kThreads, 1)
         // lanes' branches take longer than the copies, and a whole tile would wait
         // for its last slot.
         const int kv = warp - kLoadWarp;
-        int jobs = 0, slot = kv * PG + lane, fill = 0;  // the lane's page slot, and its fills before
+        int slot = kv * PG + lane, fill = 0;  // the lane's page slot, and its fills before
         const bool mine = lane < PG;
         const auto entry = [&](int j) {
             const int pos = j * NT + lane * kPageTokens;
@@ -716,7 +398,7 @@ __global__ void __launch_bounds__(Roles<PRE>::kThreads, 1)
             const float* src = head_rows<D>(p, max(id, 0), kv, u.head);
             if (--left > 0) {
                 if (++j == end_j) {
-                    next_unit<D>(p, u);
+                    next_unit<NT, kTileRows>(p, u);
                     j = 0;
                     end_j = min(u.tiles, left);
                 }
@@ -725,7 +407,7 @@ __global__ void __launch_bounds__(Roles<PRE>::kThreads, 1)
 #pragma unroll 1
             for (int g = 0; g < PG; g += 4) {
                 const bool turn = lane >= g && lane < g + 4;
-                lanes_wait(sh, turn ? b.slot_empty + slot : nullptr, (uint32_t)(fill & 1) ^ 1, p.err);
+                lanes_wait(&sh.dead, turn ? b.slot_empty + slot : nullptr, (uint32_t)(fill & 1) ^ 1, p.err);
                 if (turn && !sh.dead) {
                     sh.slot_page[slot] = id;
                     mbar_arrive_expect_tx(b.slot_full + slot, id >= 0 ? S::kPageBytes : 0);
@@ -738,17 +420,8 @@ __global__ void __launch_bounds__(Roles<PRE>::kThreads, 1)
                 slot -= S::kSlots;
                 ++fill;
             }
-            jobs += 2 * PG;
         }
-        if (sh.dead) {  // copies still in flight must land before the CTA ends
-            const uint64_t t0 = global_timer_ns();
-            for (int s = lane; s < S::kSlots; s += 32) {  // (a slot of the other producer's counts too)
-                const int fills = jobs > s ? (jobs - 1 - s) / S::kSlots + 1 : 0;
-                while (fills && !mbar_try_wait(b.slot_full + s, (uint32_t)(fills - 1) & 1) &&
-                       global_timer_ns() - t0 < kWaitLimitNs) {
-                }
-            }
-        }
+        if (sh.dead) land_copies();
         }
     } else if (count > 0 && warp == kIssueWarp) {
         // ---- issuer ----
@@ -758,8 +431,8 @@ __global__ void __launch_bounds__(Roles<PRE>::kThreads, 1)
             int i = 0, unit = 0;
             const auto issue_s = [&](int item, bool first, int un) {
                 const int st = item % kKStages;
-                if (first) chunk_wait(sh, b.q_full + un % kUnitRing, (uint32_t)(un / kUnitRing & 1), p.err);
-                chunk_wait(sh, b.k_full + st, (uint32_t)(item / kKStages & 1), p.err);
+                if (first) chunk_wait(&sh.dead, b.q_full + un % kUnitRing, (uint32_t)(un / kUnitRing & 1), p.err);
+                chunk_wait(&sh.dead, b.k_full + st, (uint32_t)(item / kKStages & 1), p.err);
                 tc_fence_after();
                 const uint32_t kb = k0 + st * 2 * S::kHalf;
                 tc_mma_split<NT, D>(tmem + S::kS + (uint32_t)(item & 1) * NT, tmem + S::kQ,
@@ -773,8 +446,8 @@ __global__ void __launch_bounds__(Roles<PRE>::kThreads, 1)
                 for (int j = 0; j < take; ++j, ++i) {
                     if (j + 1 < take) issue_s(i + 1, false, unit);
                     const int st = i % kVStages;
-                    chunk_wait(sh, b.v_full + st, (uint32_t)(i / kVStages & 1), p.err);
-                    chunk_wait(sh, b.p_full + (i & 1), (uint32_t)(i / 2 & 1), p.err);
+                    chunk_wait(&sh.dead, b.v_full + st, (uint32_t)(i / kVStages & 1), p.err);
+                    chunk_wait(&sh.dead, b.p_full + (i & 1), (uint32_t)(i / 2 & 1), p.err);
                     tc_fence_after();
                     const uint32_t vb = v0 + st * 2 * S::kHalf;
                     // P: 16 columns of high, 16 of low halves per 32 positions.  O of two
@@ -786,7 +459,7 @@ __global__ void __launch_bounds__(Roles<PRE>::kThreads, 1)
                 }
                 left -= take;
                 ++unit;
-                if (left > 0) next_unit<D>(p, u);
+                if (left > 0) next_unit<NT, kTileRows>(p, u);
             }
             // every product has been read and written before tensor memory goes
             tc_commit(&b.drained);
@@ -814,7 +487,7 @@ __global__ void __launch_bounds__(Roles<PRE>::kThreads, 1)
                     const int slot = (job + kv * PG) % S::kSlots, fill = (job + kv * PG) / S::kSlots;
                     const int st = kv ? i % kVStages : i % kKStages, stages = kv ? kVStages : kKStages;
                     // lane 0: the page, lane 1: its place in the operand tile
-                    lanes_wait(sh,
+                    lanes_wait(&sh.dead,
                                lane == 0   ? b.slot_full + slot
                                : lane == 1 ? free_bar(kv ? b.v_empty : b.k_empty, i, stages)
                                            : nullptr,
@@ -835,14 +508,14 @@ __global__ void __launch_bounds__(Roles<PRE>::kThreads, 1)
                 }
             }
             left -= take;
-            if (left > 0) next_unit<D>(p, u);
+            if (left > 0) next_unit<NT, kTileRows>(p, u);
         }
     } else if (count > 0 && warp < kSoftmaxWarps) {
         // ---- softmax: of two warpgroups each takes the tiles of its parity ----
         set_registers_up<kSoftmaxRegs>();
         const int group = warp >> 2, quad = warp & 3;
         const uint32_t lanes = (uint32_t)(quad * 32) << 16;
-        const int G = p.H / p.Hkv, per = tokens_of_tile(G);
+        const int G = p.H / p.Hkv, per = (kTileRows / G);
         const uint32_t s0_addr = tmem + S::kS + lanes, o0_addr = tmem + S::kO + lanes;
         ChunkSplit split{0, 0, 0, -1};
         // A unit of at most 32 rows would leave three of a warpgroup's four warps
@@ -916,7 +589,7 @@ __global__ void __launch_bounds__(Roles<PRE>::kThreads, 1)
             for (i = first; i < i0 + take; i += kGroups) {
                 const uint32_t ts = s0_addr + (uint32_t)(i & 1) * NT;
                 const int j = at + (i - i0), ring = i % kScaleRing;
-                lanes_wait(sh, lane == 0 ? b.scales + ring : lane == 1 ? b.s_full + (i & 1) : nullptr,
+                lanes_wait(&sh.dead, lane == 0 ? b.scales + ring : lane == 1 ? b.s_full + (i & 1) : nullptr,
                            (uint32_t)(lane == 0 ? i / kScaleRing : i / 2) & 1, p.err);
                 tc_fence_after();
                 if (busy) {
@@ -1041,7 +714,7 @@ __global__ void __launch_bounds__(Roles<PRE>::kThreads, 1)
             left -= take;
             at = 0;
             if (left > 0) {
-                next_unit<D>(p, u);
+                next_unit<NT, kTileRows>(p, u);
                 // the warpgroup of the unit's last tile knows that its queries are read
                 if (kGroups == 1 || ((i - 1) & 1) == group) queries(u, unit + 1);
             }
@@ -1076,12 +749,10 @@ __global__ void __launch_bounds__(Roles<PRE>::kThreads, 1)
             const bool whole = from == 0 && take == done.tiles;
             float* part = nullptr;
             if (!whole) {
-                part = partials + ((size_t)blockIdx.x * 2 + (from == 0)) * Partial<D>::kFloats;
+                part = partials + ((size_t)blockIdx.x * 2 + (from == 0)) * partial_floats(kTileRows, D);
                 if (from == 0) {  // goes on in the next CTAs: up to the one that holds its last tile
-                    const long long last = end + (done.tiles - take) - 1;
-                    int more = 0;
-                    while (total * (cta + more + 2) / ctas <= last) ++more;
-                    split = ChunkSplit{done.s, done.tile, done.head, more + 1};
+                    const int more = share.followers(done.tiles - take);
+                    split = ChunkSplit{done.s, done.tile, done.head, more};
                 }
             }
             float w0 = 1.0f, w1 = 0.0f;
@@ -1202,60 +873,6 @@ __global__ void __launch_bounds__(Roles<PRE>::kThreads, 1)
     }
 }
 
-// Block (c, y): 16 rows of the unit that begins in CTA c and goes on in the
-// next ones.  A warp a row forms the parts' weights, then the threads sum.
-constexpr int kCombineThreads = 256, kCombineRows = 16;
-template <int D>
-__global__ void __launch_bounds__(kCombineThreads) chunk_combine_kernel(ChunkParams p, const float* partials,
-                                                                         const ChunkSplit* splits) {
-    __shared__ float weight[kCombineRows][kChunkCtas], norm[kCombineRows];
-    pdl_wait();
-    const ChunkSplit s = splits[blockIdx.x];
-    if (s.more < 0) return;
-    Unit u;
-    u.s = s.s, u.tile = s.tile, u.head = s.head;
-    set_sequence(p, u);
-    const int G = p.H / p.Hkv, per = tokens_of_tile(G), r0 = blockIdx.y * kCombineRows;
-    const int rows = min(min(per, u.n - u.tile * per) * G - r0, kCombineRows);
-    if (rows <= 0) return;
-    const auto part = [&](int k) {
-        return partials + ((size_t)(blockIdx.x + k) * 2 + (k == 0)) * Partial<D>::kFloats;
-    };
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    for (int r = warp; r < rows; r += kCombineThreads / 32) {
-        float top = -INFINITY, l = 0.0f;
-        for (int k = lane; k <= s.more; k += 32) top = fmaxf(top, part(k)[kTileRows * D + r0 + r]);
-        for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-        const float off = top == -INFINITY ? 0.0f : top;
-        for (int k = lane; k <= s.more; k += 32) {
-            const float w = exp2f(part(k)[kTileRows * D + r0 + r] - off);
-            weight[r][k] = w;
-            l = fmaf(w, part(k)[kTileRows * (D + 1) + r0 + r], l);
-        }
-        for (int o = 16; o; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
-        const int token = u.tile * per + (r0 + r) / G;
-        if (lane == 0) norm[r] = u.len - u.n + token >= 0 ? 1.0f / l : 0.0f;
-    }
-    __syncthreads();
-    for (int e = threadIdx.x; e < rows * (D / 4); e += kCombineThreads) {
-        const int r = e / (D / 4), d4 = e % (D / 4) * 4, token = u.tile * per + (r0 + r) / G;
-        float4 o = make_float4(0, 0, 0, 0);
-#pragma unroll 4
-        for (int k = 0; k <= s.more; ++k) {
-            const float4 x = *reinterpret_cast<const float4*>(part(k) + (size_t)(r0 + r) * D + d4);
-            const float w = weight[r][k];
-            o.x = fmaf(w, x.x, o.x), o.y = fmaf(w, x.y, o.y), o.z = fmaf(w, x.z, o.z), o.w = fmaf(w, x.w, o.w);
-        }
-        float* dst = p.out + (u.first + token) * p.ld_out + (size_t)(u.head * G + (r0 + r) % G) * D + d4;
-        const float inv = norm[r];
-        const bool none = inv == 0.0f && u.len - u.n + token < 0;  // zeros, whatever the parts hold
-        dst[0] = none ? 0.0f : o.x * inv;
-        dst[1] = none ? 0.0f : o.y * inv;
-        dst[2] = none ? 0.0f : o.z * inv;
-        dst[3] = none ? 0.0f : o.w * inv;
-    }
-}
-
 // Operands of one tile of one KV head: a CTA of 8 warps, one or two pages each.
 constexpr int kOperandThreads = 256;
 template <int D>
@@ -1304,29 +921,40 @@ __global__ void __launch_bounds__(kOperandThreads) chunk_operands_kernel(ChunkPa
     for (int i = threadIdx.x; i < 4 * S::kHalf / 16; i += kOperandThreads) to[i] = from[i];
 }
 
-// The launch for a call's bounds, and its workspace: partial sums, what is
+// The launches for a call's bounds, and their workspace: partial sums, what is
 // split, and the operands where they are made beforehand.
 struct ChunkPlan {
-    int ctas;           // one per tile of work that the bounds allow, at most one per SM
-    int operand_tiles;  // of a sequence, 0: converted by the CTAs that read them
-    size_t splits, operands, scales, bytes;  // offsets, and all of it
+    int ctas, few_ctas;  // one per tile of work that the bounds allow, at most one per SM; 0: not launched
+    int operand_tiles;   // of a sequence, 0: converted by the CTAs that read them
+    size_t splits, few, few_splits, operands, scales, bytes;  // offsets, and all of it
 };
 ChunkPlan chunk_plan(long long rows, long long batch, long long max_new, long long max_len, int H, int Hkv, int d) {
     const long long G = H / Hkv, per = kTileRows / G, nt = d == 128 ? 64 : 128, len_tiles = (max_len + nt - 1) / nt;
-    const long long row_tiles = std::min(batch * ((std::min(max_new, rows) + per - 1) / per), batch + rows / per);
-    ChunkPlan c{};
     const auto most = [](long long n) { return std::min<long long>(n, kChunkCtas); };
-    c.ctas = (int)std::max<long long>(1, most(most(row_tiles) * most(Hkv) * most(len_tiles)));
+    const auto ctas = [&](long long tokens) {  // for units of so many tokens
+        const long long units = std::min(batch * ((std::min(max_new, rows) + tokens - 1) / tokens), batch + rows / tokens);
+        return (int)std::max<long long>(1, most(most(units) * most(Hkv) * most(len_tiles)));
+    };
+    ChunkPlan c{};
+    // Sequences with at most eight rows of a KV head go to chunk_few_kernel.  Where
+    // the bounds say that all have so few it takes them all, where they say that
+    // the one sequence has more the tensor-core kernel does; else each takes its own.
+    const bool few = G <= kFewRows && (max_new * G <= kFewRows || batch > 1);
+    const bool many = !few || max_new * G > kFewRows;
+    if (few) c.few_ctas = ctas(kFewRows / G);
+    if (many) c.ctas = ctas(per);
     // Made beforehand where every K and V tile is read by kPreReuse row tiles or
     // more (as far as the bounds tell) and the operands fit kPreBytes.
     constexpr long long kPreReuse = 8, kPreBytes = 1ll << 30;
     const long long tile_bytes = 8 * nt * d + 64;
     const bool fits = batch <= 65535 && len_tiles <= (1 << 24) && batch * Hkv * len_tiles <= kPreBytes / tile_bytes;
-    if (fits && rows / per >= kPreReuse * batch) c.operand_tiles = (int)len_tiles;
+    if (many && fits && rows / per >= kPreReuse * batch) c.operand_tiles = (int)len_tiles;
     const long long all_tiles = batch * Hkv * c.operand_tiles;
     const auto up = [](size_t n) { return (n + 127) & ~(size_t)127; };
-    c.splits = (size_t)c.ctas * 2 * kTileRows * (d + 2) * sizeof(float);
-    c.operands = up(c.splits + (size_t)c.ctas * sizeof(ChunkSplit));
+    c.splits = c.ctas * 2 * partial_floats(kTileRows, d) * sizeof(float);
+    c.few = up(c.splits + c.ctas * sizeof(ChunkSplit));
+    c.few_splits = c.few + c.few_ctas * 2 * partial_floats(kFewRows, d) * sizeof(float);
+    c.operands = up(c.few_splits + c.few_ctas * sizeof(ChunkSplit));
     c.scales = c.operands + (size_t)all_tiles * 8 * nt * d;
     c.bytes = c.scales + (size_t)all_tiles * 64;
     return c;
@@ -1355,12 +983,25 @@ cudaError_t launch_tiles(const ChunkParams& p, const ChunkPlan& plan, float* par
 }
 
 template <int D>
-cudaError_t launch_chunk(const ChunkParams& p, const ChunkPlan& plan, void* workspace, cudaStream_t stream) {
+cudaError_t launch_chunk(ChunkParams p, const ChunkPlan& plan, void* workspace, cudaStream_t stream) {
     uint8_t* w = static_cast<uint8_t*>(workspace);
+    cudaError_t e = cudaSuccess;
+    if (plan.few_ctas) {
+        float* partials = reinterpret_cast<float*>(w + plan.few);
+        ChunkSplit* splits = reinterpret_cast<ChunkSplit*>(w + plan.few_splits);
+        p.rows_upto = plan.ctas ? kFewRows : INT_MAX;
+        e = chunk_kernel_attributes(chunk_few_kernel<D>, Few<D>::kSmem, 0);
+        if (e != cudaSuccess) return e;
+        chunk_few_kernel<D><<<plan.few_ctas, Few<D>::kThreads, Few<D>::kSmem, stream>>>(p, partials, splits);
+        e = cudaGetLastError();
+        if (e == cudaSuccess) e = launch_combine<D, Few<D>::NT, kFewRows>(p, plan.few_ctas, partials, splits, stream);
+        p.rows_above = kFewRows;
+        p.rows_upto = INT_MAX;
+    }
+    if (e != cudaSuccess || !plan.ctas) return e;
     float* partials = reinterpret_cast<float*>(w);
     ChunkSplit* splits = reinterpret_cast<ChunkSplit*>(w + plan.splits);
     const Operands pre{w + plan.operands, reinterpret_cast<float*>(w + plan.scales), plan.operand_tiles};
-    cudaError_t e;
     if (plan.operand_tiles) {
         const size_t smem = 4 * Shape<D>::kHalf + (kOperandThreads / 32) * Shape<D>::kPageBytes;
         e = chunk_kernel_attributes(chunk_operands_kernel<D>, smem, 0);
@@ -1373,16 +1014,7 @@ cudaError_t launch_chunk(const ChunkParams& p, const ChunkPlan& plan, void* work
         e = launch_tiles<D, false>(p, plan, partials, splits, pre, stream);
     }
     if (e != cudaSuccess) return e;
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3((unsigned)plan.ctas, kTileRows / kCombineRows);
-    cfg.blockDim = dim3(kCombineThreads);
-    cfg.stream = stream;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, chunk_combine_kernel<D>, p, (const float*)partials, (const ChunkSplit*)splits);
+    return launch_combine<D, Shape<D>::NT, kTileRows>(p, plan.ctas, partials, splits, stream);
 }
 
 }  // namespace
@@ -1432,7 +1064,7 @@ extern "C" tb_status tb_paged_attention_chunk_dev(void* stream, const float* q, 
     StreamEntry entry(pool, "kv_pool");
     if (entry.status != TB_OK) return entry.status;
     ChunkParams p{q, ld_q, row_offsets, total_lens, batch, rows, pool, num_pages, table, stride, layer, num_layers, H,
-                  Hkv, out, ld_out, entry.err};
+                  Hkv, 0, INT_MAX, out, ld_out, entry.err};
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     cudaError_t e = d == 16   ? launch_chunk<16>(p, plan, workspace, s)
                     : d == 32 ? launch_chunk<32>(p, plan, workspace, s)

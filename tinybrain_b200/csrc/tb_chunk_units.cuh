@@ -1,0 +1,440 @@
+// tb_chunk_units.cuh -- what the kernels of the chunk attention (tb_chunk.cu,
+// tb_chunk_few.cu) share: the call's parameters, its division into units and
+// into equal shares of the CTAs, the partial sums of units that several CTAs
+// hold, and one row in plain fp32.
+#pragma once
+
+#include <climits>
+
+#include "tb_common.cuh"
+#include "tb_stream_entry.h"
+
+namespace tb {
+
+struct ChunkParams {
+    const float* q;
+    long long ld_q;
+    const int* row_offsets;
+    const int* total_lens;
+    int batch, rows;
+    const float* pool;
+    int num_pages;
+    const int* table;
+    int stride;
+    int layer, num_layers, H, Hkv;
+    int rows_above, rows_upto;  // the kernel's sequences: those with more and at most so many rows of a KV head
+    float* out;
+    long long ld_out;
+    int* err;
+};
+
+// The rows of sequence s that the call holds (none where another kernel has them).
+__device__ __forceinline__ void rows_of(const ChunkParams& p, int s, int& first, int& count) {
+    first = min(max(p.row_offsets[s], 0), p.rows);
+    count = max(min(p.row_offsets[s + 1], p.rows) - first, 0);
+    const long long of_head = (long long)count * (p.H / p.Hkv);
+    if (of_head <= p.rows_above || of_head > p.rows_upto) count = 0;
+}
+
+// Pool page of a table entry, -1 where there is none (evicted, or reported as bad).
+__device__ __forceinline__ int checked_page(const ChunkParams& p, int page) {
+    if (page >= p.num_pages) {
+        record_error(p.err, kDevBadPage);
+        return -1;
+    }
+    return page;
+}
+__device__ __forceinline__ int page_at(const ChunkParams& p, int s, int pos) {
+    return checked_page(p, p.table[(size_t)s * p.stride + pos / kPageTokens]);
+}
+
+template <int D>
+__device__ __forceinline__ const float* head_rows(const ChunkParams& p, int page, int kv, int head) {
+    return p.pool + ((((size_t)page * p.num_layers + p.layer) * 2 + kv) * p.Hkv + head) * (size_t)(kPageTokens * D);
+}
+
+// One query row of one head over positions [t0, t1) by one warp: lane = token
+// for the scores, lane = dim for the sums; fp32 throughout.
+template <int D>
+struct RowSum {
+    float m = -INFINITY, l = 0.0f;
+    float acc[(D + 31) / 32] = {};
+
+    __device__ void add_range(const ChunkParams& p, const float* q, float scale, int s, int head, int t0, int t1) {
+        const int lane = threadIdx.x & 31;
+        for (int base = t0; base < t1; base += 32) {
+            const int t = base + lane;
+            float score = -INFINITY;
+            int page = -1;
+            if (t < t1) {
+                page = page_at(p, s, t);
+                score = 0.0f;
+                if (page >= 0) {
+                    const float4* k = reinterpret_cast<const float4*>(head_rows<D>(p, page, 0, head) +
+                                                                      (t % kPageTokens) * D);
+#pragma unroll 4
+                    for (int i = 0; i < D / 4; ++i) {  // q may be aligned to 4 bytes only
+                        const float4 a = k[i];
+                        score = fmaf(a.x, q[4 * i], fmaf(a.y, q[4 * i + 1],
+                                                         fmaf(a.z, q[4 * i + 2], fmaf(a.w, q[4 * i + 3], score))));
+                    }
+                    score *= scale;
+                }
+            }
+            float mx = score;
+            for (int o = 16; o; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+            mx = fmaxf(mx, m);
+            const float off = mx == -INFINITY ? 0.0f : mx;  // nothing but -inf so far
+            const float w = t < t1 ? expf(score - off) : 0.0f, r = expf(m - off);
+            m = mx;
+            float sum = w;
+            for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+            l = l * r + sum;
+#pragma unroll
+            for (int i = 0; i < (D + 31) / 32; ++i) acc[i] *= r;
+            const int n = min(32, t1 - base);
+            for (int j = 0; j < n; ++j) {
+                const int pg = __shfl_sync(0xffffffffu, page, j);
+                const float wj = __shfl_sync(0xffffffffu, w, j);
+                if (pg < 0) continue;
+                const float* v = head_rows<D>(p, pg, 1, head) + ((base + j) % kPageTokens) * D;
+#pragma unroll
+                for (int i = 0; i < (D + 31) / 32; ++i)
+                    if (lane + 32 * i < D) acc[i] = fmaf(wj, v[lane + 32 * i], acc[i]);
+            }
+        }
+    }
+};
+
+constexpr int kChunkCtas = 148; // most CTAs of a launch (the workspace's size)
+
+// Sleeps until the phase completes or a millisecond has passed.  Without the
+// hint the waiting warps poll, and took a third of the issue slots.
+__device__ __forceinline__ bool sleep_on(uint64_t* bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(smem_u32(bar)), "r"(parity), "r"(1000000u)
+        : "memory");
+    return ok != 0;
+}
+// A wait that runs out sets *dead, after which nobody in the CTA waits any more.
+__device__ __forceinline__ bool chunk_wait(volatile int* dead, uint64_t* bar, uint32_t parity, int* err) {
+    if (sleep_on(bar, parity)) return true;
+    const uint64_t t0 = global_timer_ns();
+    while (!*dead) {
+        if (sleep_on(bar, parity)) return true;
+        if (global_timer_ns() - t0 > kWaitLimitNs) {
+            record_error(err, kDevWaitTimeout);
+            *dead = 1;
+        }
+    }
+    return false;
+}
+// After a wait that ran out: time for the CTA's copies in flight to land (they
+// take microseconds) before it ends.
+__device__ __forceinline__ void land_copies() {
+    const uint64_t t0 = global_timer_ns();
+    while (global_timer_ns() - t0 < 50000000ull) {
+    }
+}
+// The same for several barriers at once: every lane with one of its own (bar not
+// null) waits for it, all return together.  With the roles' code spread over the
+// instruction cache a wait costs some 300 cycles even where nothing is missing.
+__device__ __forceinline__ void lanes_wait(volatile int* dead, uint64_t* bar, uint32_t parity, int* err) {
+    bool ok = !bar || sleep_on(bar, parity);
+    if (__all_sync(0xffffffffu, ok)) return;
+    if (!ok) chunk_wait(dead, bar, parity, err);
+    __syncwarp();
+}
+// A unit: ROWS query rows of one KV head (the G = H / Hkv query heads of ROWS / G
+// consecutive tokens) over the positions they see, in tiles of NT positions.
+struct Unit {
+    int s, tile, head;
+    int first, n, len;  // the sequence's first row, rows and length
+    int limit;          // positions that the unit's last row sees
+    int tiles;          // of NT positions, at least one
+};
+
+template <int NT, int ROWS>
+__device__ __forceinline__ void set_tile(const ChunkParams& p, Unit& u) {
+    const int per = ROWS / (p.H / p.Hkv);
+    const int last = min((u.tile + 1) * per, u.n) - 1;
+    u.limit = min(max(u.len - u.n + last + 1, 0), p.stride * kPageTokens);
+    u.tiles = max(1, (u.limit + NT - 1) / NT);
+}
+__device__ __forceinline__ void set_sequence(const ChunkParams& p, Unit& u) {
+    rows_of(p, u.s, u.first, u.n);
+    u.len = p.total_lens[u.s];
+}
+template <int NT, int ROWS>
+__device__ __forceinline__ void next_unit(const ChunkParams& p, Unit& u) {
+    if (++u.head < p.Hkv) return;
+    u.head = 0;
+    ++u.tile;
+    if (u.tile * ROWS / (p.H / p.Hkv) >= u.n) {
+        u.tile = 0;
+        do {
+            ++u.s;
+            set_sequence(p, u);
+        } while (u.n == 0 && u.s + 1 < p.batch);
+    }
+    set_tile<NT, ROWS>(p, u);
+}
+// sum of floor((a i + b) / m) over i < n, for a, b >= 0 and m > 0 (Euclid's
+// algorithm on the lattice points under the line).
+__device__ __forceinline__ long long floor_sum(long long n, long long m, long long a, long long b) {
+    long long sum = 0;
+    while (n > 0) {
+        sum += (a / m) * (n * (n - 1) / 2) + (b / m) * n;
+        a %= m;
+        b %= m;
+        const long long top = a * n + b;
+        if (top < m) break;
+        n = top / m;
+        b = top % m;
+        const long long t = m;
+        m = a;
+        a = t;
+    }
+    return sum;
+}
+// Position tiles of the first `count` row tiles of u's sequence, for one head.
+template <int NT, int ROWS>
+__device__ __forceinline__ long long tiles_before(const ChunkParams& p, Unit u, int count) {
+    const int per = ROWS / (p.H / p.Hkv), held = u.len - u.n, all = (u.n + per - 1) / per;
+    if (count > 4 && held >= 0 && u.len <= p.stride * kPageTokens) {
+        // ceil((held + (t + 1) per) / NT) each, but for the last row tile of the sequence
+        const int full = min(count, all - 1);
+        long long sum = floor_sum(full, NT, per, (long long)held + per + NT - 1);
+        if (count == all && all > 0) sum += (u.len + NT - 1) / NT;
+        return sum;
+    }
+    long long sum = 0;  // a few, or lengths that do not fit (reported): one by one
+    for (u.tile = 0; u.tile < count; ++u.tile) {
+        set_tile<NT, ROWS>(p, u);
+        sum += u.tiles;
+    }
+    return sum;
+}
+// Tiles of all units of a sequence.
+template <int NT, int ROWS>
+__device__ __forceinline__ long long tiles_of_sequence(const ChunkParams& p, int s) {
+    Unit u;
+    u.s = s;
+    set_sequence(p, u);
+    const int per = ROWS / (p.H / p.Hkv);
+    return tiles_before<NT, ROWS>(p, u, (u.n + per - 1) / per) * p.Hkv;
+}
+
+// What a CTA leaves for chunk_combine_kernel: its last unit, if that begins
+// here and goes on in the next `more` CTAs.
+struct ChunkSplit {
+    int s, tile, head, more;
+};
+// Partial sums of one unit in the workspace: O [rows][D], then M and l [rows].
+__host__ __device__ constexpr size_t partial_floats(int rows, int d) { return (size_t)rows * (d + 2); }
+
+// A CTA's share: tiles [total c / C, total (c + 1) / C) of all units' tiles, one
+// unit after the other.  A ragged batch, one long sequence and a large prompt
+// thus load the SMs evenly without a plan made on the host.
+struct Share {
+    long long total, ctas, end;
+    int count;
+    // CTAs after this one that hold the `left` tiles after its last
+    __device__ __forceinline__ int followers(int left) const {
+        const long long last = end + left - 1;
+        int n = 1;
+        while (total * (blockIdx.x + n + 1) / ctas <= last) ++n;
+        return n;
+    }
+};
+struct ShareShared {
+    long long scan[32], at;
+    Unit start;  // the share's first unit
+    int tile;    // and its first tile of that
+};
+// Every CTA counts for itself: a thread takes a run of sequences, then a run of
+// the row tiles of the sequence that the share begins in.  sh.start and sh.tile
+// may be read after the caller's next barrier.
+template <int NT, int ROWS, int THREADS>
+__device__ __forceinline__ Share find_share(const ChunkParams& p, ShareShared& sh) {
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int run = (p.batch + THREADS - 1) / THREADS;
+    const int s0 = min(tid * run, p.batch), s1 = min(s0 + run, p.batch);
+    long long mine = 0;
+    for (int s = s0; s < s1; ++s) {
+        mine += tiles_of_sequence<NT, ROWS>(p, s);
+        int first, n;
+        rows_of(p, s, first, n);
+        if (n && p.total_lens[s] > p.stride * kPageTokens) record_error(p.err, kDevBadPage);
+    }
+    long long incl = mine;
+    for (int o = 1; o < 32; o <<= 1) {
+        const long long t = __shfl_up_sync(0xffffffffu, incl, o);
+        if (lane >= o) incl += t;
+    }
+    if (lane == 31) sh.scan[warp] = incl;
+    __syncthreads();
+    Share share;
+    long long before = incl - mine;
+    share.total = 0;
+    for (int w = 0; w < THREADS / 32; ++w) {
+        if (w < warp) before += sh.scan[w];
+        share.total += sh.scan[w];
+    }
+    const long long cta = blockIdx.x;
+    share.ctas = min((long long)gridDim.x, share.total);  // every share has a tile
+    const long long begin = cta < share.ctas ? share.total * cta / share.ctas : 0;
+    share.end = cta < share.ctas ? share.total * (cta + 1) / share.ctas : 0;
+    share.count = (int)(share.end - begin);
+    if (share.count > 0 && mine > 0 && before <= begin && begin < before + mine) {
+        Unit u;
+        long long at = begin - before;
+        for (u.s = s0; s1 - s0 > 1; ++u.s) {
+            const long long here = tiles_of_sequence<NT, ROWS>(p, u.s);
+            if (at < here) break;
+            at -= here;
+        }
+        set_sequence(p, u);
+        u.head = u.tile = 0;
+        sh.start = u;
+        sh.at = at;
+    }
+    __syncthreads();
+    if (share.count > 0) {
+        Unit u = sh.start;
+        const int per = ROWS / (p.H / p.Hkv), all = (u.n + per - 1) / per, each = (all + THREADS - 1) / THREADS;
+        const int t0 = min(tid * each, all), t1 = min(t0 + each, all);
+        long long here = 0;
+        for (u.tile = t0; u.tile < t1; ++u.tile) {
+            set_tile<NT, ROWS>(p, u);
+            here += (long long)u.tiles * p.Hkv;
+        }
+        long long upto = here;
+        if (all > each) {
+            for (int o = 1; o < 32; o <<= 1) {
+                const long long t = __shfl_up_sync(0xffffffffu, upto, o);
+                if (lane >= o) upto += t;
+            }
+            if (lane == 31) sh.scan[warp] = upto;
+            __syncthreads();
+            for (int w = 0; w < warp; ++w) upto += sh.scan[w];
+        }
+        long long at = sh.at - (upto - here);
+        __syncthreads();
+        if (here > 0 && at >= 0 && at < here) {
+            for (u.tile = t0;; ++u.tile) {
+                set_tile<NT, ROWS>(p, u);
+                if (at < (long long)u.tiles * p.Hkv) break;
+                at -= (long long)u.tiles * p.Hkv;
+            }
+            u.head = (int)(at / u.tiles);
+            sh.start = u;
+            sh.tile = (int)(at % u.tiles);
+        }
+    }
+    return share;
+}
+
+// Row r of a unit over positions [t0, t1) in fp32 by one warp, to the output or
+// to the unit's partial sums (whose weights carry 2^shift).  false: the unit has
+// no such row.
+template <int D, int ROWS>
+__device__ bool row_in_fp32(const ChunkParams& p, const Unit& u, int r, int t0, int t1, float* partial, float shift) {
+    const int G = p.H / p.Hkv, per = ROWS / G, lane = threadIdx.x & 31, token = u.tile * per + r / G;
+    if (r >= per * G || token >= u.n) return false;
+    const int h = u.head * G + r % G, sees = min(u.len - u.n + token + 1, u.limit);
+    RowSum<D> sum;
+    sum.add_range(p, p.q + (u.first + token) * p.ld_q + (size_t)h * D, rsqrtf((float)D), u.s, u.head, t0,
+                  min(t1, sees));
+    for (int i = 0; i < (D + 31) / 32; ++i) {
+        const int dim = lane + 32 * i;
+        if (dim >= D) continue;
+        if (partial)
+            partial[(size_t)r * D + dim] = sum.acc[i];
+        else
+            p.out[(u.first + token) * p.ld_out + (size_t)h * D + dim] = sees > 0 ? sum.acc[i] / sum.l : 0.0f;
+    }
+    if (partial && lane == 0) {
+        partial[ROWS * D + r] = sum.m * 1.4426950408889634f + shift;
+        partial[ROWS * (D + 1) + r] = sum.l;
+    }
+    return true;
+}
+
+// Block (c, y): 16 rows (or all, where there are fewer) of the unit that begins in CTA c and goes on in the
+// next ones.  A warp a row forms the parts' weights, then the threads sum.
+constexpr int kCombineThreads = 256;
+__host__ __device__ constexpr int combine_rows(int rows) { return rows < 16 ? rows : 16; }
+template <int D, int NT, int ROWS>
+__global__ void __launch_bounds__(kCombineThreads) chunk_combine_kernel(ChunkParams p, const float* partials,
+                                                                         const ChunkSplit* splits) {
+    constexpr int kRows = combine_rows(ROWS);
+    __shared__ float weight[kRows][kChunkCtas], norm[kRows];
+    pdl_wait();
+    const ChunkSplit s = splits[blockIdx.x];
+    if (s.more < 0) return;
+    Unit u;
+    u.s = s.s, u.tile = s.tile, u.head = s.head;
+    set_sequence(p, u);
+    const int G = p.H / p.Hkv, per = ROWS / G, r0 = blockIdx.y * kRows;
+    const int rows = min(min(per, u.n - u.tile * per) * G - r0, kRows);
+    if (rows <= 0) return;
+    const auto part = [&](int k) {
+        return partials + ((size_t)(blockIdx.x + k) * 2 + (k == 0)) * partial_floats(ROWS, D);
+    };
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    for (int r = warp; r < rows; r += kCombineThreads / 32) {
+        float top = -INFINITY, l = 0.0f;
+        for (int k = lane; k <= s.more; k += 32) top = fmaxf(top, part(k)[ROWS * D + r0 + r]);
+        for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+        const float off = top == -INFINITY ? 0.0f : top;
+        for (int k = lane; k <= s.more; k += 32) {
+            const float w = exp2f(part(k)[ROWS * D + r0 + r] - off);
+            weight[r][k] = w;
+            l = fmaf(w, part(k)[ROWS * (D + 1) + r0 + r], l);
+        }
+        for (int o = 16; o; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+        const int token = u.tile * per + (r0 + r) / G;
+        if (lane == 0) norm[r] = u.len - u.n + token >= 0 ? 1.0f / l : 0.0f;
+    }
+    __syncthreads();
+    for (int e = threadIdx.x; e < rows * (D / 4); e += kCombineThreads) {
+        const int r = e / (D / 4), d4 = e % (D / 4) * 4, token = u.tile * per + (r0 + r) / G;
+        float4 o = make_float4(0, 0, 0, 0);
+#pragma unroll 4
+        for (int k = 0; k <= s.more; ++k) {
+            const float4 x = *reinterpret_cast<const float4*>(part(k) + (size_t)(r0 + r) * D + d4);
+            const float w = weight[r][k];
+            o.x = fmaf(w, x.x, o.x), o.y = fmaf(w, x.y, o.y), o.z = fmaf(w, x.z, o.z), o.w = fmaf(w, x.w, o.w);
+        }
+        float* dst = p.out + (u.first + token) * p.ld_out + (size_t)(u.head * G + (r0 + r) % G) * D + d4;
+        const float inv = norm[r];
+        const bool none = inv == 0.0f && u.len - u.n + token < 0;  // zeros, whatever the parts hold
+        dst[0] = none ? 0.0f : o.x * inv;
+        dst[1] = none ? 0.0f : o.y * inv;
+        dst[2] = none ? 0.0f : o.z * inv;
+        dst[3] = none ? 0.0f : o.w * inv;
+    }
+}
+
+template <int D, int NT, int ROWS>
+cudaError_t launch_combine(const ChunkParams& p, int ctas, const float* partials, const ChunkSplit* splits,
+                           cudaStream_t stream) {
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3((unsigned)ctas, ROWS / combine_rows(ROWS));
+    cfg.blockDim = dim3(kCombineThreads);
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, chunk_combine_kernel<D, NT, ROWS>, p, partials, splits);
+}
+
+}  // namespace tb
