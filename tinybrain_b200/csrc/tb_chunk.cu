@@ -941,7 +941,15 @@ ChunkPlan chunk_plan(long long rows, long long batch, long long max_new, long lo
     // the one sequence has more the tensor-core kernel does; else each takes its own.
     const bool few = G <= kFewRows && (max_new * G <= kFewRows || batch > 1);
     const bool many = !few || max_new * G > kFewRows;
-    if (few) c.few_ctas = ctas(kFewRows / G);
+    if (few) {
+        // every warp has a share, of kFewPages pages or more
+        const long long units = std::min(batch * ((std::min(max_new, rows) + kFewRows / G - 1) / (kFewRows / G)),
+                                         batch + rows / (kFewRows / G));
+        const auto many_pages = [](long long n) { return std::min<long long>(n, 1 << 16); };
+        const long long pages = many_pages(units) * many_pages(Hkv) * many_pages((max_len + kPageTokens - 1) / kPageTokens);
+        c.few_ctas = (int)std::max<long long>(1, most((pages + kFewPages - 1) / kFewPages));
+    }
+    const int few_shares = c.few_ctas * (d == 128 ? 8 : 16);
     if (many) c.ctas = ctas(per);
     // Made beforehand where every K and V tile is read by kPreReuse row tiles or
     // more (as far as the bounds tell) and the operands fit kPreBytes.
@@ -953,8 +961,8 @@ ChunkPlan chunk_plan(long long rows, long long batch, long long max_new, long lo
     const auto up = [](size_t n) { return (n + 127) & ~(size_t)127; };
     c.splits = c.ctas * 2 * partial_floats(kTileRows, d) * sizeof(float);
     c.few = up(c.splits + c.ctas * sizeof(ChunkSplit));
-    c.few_splits = c.few + c.few_ctas * 2 * partial_floats(kFewRows, d) * sizeof(float);
-    c.operands = up(c.few_splits + c.few_ctas * sizeof(ChunkSplit));
+    c.few_splits = c.few + few_shares * 2 * partial_floats(kFewRows, d) * sizeof(float);
+    c.operands = up(c.few_splits + few_shares * sizeof(ChunkSplit));
     c.scales = c.operands + (size_t)all_tiles * 8 * nt * d;
     c.bytes = c.scales + (size_t)all_tiles * 64;
     return c;
@@ -994,7 +1002,8 @@ cudaError_t launch_chunk(ChunkParams p, const ChunkPlan& plan, void* workspace, 
         if (e != cudaSuccess) return e;
         chunk_few_kernel<D><<<plan.few_ctas, Few<D>::kThreads, Few<D>::kSmem, stream>>>(p, partials, splits);
         e = cudaGetLastError();
-        if (e == cudaSuccess) e = launch_combine<D, Few<D>::NT, kFewRows>(p, plan.few_ctas, partials, splits, stream);
+        if (e == cudaSuccess) e = launch_combine<D, kPageTokens, kFewRows>(p, plan.few_ctas * Few<D>::kWarps, partials,
+                                                                          splits, stream);
         p.rows_above = kFewRows;
         p.rows_upto = INT_MAX;
     }

@@ -3,8 +3,10 @@
 //
 // The work is reading K and V once; eight rows leave a 128-row tensor-core tile
 // empty, and making its operands costs more than the products.  Here every warp
-// streams its own pages (every 16th of a unit, 8th for D = 128) through its own
-// ring of bulk copies and needs no other warp until the unit ends:
+// takes an equal share of all pages of all units, streams them through its own
+// ring of bulk copies and waits for no other warp; units that several warps hold
+// are joined by chunk_combine_kernel.  (Sixteen warps on one unit, joined at its
+// end, spent a fifth of their time at that barrier.)  Per page of 16 tokens:
 //   scores  mma.sync m16n8k8 on the fp32 page as it lies: A = 16 tokens, B = the
 //           rows' queries from registers, both split into a TF32 high part and
 //           the rest (3 products in separate chains, the small ones apart);
@@ -12,11 +14,8 @@
 //           it by 2^8 (one vote a page);
 //   sums    V in plain fp32 FMAs: a lane holds D / 32 dims of all rows, a row of
 //           V is one conflict-free load, the weights are broadcast loads.
-// At a unit's end the warps' sums meet in shared memory.  The dims of a lane in
-// the scores' products are four neighbours: k is a label, the same for A and B.
-//
-// Bound by HBM: a 16-token page of K and V takes a warp about 450 instructions,
-// a quarter of what the SM could issue while they arrive.
+// The dims of a lane in the scores' products are four neighbours: k is a label,
+// the same for A and B.
 #pragma once
 
 #include "tb_chunk_units.cuh"
@@ -28,26 +27,21 @@ constexpr int kFewRows = 8;
 
 template <int D>
 struct Few {
-    static constexpr int NT = D == 128 ? 64 : 128, PG = NT / kPageTokens;
     static constexpr int kWarps = D == 128 ? 8 : 16, kThreads = kWarps * 32;
     static constexpr int kPageBytes = kPageTokens * D * 4;
     static constexpr int kRing = D >= 64 ? 3 : D == 32 ? 6 : 8;  // pages of a warp on their way
     static constexpr int kLaneDims = D < 32 ? 1 : D / 32;
-    static constexpr int kSumDims = D < 32 ? D : 32;  // dims of a round of the final sum
     static constexpr size_t kSmem = (size_t)kWarps * kRing * kPageBytes;
 };
+constexpr int kFewPages = 2;  // least pages of a share
 
 template <int D>
 struct FewShared {
     using F = Few<D>;
     alignas(16) float weight[F::kWarps][kPageTokens][kFewRows];
-    float sum[F::kWarps][kFewRows][F::kSumDims + 1];
-    float m[F::kWarps][kFewRows], l[F::kWarps][kFewRows];
-    float inverse[kFewRows];  // of the rows' sums
-    int wild[F::kWarps];
     uint64_t full[F::kWarps][F::kRing];
     int id[F::kWarps][F::kRing];
-    ShareShared share;
+    long long scan[F::kWarps], before[F::kThreads], mine[F::kThreads];
     volatile int dead;
 };
 
@@ -68,42 +62,37 @@ __device__ __forceinline__ float few_ex2(float x) {
     return y;
 }
 
-// The pages of the CTA's share that a warp takes, in order.
-template <int D>
+// A warp's share of the pages, in order: units' pages are tiles of 16 positions.
 struct WarpPages {
-    using F = Few<D>;
     Unit u;
-    int at, take, left;  // the piece's first tile and tiles, the tiles after it
-    int page, end;       // the warp's page and the end of the piece's pages
-    int ids, base;       // lane l: the pool page of page base + l * warps
+    int page, end, left;  // the next page, the end of the piece's, and the pages after the piece
+    int ids, base;        // lane l: the pool page of page base + l
 
-    __device__ void piece(const ChunkParams& p, int warp) {
-        take = min(u.tiles - at, left);
-        left -= take;
-        page = at * F::PG + warp;
-        end = min((at + take) * F::PG, (u.limit + kPageTokens - 1) / kPageTokens);
+    __device__ __forceinline__ void piece(const ChunkParams& p, int from) {
+        page = from;
+        end = min(u.tiles, from + left);
+        left -= end - from;
         load(p);
     }
-    __device__ void load(const ChunkParams& p) {
+    __device__ __forceinline__ void load(const ChunkParams& p) {
         base = page;
-        const int mine = base + (threadIdx.x & 31) * F::kWarps;
-        ids = mine < end ? checked_page(p, p.table[(size_t)u.s * p.stride + mine]) : -1;
+        const int mine = base + (threadIdx.x & 31);  // (a unit without positions has one page, all of it beyond)
+        ids = mine < end && mine * kPageTokens < u.limit
+                  ? checked_page(p, p.table[(size_t)u.s * p.stride + mine])
+                  : -1;
     }
-    __device__ bool next_piece(const ChunkParams& p, int warp) {
+    __device__ __forceinline__ bool next_piece(const ChunkParams& p) {
         if (left == 0) return false;
-        next_unit<F::NT, kFewRows>(p, u);
-        at = 0;
-        piece(p, warp);
+        next_unit<kPageTokens, kFewRows>(p, u);
+        piece(p, 0);
         return true;
     }
-    // to the next page, over pieces without one; false: none is left
-    __device__ bool settle(const ChunkParams& p, int warp) {
-        while (page >= end)
-            if (!next_piece(p, warp)) return false;
-        if (page - base >= 32 * F::kWarps) load(p);
+    __device__ __forceinline__ bool next_page(const ChunkParams& p) {
+        if (++page == end) return next_piece(p);
+        if (page - base == 32) load(p);
         return true;
     }
-    __device__ int id() const { return __shfl_sync(0xffffffffu, ids, (page - base) / F::kWarps); }
+    __device__ __forceinline__ int id() const { return __shfl_sync(0xffffffffu, ids, page - base); }
 };
 
 template <int D>
@@ -122,24 +111,76 @@ __global__ void __launch_bounds__(Few<D>::kThreads, 1)
         fence_barrier_init();
         fence_proxy_async_shared();
     }
-    const Share share = find_share<F::NT, kFewRows, F::kThreads>(p, sh.share);
+
+    // ---- the warp's share of all units' pages: shares w, w + CTAs, ... fall to one CTA,
+    //      so that few pages spread over the SMs ----
+    const int run = (p.batch + F::kThreads - 1) / F::kThreads;
+    long long mine = 0;
+    {
+        const int s0 = min(tid * run, p.batch), s1 = min(s0 + run, p.batch);
+        for (int s = s0; s < s1; ++s) {
+            mine += tiles_of_sequence<kPageTokens, kFewRows>(p, s);
+            int first, n;
+            rows_of(p, s, first, n);
+            if (n && p.total_lens[s] > p.stride * kPageTokens) record_error(p.err, kDevBadPage);
+        }
+    }
+    long long upto = mine;
+    for (int o = 1; o < 32; o <<= 1) {
+        const long long t = __shfl_up_sync(0xffffffffu, upto, o);
+        if (lane >= o) upto += t;
+    }
+    if (lane == 31) sh.scan[warp] = upto;
+    __syncthreads();
+    Share share;
+    share.total = 0;
+    for (int w = 0; w < F::kWarps; ++w) {
+        if (w < warp) upto += sh.scan[w];
+        share.total += sh.scan[w];
+    }
+    sh.before[tid] = upto - mine;
+    sh.mine[tid] = mine;
     __syncthreads();
     pdl_launch_dependents();
-    if (share.count == 0) {
-        if (tid == 0) splits[blockIdx.x] = ChunkSplit{0, 0, 0, -1};
+    share.index = warp * gridDim.x + blockIdx.x;
+    share.shares = min((long long)gridDim.x * F::kWarps, (share.total + kFewPages - 1) / kFewPages);
+    if (share.index >= share.shares) {
+        if (lane == 0) splits[share.index] = ChunkSplit{0, 0, 0, -1};
         return;
+    }
+    const long long begin = share.total * share.index / share.shares;
+    share.end = share.total * (share.index + 1) / share.shares;
+    WarpPages fetch, now;
+    {
+        int holder = 0;
+        for (int t = lane; t < F::kThreads; t += 32) {
+            const bool has = sh.before[t] <= begin && begin < sh.before[t] + sh.mine[t];
+            if (has) holder = t + 1;
+        }
+        holder = __reduce_max_sync(0xffffffffu, holder) - 1;
+        long long at = begin - sh.before[holder];
+        Unit& u = now.u;
+        for (u.s = holder * run;; ++u.s) {
+            const long long here = run == 1 ? LLONG_MAX : tiles_of_sequence<kPageTokens, kFewRows>(p, u.s);
+            if (at < here) break;
+            at -= here;
+        }
+        set_sequence(p, u);
+        for (u.tile = 0;; ++u.tile) {
+            set_tile<kPageTokens, kFewRows>(p, u);
+            if (at < (long long)u.tiles * p.Hkv) break;
+            at -= (long long)u.tiles * p.Hkv;
+        }
+        u.head = (int)(at / u.tiles);
+        now.left = (int)(share.end - begin);
+        now.piece(p, (int)(at % u.tiles));
+        fetch = now;
     }
     const int G = p.H / p.Hkv, per = kFewRows / G;
     ChunkSplit split{0, 0, 0, -1};
 
-    // K and V pages alternate through the ring; `fetch` runs ahead of the pieces
-    WarpPages<D> fetch, now;
-    fetch.u = now.u = sh.share.start;
-    fetch.at = now.at = sh.share.tile;
-    fetch.left = now.left = share.count;
-    fetch.piece(p, warp);
-    now.piece(p, warp);
-    bool more = fetch.settle(p, warp);
+    // K and V pages alternate through the ring; `fetch` runs ahead of `now`
+    bool more = true;
     int fetch_kv = 0, fetch_slot = 0, held = 0;  // held: pages fetched and not yet read
     int slot = 0, phase = 0;
     const auto fill = [&]() {
@@ -155,10 +196,7 @@ __global__ void __launch_bounds__(Few<D>::kThreads, 1)
             }
             ++held;
             if (++fetch_slot == kRing) fetch_slot = 0;
-            if (fetch_kv) {
-                fetch.page += F::kWarps;
-                more = fetch.settle(p, warp);
-            }
+            if (fetch_kv) more = fetch.next_page(p);
             fetch_kv ^= 1;
         }
     };
@@ -180,8 +218,9 @@ __global__ void __launch_bounds__(Few<D>::kThreads, 1)
     };
     fill();
 
-    while (true) {
+    do {
         const Unit& u = now.u;
+        const int from = now.page;
         // the rows' queries, times log2(e) / sqrt(D): B fragments (k = dims, n = rows)
         uint32_t qh[kSteps][2], ql[kSteps][2];
         {
@@ -206,14 +245,14 @@ __global__ void __launch_bounds__(Few<D>::kThreads, 1)
         }
         const int rows = min(per, u.n - u.tile * per) * G, all_see = min(held_tokens + 1, u.limit);
         float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
-        float acc[kFewRows][kDims];
+        float2 acc[kFewRows / 2][kDims];  // two rows side by side
 #pragma unroll
-        for (int r = 0; r < kFewRows; ++r)
+        for (int r = 0; r < kFewRows / 2; ++r)
 #pragma unroll
-            for (int d = 0; d < kDims; ++d) acc[r][d] = 0.0f;
+            for (int d = 0; d < kDims; ++d) acc[r][d] = make_float2(0.0f, 0.0f);
         bool wild = false;
         float(*weight)[kFewRows] = sh.weight[warp];
-        for (; now.page < now.end; now.page += F::kWarps) {
+        for (; now.page < now.end; ++now.page) {
             const int pos0 = now.page * kPageTokens;
             const float* rows_k;
             const int id = take_page(rows_k);
@@ -246,11 +285,15 @@ __global__ void __launch_bounds__(Few<D>::kThreads, 1)
             done_page();
             // c[0], c[1]: token g, rows 2 tig, 2 tig + 1; c[2], c[3]: token g + 8
             const bool masked = all_see < pos0 + kPageTokens;
+            if (masked) {
 #pragma unroll
-            for (int x = 0; x < 4; ++x) {
-                const bool vis = !masked || pos0 + g + (x / 2) * 8 < sees[x % 2];
-                wild |= vis && !(fabsf(c[x]) <= 3.4028234e38f);
-                if (!vis) c[x] = -INFINITY;
+                for (int x = 0; x < 4; ++x) {
+                    const bool vis = pos0 + g + (x / 2) * 8 < sees[x % 2];
+                    wild |= vis && !(fabsf(c[x]) <= 3.4028234e38f);
+                    if (!vis) c[x] = -INFINITY;
+                }
+            } else {  // (a sum is finite only if its terms are)
+                wild |= !(fabsf(c[0] * 0.25f + c[1] * 0.25f) + fabsf(c[2] * 0.25f + c[3] * 0.25f) <= 3.4028234e38f);
             }
             float top[2] = {fmaxf(c[0], c[2]), fmaxf(c[1], c[3])};
             bool grow = false;
@@ -268,9 +311,10 @@ __global__ void __launch_bounds__(Few<D>::kThreads, 1)
                 }
                 __syncwarp();
 #pragma unroll
-                for (int r = 0; r < kFewRows; ++r)
+                for (int r = 0; r < kFewRows / 2; ++r)
 #pragma unroll
-                    for (int d = 0; d < kDims; ++d) acc[r][d] *= weight[0][r];
+                    for (int d = 0; d < kDims; ++d)
+                        acc[r][d] = __fmul2_rn(acc[r][d], make_float2(weight[0][2 * r], weight[0][2 * r + 1]));
                 __syncwarp();
             }
             float w[4];
@@ -284,8 +328,9 @@ __global__ void __launch_bounds__(Few<D>::kThreads, 1)
             const int id_v = take_page(rows_v);  // (its barrier orders the weights too)
             if (id_v >= 0 && (D >= 32 || lane < D)) {
                 const int tokens = min(kPageTokens, u.limit - pos0);
-                const auto load_v = [&](int t, float (&v)[kDims]) {
+                const auto add_token = [&](int t, const float4& w0, const float4& w1) {
                     const float* at = rows_v + t * D + lane * kDims;
+                    float v[kDims];
                     if constexpr (kDims == 4) {
                         const float4 f = lds128f(at);
                         v[0] = f.x, v[1] = f.y, v[2] = f.z, v[3] = f.w;
@@ -295,29 +340,31 @@ __global__ void __launch_bounds__(Few<D>::kThreads, 1)
                     } else {
                         v[0] = at[0];
                     }
+                    const float2 ws[4] = {make_float2(w0.x, w0.y), make_float2(w0.z, w0.w), make_float2(w1.x, w1.y),
+                                          make_float2(w1.z, w1.w)};
+#pragma unroll
+                    for (int d = 0; d < kDims; ++d)
+#pragma unroll
+                        for (int r = 0; r < kFewRows / 2; ++r)
+                            acc[r][d] = __ffma2_rn(ws[r], make_float2(v[d], v[d]), acc[r][d]);
                 };
                 if (!masked) {
 #pragma unroll 4
-                    for (int t = 0; t < kPageTokens; ++t) {
-                        float v[kDims];
-                        load_v(t, v);
-                        const float4 w0 = lds128f(&weight[t][0]), w1 = lds128f(&weight[t][4]);
-                        const float ws[8] = {w0.x, w0.y, w0.z, w0.w, w1.x, w1.y, w1.z, w1.w};
-#pragma unroll
-                        for (int r = 0; r < kFewRows; ++r)
-#pragma unroll
-                            for (int d = 0; d < kDims; ++d) acc[r][d] = fmaf(ws[r], v[d], acc[r][d]);
-                    }
+                    for (int t = 0; t < kPageTokens; ++t)
+                        add_token(t, lds128f(&weight[t][0]), lds128f(&weight[t][4]));
                 } else {  // what a row does not see may be anything
 #pragma unroll 1
                     for (int t = 0; t < tokens; ++t) {
-                        float v[kDims];
-                        load_v(t, v);
+                        const float* at = rows_v + t * D + lane * kDims;
 #pragma unroll
                         for (int r = 0; r < kFewRows; ++r) {
                             if (r >= rows || pos0 + t >= held_tokens + r / G + 1) continue;
+                            const float wr = weight[t][r];
 #pragma unroll
-                            for (int d = 0; d < kDims; ++d) acc[r][d] = fmaf(weight[t][r], v[d], acc[r][d]);
+                            for (int d = 0; d < kDims; ++d) {
+                                float& a = r % 2 ? acc[r / 2][d].y : acc[r / 2][d].x;
+                                a = fmaf(wr, at[d], a);
+                            }
                         }
                     }
                 }
@@ -325,81 +372,46 @@ __global__ void __launch_bounds__(Few<D>::kThreads, 1)
             done_page();
         }
 
-        // ---- the unit's end: the warps' sums on a common maximum ----
+        // ---- the piece's end: the unit's rows, or their partial sums ----
 #pragma unroll
-        for (int x = 0; x < 2; ++x) {
+        for (int x = 0; x < 2; ++x)
             for (int o = 4; o < 32; o <<= 1) l[x] += __shfl_xor_sync(0xffffffffu, l[x], o);
-            if (g == 0) {
-                sh.m[warp][2 * tig + x] = m[x];
-                sh.l[warp][2 * tig + x] = l[x];
-            }
-        }
         wild = __any_sync(0xffffffffu, wild);
-        if (lane == 0) sh.wild[warp] = wild;
-        __syncthreads();
-        float top = -INFINITY;
-        for (int k = lane >> 3; k < F::kWarps; k += 4) {
-            top = fmaxf(top, sh.m[k][lane & 7]);
-            wild |= sh.wild[k] != 0;
-        }
-        wild = __any_sync(0xffffffffu, wild);
-        for (int o = 8; o < 32; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-        const float off = top == -INFINITY ? 0.0f : top;
-        float all = 0.0f;
-        for (int k = lane >> 3; k < F::kWarps; k += 4)
-            all = fmaf(few_ex2(sh.m[k][lane & 7] - off), sh.l[k][lane & 7], all);
-        for (int o = 8; o < 32; o <<= 1) all += __shfl_xor_sync(0xffffffffu, all, o);
-        const float mine = few_ex2(sh.m[warp][lane & 7] - off);  // of row lane % 8
-        if (warp == 0 && lane < kFewRows) sh.inverse[lane] = 1.0f / all;
-        const bool whole = now.at == 0 && now.take == u.tiles;
+        const bool whole = from == 0 && now.end == u.tiles;
         float* part = nullptr;
         if (!whole) {
-            part = partials + ((size_t)blockIdx.x * 2 + (now.at == 0)) * partial_floats(kFewRows, D);
-            if (now.at == 0) split = ChunkSplit{u.s, u.tile, u.head, share.followers(u.tiles - now.take)};
+            part = partials + (share.index * 2 + (from == 0)) * partial_floats(kFewRows, D);
+            if (from == 0) split = ChunkSplit{u.s, u.tile, u.head, share.followers(u.tiles - now.end)};
         }
+        if (wild) {
+            for (int r = 0; r < rows; ++r)
+                row_in_fp32<D, kFewRows>(p, u, r, from * kPageTokens, now.end * kPageTokens, part, 0.0f);
+        } else {
 #pragma unroll
-        for (int r = 0; r < kFewRows; ++r) {
-            const float f = __shfl_sync(0xffffffffu, mine, r);
+            for (int r = 0; r < kFewRows; ++r) {
+                const float lr = __shfl_sync(0xffffffffu, r % 2 ? l[1] : l[0], r / 2);
+                const float mr = __shfl_sync(0xffffffffu, r % 2 ? m[1] : m[0], r / 2);
+                if (r >= rows) continue;
+                const int token = u.tile * per + r / G;
+                float* dst = part ? part + r * D
+                                  : p.out + (u.first + token) * p.ld_out + (size_t)(u.head * G + r % G) * D;
+                const bool some = held_tokens + r / G + 1 > 0;
+                const float f = part ? 1.0f : 1.0f / lr;
+                if (D >= 32 || lane < D) {
 #pragma unroll
-            for (int d = 0; d < kDims; ++d) acc[r][d] *= f;
-        }
-#pragma unroll 1
-        for (int o = 0; o < D; o += F::kSumDims) {
-            const int d0 = lane * kDims - o;
-            if (d0 >= 0 && d0 < F::kSumDims)
-#pragma unroll
-                for (int r = 0; r < kFewRows; ++r)
-#pragma unroll
-                    for (int d = 0; d < kDims; ++d) sh.sum[warp][r][d0 + d] = acc[r][d];
-            __syncthreads();
-            for (int e = tid; e < kFewRows * F::kSumDims; e += F::kThreads) {
-                const int r = e / F::kSumDims, d = e % F::kSumDims;
-                float x = 0.0f;
-#pragma unroll
-                for (int k = 0; k < F::kWarps; ++k) x += sh.sum[k][r][d];
-                if (r < rows && !wild) {
-                    if (part) {
-                        part[r * D + o + d] = x;
-                    } else {
-                        const int token = u.tile * per + r / G;
-                        p.out[(u.first + token) * p.ld_out + (size_t)(u.head * G + r % G) * D + o + d] =
-                            held_tokens + r / G + 1 > 0 ? x * sh.inverse[r] : 0.0f;
+                    for (int d = 0; d < kDims; ++d) {
+                        const float a = r % 2 ? acc[r / 2][d].y : acc[r / 2][d].x;
+                        dst[lane * kDims + d] = part || some ? a * f : 0.0f;
                     }
                 }
+                if (part && lane == 0) {
+                    part[kFewRows * D + r] = mr;
+                    part[kFewRows * (D + 1) + r] = lr;
+                }
             }
-            __syncthreads();
         }
-        if (part && warp == 0 && lane < rows && !wild) {
-            part[kFewRows * D + lane] = top;
-            part[kFewRows * (D + 1) + lane] = all;
-        }
-        if (wild)
-            for (int r = warp; r < rows; r += F::kWarps)
-                row_in_fp32<D, kFewRows>(p, u, r, now.at * F::NT, (now.at + now.take) * F::NT, part, 0.0f);
-        __syncthreads();  // the sums' buffers are free again
-        if (!now.next_piece(p, warp)) break;
-    }
-    if (tid == 0) splits[blockIdx.x] = split;
+    } while (now.next_piece(p));
+    if (lane == 0) splits[share.index] = split;
     if (sh.dead) land_copies();
 }
 

@@ -230,8 +230,8 @@ __device__ __forceinline__ long long tiles_of_sequence(const ChunkParams& p, int
     return tiles_before<NT, ROWS>(p, u, (u.n + per - 1) / per) * p.Hkv;
 }
 
-// What a CTA leaves for chunk_combine_kernel: its last unit, if that begins
-// here and goes on in the next `more` CTAs.
+// What a share leaves for chunk_combine_kernel: its last unit, if that begins
+// here and goes on in the next `more` shares.
 struct ChunkSplit {
     int s, tile, head, more;
 };
@@ -242,13 +242,14 @@ __host__ __device__ constexpr size_t partial_floats(int rows, int d) { return (s
 // unit after the other.  A ragged batch, one long sequence and a large prompt
 // thus load the SMs evenly without a plan made on the host.
 struct Share {
-    long long total, ctas, end;
+    long long total, shares, index, end;  // all tiles; the shares and this one of them; where it ends
     int count;
-    // CTAs after this one that hold the `left` tiles after its last
+    // shares after this one that hold the `left` tiles after its last
     __device__ __forceinline__ int followers(int left) const {
         const long long last = end + left - 1;
-        int n = 1;
-        while (total * (blockIdx.x + n + 1) / ctas <= last) ++n;
+        int n = (int)max(last * shares / total - index, 1ll);  // about: shares differ by a tile
+        while (n > 1 && total * (index + n) / shares > last) --n;
+        while (total * (index + n + 1) / shares <= last) ++n;
         return n;
     }
 };
@@ -286,10 +287,11 @@ __device__ __forceinline__ Share find_share(const ChunkParams& p, ShareShared& s
         if (w < warp) before += sh.scan[w];
         share.total += sh.scan[w];
     }
-    const long long cta = blockIdx.x;
-    share.ctas = min((long long)gridDim.x, share.total);  // every share has a tile
-    const long long begin = cta < share.ctas ? share.total * cta / share.ctas : 0;
-    share.end = cta < share.ctas ? share.total * (cta + 1) / share.ctas : 0;
+    share.index = blockIdx.x;
+    share.shares = min((long long)gridDim.x, share.total);  // every share has a tile
+    const bool has = share.index < share.shares;
+    const long long begin = has ? share.total * share.index / share.shares : 0;
+    share.end = has ? share.total * (share.index + 1) / share.shares : 0;
     share.count = (int)(share.end - begin);
     if (share.count > 0 && mine > 0 && before <= begin && begin < before + mine) {
         Unit u;
@@ -366,15 +368,16 @@ __device__ bool row_in_fp32(const ChunkParams& p, const Unit& u, int r, int t0, 
     return true;
 }
 
-// Block (c, y): 16 rows (or all, where there are fewer) of the unit that begins in CTA c and goes on in the
-// next ones.  A warp a row forms the parts' weights, then the threads sum.
+// Block (c, y): 16 rows (or all, where there are fewer) of the unit that begins
+// in share c and goes on in the next ones.  A warp a row forms the maximum and the
+// sum; then 64 parts at a time their weights and the threads' sums.
 constexpr int kCombineThreads = 256;
 __host__ __device__ constexpr int combine_rows(int rows) { return rows < 16 ? rows : 16; }
 template <int D, int NT, int ROWS>
 __global__ void __launch_bounds__(kCombineThreads) chunk_combine_kernel(ChunkParams p, const float* partials,
                                                                          const ChunkSplit* splits) {
-    constexpr int kRows = combine_rows(ROWS);
-    __shared__ float weight[kRows][kChunkCtas], norm[kRows];
+    constexpr int kRows = combine_rows(ROWS), kParts = 64, kEach = (kRows * D / 4 + kCombineThreads - 1) / kCombineThreads;
+    __shared__ float weight[kRows][kParts], top_of[kRows], norm[kRows];
     pdl_wait();
     const ChunkSplit s = splits[blockIdx.x];
     if (s.more < 0) return;
@@ -393,40 +396,57 @@ __global__ void __launch_bounds__(kCombineThreads) chunk_combine_kernel(ChunkPar
         for (int k = lane; k <= s.more; k += 32) top = fmaxf(top, part(k)[ROWS * D + r0 + r]);
         for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
         const float off = top == -INFINITY ? 0.0f : top;
-        for (int k = lane; k <= s.more; k += 32) {
-            const float w = exp2f(part(k)[ROWS * D + r0 + r] - off);
-            weight[r][k] = w;
-            l = fmaf(w, part(k)[ROWS * (D + 1) + r0 + r], l);
-        }
+        for (int k = lane; k <= s.more; k += 32)
+            l = fmaf(exp2f(part(k)[ROWS * D + r0 + r] - off), part(k)[ROWS * (D + 1) + r0 + r], l);
         for (int o = 16; o; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
-        const int token = u.tile * per + (r0 + r) / G;
-        if (lane == 0) norm[r] = u.len - u.n + token >= 0 ? 1.0f / l : 0.0f;
-    }
-    __syncthreads();
-    for (int e = threadIdx.x; e < rows * (D / 4); e += kCombineThreads) {
-        const int r = e / (D / 4), d4 = e % (D / 4) * 4, token = u.tile * per + (r0 + r) / G;
-        float4 o = make_float4(0, 0, 0, 0);
-#pragma unroll 4
-        for (int k = 0; k <= s.more; ++k) {
-            const float4 x = *reinterpret_cast<const float4*>(part(k) + (size_t)(r0 + r) * D + d4);
-            const float w = weight[r][k];
-            o.x = fmaf(w, x.x, o.x), o.y = fmaf(w, x.y, o.y), o.z = fmaf(w, x.z, o.z), o.w = fmaf(w, x.w, o.w);
+        if (lane == 0) {
+            top_of[r] = off;
+            norm[r] = 1.0f / l;
         }
+    }
+    float4 sum[kEach];
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) sum[i] = make_float4(0, 0, 0, 0);
+    for (int k0 = 0; k0 <= s.more; k0 += kParts) {
+        const int parts = min(kParts, s.more + 1 - k0);
+        __syncthreads();
+        for (int e = threadIdx.x; e < rows * kParts; e += kCombineThreads) {
+            const int r = e / kParts, k = e % kParts;
+            if (k < parts) weight[r][k] = exp2f(part(k0 + k)[ROWS * D + r0 + r] - top_of[r]);
+        }
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) {
+            const int e = threadIdx.x + i * kCombineThreads, r = e / (D / 4), d4 = e % (D / 4) * 4;
+            if (r >= rows) continue;
+#pragma unroll 8
+            for (int k = 0; k < parts; ++k) {
+                const float4 x = *reinterpret_cast<const float4*>(part(k0 + k) + (size_t)(r0 + r) * D + d4);
+                const float w = weight[r][k];
+                sum[i].x = fmaf(w, x.x, sum[i].x), sum[i].y = fmaf(w, x.y, sum[i].y);
+                sum[i].z = fmaf(w, x.z, sum[i].z), sum[i].w = fmaf(w, x.w, sum[i].w);
+            }
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+        const int e = threadIdx.x + i * kCombineThreads, r = e / (D / 4), d4 = e % (D / 4) * 4;
+        if (r >= rows) continue;
+        const int token = u.tile * per + (r0 + r) / G;
         float* dst = p.out + (u.first + token) * p.ld_out + (size_t)(u.head * G + (r0 + r) % G) * D + d4;
-        const float inv = norm[r];
-        const bool none = inv == 0.0f && u.len - u.n + token < 0;  // zeros, whatever the parts hold
-        dst[0] = none ? 0.0f : o.x * inv;
-        dst[1] = none ? 0.0f : o.y * inv;
-        dst[2] = none ? 0.0f : o.z * inv;
-        dst[3] = none ? 0.0f : o.w * inv;
+        const bool some = u.len - u.n + token >= 0;  // else zeros, whatever the parts hold
+        dst[0] = some ? sum[i].x * norm[r] : 0.0f;
+        dst[1] = some ? sum[i].y * norm[r] : 0.0f;
+        dst[2] = some ? sum[i].z * norm[r] : 0.0f;
+        dst[3] = some ? sum[i].w * norm[r] : 0.0f;
     }
 }
 
 template <int D, int NT, int ROWS>
-cudaError_t launch_combine(const ChunkParams& p, int ctas, const float* partials, const ChunkSplit* splits,
+cudaError_t launch_combine(const ChunkParams& p, int shares, const float* partials, const ChunkSplit* splits,
                            cudaStream_t stream) {
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3((unsigned)ctas, ROWS / combine_rows(ROWS));
+    cfg.gridDim = dim3((unsigned)shares, ROWS / combine_rows(ROWS));
     cfg.blockDim = dim3(kCombineThreads);
     cfg.stream = stream;
     cudaLaunchAttribute attr[1];
