@@ -8,6 +8,8 @@
 // Rows of an evicted page (table entry -1) are zeros, as in the decode
 // attention (ModelRunner.swift:519-579 over KVCache.swift's pages).
 #include "tb_chunk_mma.cuh"
+#include <atomic>
+
 #include "tb_chunk_few.cuh"
 #include "tb_chunk_units.cuh"
 
@@ -952,7 +954,9 @@ ChunkPlan chunk_plan(long long rows, long long batch, long long max_new, long lo
     const int few_shares = c.few_ctas * (d == 128 ? 8 : 16);
     if (many) c.ctas = ctas(per);
     // Made beforehand where every K and V tile is read by kPreReuse row tiles or
-    // more (as far as the bounds tell) and the operands fit kPreBytes.
+    // more (as far as the bounds tell) and the operands fit kPreBytes.  Measured:
+    // 1.6 row tiles (D = 128) 290 us without, 333 with; 4 (D = 64) 29 and 31; 128
+    // (D = 64) 750 and 400.
     constexpr long long kPreReuse = 8, kPreBytes = 1ll << 30;
     const long long tile_bytes = 8 * nt * d + 64;
     const bool fits = batch <= 65535 && len_tiles <= (1 << 24) && batch * Hkv * len_tiles <= kPreBytes / tile_bytes;
@@ -968,22 +972,33 @@ ChunkPlan chunk_plan(long long rows, long long batch, long long max_new, long lo
     return c;
 }
 
-template <class K>
-cudaError_t chunk_kernel_attributes(K kernel, size_t smem, int regs) {
-    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-    if (e != cudaSuccess || !regs) return e;
-    // setmaxnreg moves registers within what the CTA was launched with: with
-    // fewer than planned the softmax warps would wait for them
-    cudaFuncAttributes a{};
-    e = cudaFuncGetAttributes(&a, kernel);
-    return e == cudaSuccess && a.numRegs != regs ? cudaErrorNotSupported : e;
+// Once per kernel and device (the calls cost more than a launch).  K names the
+// kernel: each has its own record.
+template <auto K>
+cudaError_t chunk_kernel_attributes(size_t smem, int regs) {
+    static std::atomic<uint64_t> done{0};
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess || (dev < 64 && done.load(std::memory_order_relaxed) >> dev & 1)) return e;
+    e = cudaFuncSetAttribute(K, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (e != cudaSuccess) return e;
+    if (regs) {
+        // setmaxnreg moves registers within what the CTA was launched with: with
+        // fewer than planned the softmax warps would wait for them
+        cudaFuncAttributes a{};
+        e = cudaFuncGetAttributes(&a, K);
+        if (e != cudaSuccess) return e;
+        if (a.numRegs != regs) return cudaErrorNotSupported;
+    }
+    if (dev < 64) done.fetch_or(1ull << dev, std::memory_order_relaxed);
+    return cudaSuccess;
 }
 
 template <int D, bool PRE>
 cudaError_t launch_tiles(const ChunkParams& p, const ChunkPlan& plan, float* partials, ChunkSplit* splits,
                          const Operands& pre, cudaStream_t stream) {
     const bool wide_q = p.ld_q % 4 == 0 && aligned_to(p.q, 16), wide_out = p.ld_out % 4 == 0 && aligned_to(p.out, 16);
-    cudaError_t e = chunk_kernel_attributes(chunk_tiles_kernel<D, PRE>, Shape<D>::template kSmem<PRE>, Roles<PRE>::kLaunchRegs);
+    cudaError_t e = chunk_kernel_attributes<chunk_tiles_kernel<D, PRE>>(Shape<D>::template kSmem<PRE>, Roles<PRE>::kLaunchRegs);
     if (e != cudaSuccess) return e;
     chunk_tiles_kernel<D, PRE><<<plan.ctas, Roles<PRE>::kThreads, Shape<D>::template kSmem<PRE>, stream>>>(p, partials, splits, pre,
                                                                                                wide_q, wide_out);
@@ -998,7 +1013,7 @@ cudaError_t launch_chunk(ChunkParams p, const ChunkPlan& plan, void* workspace, 
         float* partials = reinterpret_cast<float*>(w + plan.few);
         ChunkSplit* splits = reinterpret_cast<ChunkSplit*>(w + plan.few_splits);
         p.rows_upto = plan.ctas ? kFewRows : INT_MAX;
-        e = chunk_kernel_attributes(chunk_few_kernel<D>, Few<D>::kSmem, 0);
+        e = chunk_kernel_attributes<chunk_few_kernel<D>>(Few<D>::kSmem, 0);
         if (e != cudaSuccess) return e;
         chunk_few_kernel<D><<<plan.few_ctas, Few<D>::kThreads, Few<D>::kSmem, stream>>>(p, partials, splits);
         e = cudaGetLastError();
@@ -1013,7 +1028,7 @@ cudaError_t launch_chunk(ChunkParams p, const ChunkPlan& plan, void* workspace, 
     const Operands pre{w + plan.operands, reinterpret_cast<float*>(w + plan.scales), plan.operand_tiles};
     if (plan.operand_tiles) {
         const size_t smem = 4 * Shape<D>::kHalf + (kOperandThreads / 32) * Shape<D>::kPageBytes;
-        e = chunk_kernel_attributes(chunk_operands_kernel<D>, smem, 0);
+        e = chunk_kernel_attributes<chunk_operands_kernel<D>>(smem, 0);
         if (e != cudaSuccess) return e;
         chunk_operands_kernel<D><<<dim3((unsigned)plan.operand_tiles, (unsigned)p.Hkv, (unsigned)p.batch),
                                    kOperandThreads, smem, stream>>>(p, pre);

@@ -25,6 +25,7 @@ A step (row counts on the device; buffers of the largest step):
 from __future__ import annotations
 
 import ctypes as C
+import functools
 
 import torch
 
@@ -44,23 +45,29 @@ def _need(ok, message):
         raise ValueError(message)
 
 
-def _flat(t, name, dtype, device, n=None):
-    """A contiguous 1-D tensor of `dtype` on `device`, of n values where n is given."""
-    if not (isinstance(t, torch.Tensor) and t.dtype == dtype and t.device == device and t.dim() == 1
-            and (n is None or t.shape[0] == n) and (t.shape[0] <= 1 or t.stride(0) == 1)):
-        raise ValueError(f"{name} must be a contiguous {dtype} tensor [{'n' if n is None else n}] on {device}, got "
-                         f"{_say(t)}")
-    return t.data_ptr()
+# The checks below run for every tensor of every call, a large part of a small
+# call's cost: attributes that torch answers fastest, the messages only on failure.
+def _flat(t, name, dtype, gpu, n=None):
+    """The address of a contiguous 1-D tensor of `dtype` on GPU `gpu`, of n values where n is given."""
+    if (isinstance(t, torch.Tensor) and t.dtype is dtype and t.get_device() == gpu and t.dim() == 1
+            and (n is None or t.numel() == n) and t.is_contiguous()):
+        return t.data_ptr()
+    raise ValueError(f"{name} must be a contiguous {dtype} tensor [{'n' if n is None else n}] on cuda:{gpu}, got "
+                     f"{_say(t)}")
 
 
-def _rows(t, name, device, rows=None, cols=None):
-    """An fp32 tensor [rows, cols] whose rows are contiguous (any row stride of at least a row)."""
-    if not (isinstance(t, torch.Tensor) and t.dtype == _F32 and t.device == device and t.dim() == 2
-            and (rows is None or t.shape[0] == rows) and (cols is None or t.shape[1] == cols)
-            and (t.shape[1] <= 1 or t.stride(1) == 1) and (t.shape[0] <= 1 or t.stride(0) >= t.shape[1])):
-        want = [("rows" if rows is None else rows), ("cols" if cols is None else cols)]
-        raise ValueError(f"{name} must be a float32 tensor {want} with contiguous rows on {device}, got {_say(t)}")
-    return t.data_ptr(), (t.stride(0) if t.shape[0] > 1 else t.shape[1])
+def _rows(t, name, gpu, rows=None, cols=None):
+    """Address and row stride of an fp32 tensor [rows, cols] whose rows are contiguous (any stride of at least a row)."""
+    if isinstance(t, torch.Tensor) and t.dtype is _F32 and t.get_device() == gpu and t.dim() == 2:
+        n, width = t.shape
+        if (rows is None or n == rows) and (cols is None or width == cols):
+            if t.is_contiguous():
+                return t.data_ptr(), width
+            step, inner = t.stride()
+            if (inner == 1 or width <= 1) and (n <= 1 or step >= width):
+                return t.data_ptr(), step if n > 1 else width
+    want = [("rows" if rows is None else rows), ("cols" if cols is None else cols)]
+    raise ValueError(f"{name} must be a float32 tensor {want} with contiguous rows on cuda:{gpu}, got {_say(t)}")
 
 
 def _say(t):
@@ -72,24 +79,33 @@ def _say(t):
 def _gpu(t, name):
     if not (isinstance(t, torch.Tensor) and t.is_cuda):
         raise ValueError(f"{name} must be a CUDA tensor, got {_say(t)}")
-    return t.device
+    return t.get_device()
 
 
-def _pool(pool, device, layer):
-    if not (isinstance(pool, torch.Tensor) and pool.dtype == _F32 and pool.device == device and pool.dim() == 6
-            and pool.shape[2] == 2 and pool.shape[4] == PAGE_TOKENS and pool.is_contiguous() and pool.numel()):
-        raise ValueError("kv pool must be a contiguous float32 tensor [pages, layers, 2, kv_heads, 16, head_dim] on "
-                         f"{device}, got {_say(pool)}")
-    _need(0 <= layer < pool.shape[1], f"layer {layer} is outside the pool's {pool.shape[1]} layers")
-    return pool.shape[0], pool.shape[1], pool.shape[3], pool.shape[5]
+def _pool(pool, layer):
+    gpu = _gpu(pool, "kv pool")
+    shape = pool.shape
+    if not (pool.dtype is _F32 and len(shape) == 6 and shape[2] == 2 and shape[4] == PAGE_TOKENS
+            and pool.is_contiguous() and pool.numel()):
+        raise ValueError(f"kv pool must be a contiguous float32 tensor [pages, layers, 2, kv_heads, 16, head_dim], got "
+                         f"{_say(pool)}")
+    if not 0 <= layer < shape[1]:
+        raise ValueError(f"layer {layer} is outside the pool's {shape[1]} layers")
+    return gpu, shape[0], shape[1], shape[3], shape[5]
 
 
-def _table(table, device):
-    if not (isinstance(table, torch.Tensor) and table.dtype == _I32 and table.device == device and table.dim() == 2
+def _table(table, gpu):
+    if not (isinstance(table, torch.Tensor) and table.dtype is _I32 and table.get_device() == gpu and table.dim() == 2
             and table.is_contiguous() and table.numel()):
-        raise ValueError(f"page table must be a contiguous int32 tensor [sequences, pages] on {device}, got "
+        raise ValueError(f"page table must be a contiguous int32 tensor [sequences, pages] on cuda:{gpu}, got "
                          f"{_say(table)}")
     return table.shape
+
+
+def _call(name, *args):
+    status = getattr(_lib.load(), name)(*args)
+    if status:
+        _lib.check(status)
 
 
 def build_page_tables(cached_lens, new_lens, free_pages, page_table, row_offsets, total_lens, row_seq, row_pos,
@@ -101,16 +117,16 @@ def build_page_tables(cached_lens, new_lens, free_pages, page_table, row_offsets
     total_lens [sequences], row_seq, row_pos [rows], row_slot int64 [rows], info
     int32 [4] = rows, pages taken (off free_pages' front), PAGES_* status, first
     bad sequence.  A step that does not fit has no rows and takes no page."""
-    device = _gpu(page_table, "page_table")
-    batch, stride = _table(page_table, device)
-    rows = row_seq.shape[0] if isinstance(row_seq, torch.Tensor) and row_seq.dim() == 1 else None
-    call("tb_page_tables_build_dev", _stream_of(device.index), _flat(cached_lens, "cached_lens", _I32, device, batch),
-         _flat(new_lens, "new_lens", _I32, device, batch), batch, _flat(free_pages, "free_pages", _I32, device) or None,
-         free_pages.shape[0], page_table.data_ptr(), stride, rows,
-         _flat(row_offsets, "row_offsets", _I32, device, batch + 1),
-         _flat(total_lens, "total_lens", _I32, device, batch), _flat(row_seq, "row_seq", _I32, device),
-         _flat(row_pos, "row_pos", _I32, device, rows), _flat(row_slot, "row_slot", _I64, device, rows),
-         _flat(info, "info", _I32, device, 4))
+    gpu = _gpu(page_table, "page_table")
+    batch, stride = _table(page_table, gpu)
+    rows = row_seq.numel() if isinstance(row_seq, torch.Tensor) else None
+    free = _flat(free_pages, "free_pages", _I32, gpu)
+    _call("tb_page_tables_build_dev", _stream_of(gpu), _flat(cached_lens, "cached_lens", _I32, gpu, batch),
+          _flat(new_lens, "new_lens", _I32, gpu, batch), batch, free or None, free_pages.numel(), page_table.data_ptr(),
+          stride, rows, _flat(row_offsets, "row_offsets", _I32, gpu, batch + 1),
+          _flat(total_lens, "total_lens", _I32, gpu, batch), _flat(row_seq, "row_seq", _I32, gpu),
+          _flat(row_pos, "row_pos", _I32, gpu, rows), _flat(row_slot, "row_slot", _I64, gpu, rows),
+          _flat(info, "info", _I32, gpu, 4))
     return info
 
 
@@ -127,33 +143,27 @@ def rope_append(q, k, v, row_pos, row_slot, rope, pool, q_out=None, *, layer, nu
     q [rows, heads * d], k and v [rows, kv_heads * d] with any row stride (the
     columns of a fused projection); q_out may be q.  num_rows: the step's row
     count on the device (row_offsets[-1:]), or None for all.  Returns q_out."""
-    device = _gpu(pool, "kv pool")
-    pages, layers, kv, d = _pool(pool, device, layer)
-    qp, ld_q = _rows(q, "q", device)
-    rows = q.shape[0]
+    gpu, pages, layers, kv, d = _pool(pool, layer)
+    qp, ld_q = _rows(q, "q", gpu)
+    rows, cols = q.shape
     if q_out is None:
-        q_out = torch.empty(rows, q.shape[1], dtype=_F32, device=device)
-    _need(q.shape[1] % (kv * d) == 0 and q.shape[1], f"q has {q.shape[1]} columns for {kv} kv heads of {d}")
-    kp, ld_k = _rows(k, "k", device, rows, kv * d)
-    vp, ld_v = _rows(v, "v", device, rows, kv * d)
-    op, ld_o = _rows(q_out, "q_out", device, rows, q.shape[1])
-    if not (isinstance(rope, torch.Tensor) and rope.dtype == _F32 and rope.device == device and rope.dim() == 3
-            and rope.shape[1] * 2 == d and rope.shape[2] == 2 and rope.is_contiguous() and rope.numel()):
-        raise ValueError(f"rope must be a contiguous float32 tensor [positions, {d // 2}, 2] on {device}, got "
+        q_out = torch.empty(rows, cols, dtype=_F32, device=pool.device)
+    _need(cols and cols % (kv * d) == 0, "q has no whole heads per kv head")
+    kp, ld_k = _rows(k, "k", gpu, rows, kv * d)
+    vp, ld_v = _rows(v, "v", gpu, rows, kv * d)
+    op, ld_o = _rows(q_out, "q_out", gpu, rows, cols)
+    if not (isinstance(rope, torch.Tensor) and rope.dtype is _F32 and rope.get_device() == gpu and rope.dim() == 3
+            and rope.shape[1:] == (d // 2, 2) and d % 2 == 0 and rope.is_contiguous() and rope.numel()):
+        raise ValueError(f"rope must be a contiguous float32 tensor [positions, {d // 2}, 2] on cuda:{gpu}, got "
                          f"{_say(rope)}")
+    pos, slot = _flat(row_pos, "row_pos", _I32, gpu), _flat(row_slot, "row_slot", _I64, gpu)
+    if row_pos.numel() < rows or row_slot.numel() < rows:
+        raise ValueError(f"row_pos and row_slot hold {row_pos.numel()} and {row_slot.numel()} of {rows} rows")
+    count = None if num_rows is None else _flat(num_rows, "num_rows", _I32, gpu, 1)
     if rows:
-        call("tb_rope_append_paged_dev", _stream_of(device.index), qp, ld_q, kp, ld_k, vp, ld_v, rows,
-             None if num_rows is None else _flat(num_rows, "num_rows", _I32, device, 1),
-             _flat(row_pos, "row_pos", _I32, device)
-             if row_pos.shape[0] >= rows else _short("row_pos", row_pos, rows),
-             _flat(row_slot, "row_slot", _I64, device)
-             if row_slot.shape[0] >= rows else _short("row_slot", row_slot, rows),
-             rope.data_ptr(), rope.shape[0], layer, layers, q.shape[1] // d, kv, d, pool.data_ptr(), pages, op, ld_o)
+        _call("tb_rope_append_paged_dev", _stream_of(gpu), qp, ld_q, kp, ld_k, vp, ld_v, rows, count, pos, slot,
+              rope.data_ptr(), rope.shape[0], layer, layers, cols // d, kv, d, pool.data_ptr(), pages, op, ld_o)
     return q_out
-
-
-def _short(name, t, rows):
-    raise ValueError(f"{name} holds {t.shape[0]} of {rows} rows")
 
 
 def paged_attention_chunk(q, row_offsets, total_lens, pool, page_table, out=None, *, layer, max_new, max_len,
@@ -166,33 +176,33 @@ def paged_attention_chunk(q, row_offsets, total_lens, pool, page_table, out=None
     right).  workspace: a uint8 tensor of paged_attention_chunk_workspace bytes
     that no overlapping call uses; None takes one from torch's allocator for
     this call.  Returns out."""
-    device = _gpu(pool, "kv pool")
-    pages, layers, kv, d = _pool(pool, device, layer)
-    batch, stride = _table(page_table, device)
-    qp, ld_q = _rows(q, "q", device)
+    gpu, pages, layers, kv, d = _pool(pool, layer)
+    batch, stride = _table(page_table, gpu)
+    qp, ld_q = _rows(q, "q", gpu)
     rows, cols = q.shape
     if out is None:
-        out = torch.empty(rows, cols, dtype=_F32, device=device)
-    op, ld_o = _rows(out, "out", device, rows, cols)
-    _need(cols % (kv * d) == 0 and cols, f"q has {cols} columns for {kv} kv heads of {d}")
-    offsets = _flat(row_offsets, "row_offsets", _I32, device, batch + 1)
-    totals = _flat(total_lens, "total_lens", _I32, device, batch)
+        out = torch.empty(rows, cols, dtype=_F32, device=pool.device)
+    op, ld_o = _rows(out, "out", gpu, rows, cols)
+    _need(cols and cols % (kv * d) == 0, "q has no whole heads per kv head")
+    offsets = _flat(row_offsets, "row_offsets", _I32, gpu, batch + 1)
+    totals = _flat(total_lens, "total_lens", _I32, gpu, batch)
     _need(1 <= max_new < 1 << 31 and 1 <= max_len < 1 << 31, "max_new and max_len must be at least 1")
     if not rows:
         return out
     heads = cols // d
     if workspace is None:
         workspace = torch.empty(paged_attention_chunk_workspace(rows, batch, max_new, max_len, heads, kv, d),
-                                dtype=torch.uint8, device=device)
-    wp = _flat(workspace, "workspace", torch.uint8, device)
-    call("tb_paged_attention_chunk_dev", _stream_of(device.index), qp, ld_q, rows, offsets, totals, batch,
-         pool.data_ptr(), pages, page_table.data_ptr(), stride, max_new, max_len, layer, layers, heads, kv, d, op,
-         ld_o, wp or None, workspace.shape[0])
+                                dtype=torch.uint8, device=pool.device)
+    work = _flat(workspace, "workspace", torch.uint8, gpu)
+    _call("tb_paged_attention_chunk_dev", _stream_of(gpu), qp, ld_q, rows, offsets, totals, batch, pool.data_ptr(),
+          pages, page_table.data_ptr(), stride, max_new, max_len, layer, layers, heads, kv, d, op, ld_o, work or None,
+          workspace.numel())
     return out
 
 
+@functools.lru_cache(maxsize=1024)
 def paged_attention_chunk_workspace(rows, batch, max_new, max_len, num_heads, num_kv_heads, head_dim) -> int:
-    """Bytes of workspace that paged_attention_chunk needs for these bounds on the current GPU's model."""
+    """Bytes of workspace that paged_attention_chunk needs for these bounds."""
     n = C.c_int64(0)
     call("tb_paged_attention_chunk_workspace", rows, batch, max_new, max_len, num_heads, num_kv_heads, head_dim,
          C.byref(n))
@@ -205,19 +215,24 @@ def sample_rows(logits, uniform, token=None, prob=None, entropy=None, *, tempera
 
     temperature, top_p, min_p float32 and top_k int32 [rows], or None for off.
     Returns (token int32, prob, entropy); a row with nothing above -inf gives -1."""
-    device = _gpu(logits, "logits")
-    lp, ld = _rows(logits, "logits", device)
+    gpu = _gpu(logits, "logits")
+    lp, ld = _rows(logits, "logits", gpu)
     rows, vocab = logits.shape
     _need(vocab >= 1, "logits have no columns")
-    token = torch.empty(rows, dtype=_I32, device=device) if token is None else token
-    prob = torch.empty(rows, dtype=_F32, device=device) if prob is None else prob
-    entropy = torch.empty(rows, dtype=_F32, device=device) if entropy is None else entropy
+    if token is None:
+        token = torch.empty(rows, dtype=_I32, device=logits.device)
+    if prob is None:
+        prob = torch.empty(rows, dtype=_F32, device=logits.device)
+    if entropy is None:
+        entropy = torch.empty(rows, dtype=_F32, device=logits.device)
     if rows:
-        each = lambda t, name, dtype: None if t is None else _flat(t, name, dtype, device, rows)  # noqa: E731
-        call("tb_sample_rows_dev", _stream_of(device.index), lp, ld, rows, vocab, each(temperature, "temperature", _F32),
-             each(top_k, "top_k", _I32), each(top_p, "top_p", _F32), each(min_p, "min_p", _F32),
-             _flat(uniform, "uniform", _F32, device, rows), _flat(token, "token", _I32, device, rows),
-             _flat(prob, "prob", _F32, device, rows), _flat(entropy, "entropy", _F32, device, rows))
+        _call("tb_sample_rows_dev", _stream_of(gpu), lp, ld, rows, vocab,
+              None if temperature is None else _flat(temperature, "temperature", _F32, gpu, rows),
+              None if top_k is None else _flat(top_k, "top_k", _I32, gpu, rows),
+              None if top_p is None else _flat(top_p, "top_p", _F32, gpu, rows),
+              None if min_p is None else _flat(min_p, "min_p", _F32, gpu, rows),
+              _flat(uniform, "uniform", _F32, gpu, rows), _flat(token, "token", _I32, gpu, rows),
+              _flat(prob, "prob", _F32, gpu, rows), _flat(entropy, "entropy", _F32, gpu, rows))
     return token, prob, entropy
 
 
