@@ -110,7 +110,10 @@ struct Shape {
 };
 
 struct ChunkBars {
-    uint64_t slot_full[64], slot_empty[64];
+    // By fill: a slot's fills come from two producers and go to converters that may be
+    // two tiles apart, so one barrier's parity would not tell a fill from the one two
+    // before it.  With two, that one is four fills and at least two V tiles back.
+    uint64_t slot_full[2][64], slot_empty[2][64];
     uint64_t k_full[3], v_full[3];
     uint64_t k_empty[kEmptyRing], v_empty[kEmptyRing];  // by tile, see kEmptyRing
     uint64_t scales[kScaleRing];
@@ -316,8 +319,10 @@ __global__ void __launch_bounds__(Roles<PRE>::kThreads, 1)
     if (tid == 0) {
         sh.dead = 0;
         for (int i = 0; i < S::kSlots; ++i) {
-            mbar_init(b.slot_full + i, 1);
-            mbar_init(b.slot_empty + i, 1);
+            for (int f = 0; f < 2; ++f) {
+                mbar_init(b.slot_full[f] + i, 1);
+                mbar_init(b.slot_empty[f] + i, 1);
+            }
         }
         for (int i = 0; i < 3; ++i) {
             mbar_init(b.k_full + i, PRE ? 1 : PG);
@@ -409,11 +414,14 @@ __global__ void __launch_bounds__(Roles<PRE>::kThreads, 1)
 #pragma unroll 1
             for (int g = 0; g < PG; g += 4) {
                 const bool turn = lane >= g && lane < g + 4;
-                lanes_wait(&sh.dead, turn ? b.slot_empty + slot : nullptr, (uint32_t)(fill & 1) ^ 1, p.err);
+                const int last = fill - 1;
+                lanes_wait(&sh.dead, turn && fill ? b.slot_empty[last & 1] + slot : nullptr, (uint32_t)(last >> 1) & 1,
+                           p.err);
                 if (turn && !sh.dead) {
                     sh.slot_page[slot] = id;
-                    mbar_arrive_expect_tx(b.slot_full + slot, id >= 0 ? S::kPageBytes : 0);
-                    if (id >= 0) bulk_g2s(pages + slot * S::kPageBytes, src, S::kPageBytes, b.slot_full + slot);
+                    uint64_t* full = b.slot_full[fill & 1] + slot;
+                    mbar_arrive_expect_tx(full, id >= 0 ? S::kPageBytes : 0);
+                    if (id >= 0) bulk_g2s(pages + slot * S::kPageBytes, src, S::kPageBytes, full);
                 }
                 __syncwarp();
             }
@@ -490,10 +498,10 @@ __global__ void __launch_bounds__(Roles<PRE>::kThreads, 1)
                     const int st = kv ? i % kVStages : i % kKStages, stages = kv ? kVStages : kKStages;
                     // lane 0: the page, lane 1: its place in the operand tile
                     lanes_wait(&sh.dead,
-                               lane == 0   ? b.slot_full + slot
+                               lane == 0   ? b.slot_full[fill & 1] + slot
                                : lane == 1 ? free_bar(kv ? b.v_empty : b.k_empty, i, stages)
                                            : nullptr,
-                               lane == 0 ? (uint32_t)fill & 1 : free_parity(i, stages), p.err);
+                               lane == 0 ? (uint32_t)(fill >> 1) & 1 : free_parity(i, stages), p.err);
                     const int valid = sh.slot_page[slot] < 0 ? 0 : max(0, min(valid_here, kPageTokens));
                     const float* src = reinterpret_cast<const float*>(pages + slot * S::kPageBytes);
                     uint8_t* op = (kv ? v_ops : k_ops) + st * 2 * S::kHalf;
@@ -505,7 +513,7 @@ __global__ void __launch_bounds__(Roles<PRE>::kThreads, 1)
                     __syncwarp();
                     if (lane < 3)
                         mbar_arrive(lane == 0   ? (kv ? b.v_full : b.k_full) + st
-                                    : lane == 1 ? b.slot_empty + slot
+                                    : lane == 1 ? b.slot_empty[fill & 1] + slot
                                                 : b.scales + ring);
                 }
             }
