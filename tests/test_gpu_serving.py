@@ -574,6 +574,21 @@ def test_sample_masked_and_infinite_values(serving, s):
     check_sample(serving, x, np.linspace(0, 0.99, 10).astype(np.float32), **s)
 
 
+@pytest.mark.parametrize("V", [5000, 40001, 400000])
+@pytest.mark.parametrize("s", [dict(k=1777), dict(p=0.6), dict(k=2500, p=0.3), dict(k=2500, p=0.9999), dict(k=4900, p=1e-4),
+                               dict(t=np.inf, p=0.5), dict(t=1e-30, k=40, p=0.9), dict(t=3.0, k=4000, m=0.999)])
+@pytest.mark.parametrize("kind", ["dense", "steps", "far below"])
+def test_sample_boundary_among_many_like_values(serving, kind, s, V):
+    # thousands of elements within a few hundredths of a nat, apart from one another,
+    # in a few equal steps, or so far below one maximum that they have no mass
+    g = np.random.default_rng(V)
+    x = {"dense": g.random((3, V)) / 50, "steps": g.integers(0, 4, (3, V)) / 100.0,
+         "far below": -60 + g.random((3, V))}[kind].astype(np.float32)
+    if kind == "far below":
+        x[:, V // 3] = 5.0
+    check_sample(serving, x, np.array([0.0, 0.4, 0.97], np.float32), **s)
+
+
 def test_sample_ends_of_the_unit_interval(serving):
     x = np.full((4, 50), -np.inf, np.float32)
     x[:, [3, 9, 47]] = 0.0
