@@ -9,7 +9,7 @@
 //   token   the first kept index, in index order, whose running mass passes
 //           u times the kept mass.
 // T = 0 takes the maximum (its first index).  NaN counts as -inf, and a row of
-// -inf alone yields token -1.
+// -inf alone yields token -1.  Weights below e^-700 count as 0.
 //
 // A whole-number result has to come out the same whatever the launch shape, so
 // nothing here depends on the order in which threads arrive: the weights are
@@ -19,7 +19,7 @@
 //
 // A row is read once, by a cluster of P CTAs (P = 1, 2, 4, 8) that keep it in
 // shared memory, each of their warps a run of consecutive elements.  A truncated
-// row then takes one histogram of 1024 bins over (m - x) / T -- counts for top-k,
+// row then takes one histogram of 2048 bins over (m - x) / T -- counts for top-k,
 // masses for top-p -- and the elements of the one bin that holds the boundary,
 // which every CTA ranks for itself (no sort: a select needs the boundary, not the
 // order).  A bin of more elements than the list holds is narrowed by histograms
@@ -35,11 +35,15 @@ namespace {
 
 constexpr int kRowThreads = 512;
 constexpr int kRowWarps = kRowThreads / 32;
-constexpr int kRowBins = 1024;
+constexpr int kRowBins = 2048;
+constexpr int kBinsEach = kRowBins / kRowThreads;
+constexpr int kBinGroups = kRowBins / 32;
 constexpr int kMaxCluster = 8;
 constexpr int kList = 512;           // boundary elements that a CTA notes, and that are ranked
 constexpr int kStagedMax = 44 * 1024;  // elements of a CTA that fit its shared memory
-constexpr double kBinSpan = 40.0;    // nats below the maximum that the histogram resolves
+constexpr float kBinSpan = 24.0f;      // nats below the maximum that the histogram resolves
+constexpr float kNoWeight = 700.0f;    // nats below the maximum where weights end
+constexpr int kRoots = 64;
 
 struct RowsParams {
     const float* logits;
@@ -60,14 +64,19 @@ typedef unsigned long long u64;
 
 struct __align__(16) RowShared {
     u64 mass[kRowBins];             // as low, high words
-    unsigned int count[kRowBins];
+    union {
+        unsigned int count[kRowBins];
+        struct {
+            u64 all[kList], weight[kList];  // the listed elements of all CTAs, once the counts have been read
+        };
+    };
     u64 red[2][kMaxCluster * kRowWarps];  // a reduction's values from all CTAs, alternating
     u64 list[kList];                // the CTA's boundary elements: key, then the index's complement
     int listed[2];                  // how many, for top-k and for top-p
-    u64 all[kList], weight[kList];  // all CTAs'
     int all_n;
-    u64 scan[kRowWarps];
+    u64 groups[2][kMaxCluster][kBinGroups];  // sums of 32 bins from all CTAs, alternating
     u64 found[3];
+    double root[kRoots];            // 2^(j / kRoots)
     double mass_of[kMaxCluster * kRowWarps], moment_of[kMaxCluster * kRowWarps];  // by run
     int ties[kMaxCluster * kRowWarps];
     u64 tie_index[kMaxCluster];
@@ -110,10 +119,12 @@ struct Row {
     float* kept;      // STAGED: the CTA's part of it
     int cta_begin, begin, end;  // the CTA's first element, the warp's run
     int lane, warp, rank;
-    int turn = 0;     // which of the alternating buffers is next
+    int turn = 0, group_turn = 0;  // which of the alternating buffers is next
+    u64 group[2], before_group;    // the lane's groups of bins, and what stands before them
     float top = 0.0f;
     double inv_t = 0.0;
     float bin_scale = 0.0f;
+    double floor_w = 0.0;  // min-p's
     // the last element of the kept prefix
     float cut = -INFINITY;
     int cut_index = -1;
@@ -137,18 +148,16 @@ struct Row {
 
     __device__ __forceinline__ float at(int i) const { return STAGED ? kept[i - cta_begin] : clean(x[i]); }
     __device__ __forceinline__ bool in_prefix(float v, int i) const { return v > cut || (v == cut && i <= cut_index); }
-    // f(value, index) over the warp's run, in steps of 32 consecutive elements
+    // f(values, index) over the warp's run, four at a time: of index + 32 k, and -inf
+    // behind the run's end
     template <class F>
     __device__ __forceinline__ void each(F f) const {
-        int i = begin + lane;
-        for (; i + 96 < end; i += 128) {
+        for (int i = begin + lane; i - lane < end; i += 128) {
             float v[4];
 #pragma unroll
-            for (int k = 0; k < 4; ++k) v[k] = at(i + 32 * k);
-#pragma unroll
-            for (int k = 0; k < 4; ++k) f(v[k], i + 32 * k);
+            for (int k = 0; k < 4; ++k) v[k] = i + 32 * k < end ? at(i + 32 * k) : -INFINITY;
+            f(v, i);
         }
-        for (; i < end; i += 32) f(at(i), i);
     }
     // the first reading, which stages the row
     template <class F>
@@ -171,19 +180,52 @@ struct Row {
         }
     }
 
-    __device__ __forceinline__ double exponent(float v) const {
-        return v == top ? 0.0 : ((double)v - (double)top) * inv_t;
+    // exp(y) of y = (v - top) / T in [-701, 0] as 2^q 2^(j / 64) e^r, |r| <= ln 2 / 128,
+    // the root of two from a table and e^r by its series to r^5 / 5! (the next term is
+    // below 2^-54): the table-driven method of P. T. P. Tang, ACM TOMS 15 (1989).  exp()
+    // itself has a branch for its ends, across which four elements do not overlap.
+    __device__ __forceinline__ double weight(float v, double& y) const {
+        const double ln2 = 0.6931471805599453094, ln2_rest = 2.319046813846299558e-17;
+        y = v == top ? 0.0 : ((double)v - (double)top) * inv_t;
+        const double shift = 6755399441055744.0;  // 1.5 * 2^52: adding it rounds to a whole number
+        const double sum = fma(y, kRoots / ln2, shift), t = sum - shift;
+        const int n = __double2loint(sum);
+        const double r = fma(t, -ln2_rest / kRoots, fma(t, -ln2 / kRoots, y));
+        double e = fma(r, 1.0 / 120.0, 1.0 / 24.0);
+        e = fma(e, r, 1.0 / 6.0);
+        e = fma(e, r, 0.5);
+        e = fma(e, r, 1.0);
+        const double root = sh.root[n & (kRoots - 1)];
+        e = fma(root * r, e, root);
+        return __hiloint2double(__double2hiint(e) + ((n >> 6) << 20), __double2loint(e));
     }
-    __device__ __forceinline__ double weight(float v) const { return v == top ? 1.0 : exp(exponent(v)); }
     __device__ __forceinline__ u64 fixed(float v) const {
-        const double w = weight(v);  // NaN where an infinite maximum meets an infinite T: no mass
-        return w > 0.0 ? (u64)__double2ll_rn(w * p.one) : 0ull;
+        double y;
+        return (u64)__double2ll_rn(weight(v, y) * p.one);
+    }
+    // The weights of four elements of the kept prefix, 0 for others and those that
+    // min-p leaves out, and their exponents.
+    __device__ __forceinline__ void weights(const float (&v)[4], int i, double (&w)[4], double (&y)[4]) const {
+        bool in[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            in[k] = in_prefix(v[k], i + 32 * k);
+            w[k] = y[k] = 0.0;
+        }
+        if (in[0] || in[1] || in[2] || in[3]) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const double e = weight(v[k], y[k]);
+                w[k] = in[k] && e >= floor_w ? e : 0.0;
+                y[k] = in[k] ? y[k] : 0.0;  // (else it may be anything)
+            }
+        }
     }
     // Monotone in the value: 0 for the maximum, the last bin for all that lies
     // kBinSpan nats or more below it.
     __device__ __forceinline__ int bin_of(float v) const {
         if (v == top) return 0;
-        return (int)fminf((top - v) * bin_scale, (float)(kRowBins - 1));
+        return (int)fminf((top - v) * bin_scale, (float)(kRowBins - 1));  // (NaN: the last)
     }
 
     // Reduction over the cluster by an associative, commutative f with f(v, v) = v:
@@ -201,68 +243,87 @@ struct Row {
         return v;
     }
 
-    __device__ __forceinline__ void add_mass(int bin, u64 w) {
-        unsigned int* m = reinterpret_cast<unsigned int*>(sh.mass + bin);
-        const unsigned int lo = (unsigned int)w;
-        unsigned int hi = (unsigned int)(w >> 32);
-        if (lo && atomicAdd(m, lo) + lo < lo) ++hi;  // carry
-        if (hi) atomicAdd(m + 1, hi);
+    // Adds four elements' masses; a bin of -1: none.
+    __device__ __forceinline__ void add_masses(const float (&v)[4], const int (&bin)[4]) {
+        if (bin[0] < 0 && bin[1] < 0 && bin[2] < 0 && bin[3] < 0) return;
+        unsigned int lo[4], hi[4], sum[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const u64 w = fixed(v[k]);
+            lo[k] = bin[k] >= 0 ? (unsigned int)w : 0u;
+            hi[k] = bin[k] >= 0 ? (unsigned int)(w >> 32) : 0u;
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            sum[k] = 0;
+            if (lo[k]) sum[k] = atomicAdd(reinterpret_cast<unsigned int*>(sh.mass + bin[k]), lo[k]) + lo[k];
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            if (sum[k] < lo[k]) ++hi[k];  // carry
+            if (hi[k]) atomicAdd(reinterpret_cast<unsigned int*>(sh.mass + bin[k]) + 1, hi[k]);
+        }
     }
-    // After sync(): bins 2 t and 2 t + 1 of all CTAs (BY_MASS: masses, else counts)
-    // and what stands before them in the order of the bins; the result is the sum.
+    // Adds up the cluster's bins (BY_MASS: masses, else counts), 32 to a group; the
+    // result is the sum.  Each CTA hands its groups' sums to the others: their bins
+    // (128 KB for P = 8) would take 7 us.
     template <bool BY_MASS>
-    __device__ u64 bins(u64 (&b)[2], u64& before) {
-        u64 part[P][2];
+    __device__ u64 add_bins() {
+        static_assert(kBinsEach == 4 && kBinGroups == 64 && P <= 8, "eight threads to a group");
+        __syncthreads();
+        u64 sum = 0;
+#pragma unroll
+        for (int k = 0; k < kBinsEach; ++k) {
+            const int bin = kBinsEach * threadIdx.x + k;
+            sum += BY_MASS ? sh.mass[bin] : sh.count[bin];
+        }
+        for (int o = 1; o < 8; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        u64(&groups)[kMaxCluster][kBinGroups] = sh.groups[group_turn ^= 1];
+        if (lane % 8 < P) dsmem_st_u64(dsmem_map(&groups[rank][threadIdx.x / 8], lane % 8), sum);
+        sync();
+        group[0] = group[1] = 0;
 #pragma unroll
         for (int r = 0; r < P; ++r) {
-            if (BY_MASS) {
-                asm volatile("ld.shared::cluster.v2.u64 {%0, %1}, [%2];"
-                             : "=l"(part[r][0]), "=l"(part[r][1])
-                             : "r"(dsmem_map(sh.mass + 2 * threadIdx.x, r)));
-            } else {
-                unsigned int c0, c1;
-                asm volatile("ld.shared::cluster.v2.u32 {%0, %1}, [%2];"
-                             : "=r"(c0), "=r"(c1)
-                             : "r"(dsmem_map(sh.count + 2 * threadIdx.x, r)));
-                part[r][0] = c0;
-                part[r][1] = c1;
-            }
+            group[0] += groups[r][2 * lane];
+            group[1] += groups[r][2 * lane + 1];
         }
-        b[0] = b[1] = 0;
-#pragma unroll
-        for (int r = 0; r < P; ++r) {
-            b[0] += part[r][0];
-            b[1] += part[r][1];
-        }
-        u64 incl = b[0] + b[1];
+        u64 incl = group[0] + group[1];
         for (int o = 1; o < 32; o <<= 1) {
             const u64 t = __shfl_up_sync(0xffffffffu, incl, o);
             if (lane >= o) incl += t;
         }
-        if (lane == 31) sh.scan[warp] = incl;
-        if (threadIdx.x == 0) sh.found[0] = ~0ull;
-        __syncthreads();
-        before = incl - b[0] - b[1];
-        const u64 warps = lane < kRowWarps ? sh.scan[lane] : 0;
-        u64 sum = warps, lower = lane < warp ? warps : 0;
-        for (int o = kRowWarps / 2; o; o >>= 1) {
-            sum += __shfl_xor_sync(0xffffffffu, sum, o);
-            lower += __shfl_xor_sync(0xffffffffu, lower, o);
-        }
-        before += __shfl_sync(0xffffffffu, lower, 0);
-        return __shfl_sync(0xffffffffu, sum, 0);
+        before_group = incl - group[0] - group[1];
+        return __shfl_sync(0xffffffffu, incl, 31);
     }
-    // After bins(): the bin where the running weight, from `base` on, reaches target
-    // (-1: it does not), and the weight before it.
-    __device__ __forceinline__ int bin_at(const u64 (&b)[2], u64 before, u64 base, u64 target, u64* above) {
-        before += base;
+    // After that: the bin where the running weight, from *above on, reaches target,
+    // and the weight before it.
+    template <bool BY_MASS>
+    __device__ int bin_at(u64 target, u64* above) {
+        if (warp == 0) {
+            u64 before = *above + before_group;
+            const bool second = before + group[0] < target;
+            if (second) before += group[0];
+            const bool here = before < target && before + (second ? group[1] : group[0]) >= target;
+            const unsigned who = __ballot_sync(0xffffffffu, here);
+            const int src = who ? __ffs(who) - 1 : 0;
+            const int bin = 32 * __shfl_sync(0xffffffffu, 2 * lane + second, src) + lane;
+            before = __shfl_sync(0xffffffffu, before, src);
+            u64 part[P], own = 0;
 #pragma unroll
-        for (int k = 0; k < 2; ++k) {
-            if (before < target && before + b[k] >= target) {
-                sh.found[0] = 2 * threadIdx.x + k;
-                sh.found[1] = before;
+            for (int r = 0; r < P; ++r)
+                part[r] = BY_MASS ? dsmem_ld_u64(dsmem_map(sh.mass + bin, r)) : dsmem_ld_u32(dsmem_map(sh.count + bin, r));
+#pragma unroll
+            for (int r = 0; r < P; ++r) own += part[r];
+            u64 incl = own;
+            for (int o = 1; o < 32; o <<= 1) {
+                const u64 t = __shfl_up_sync(0xffffffffu, incl, o);
+                if (lane >= o) incl += t;
             }
-            before += b[k];
+            incl += before;
+            if (incl >= target && incl - own < target) {
+                sh.found[0] = bin;
+                sh.found[1] = incl - own;
+            }
         }
         __syncthreads();
         *above = sh.found[1];
@@ -272,11 +333,13 @@ struct Row {
     // The prefix's elements in a bin, from all CTAs, as sh.all; false: more than the
     // list holds.
     __device__ bool gather(int bin, int which) {
-        each([&](float v, int i) {
-            if (bin_of(v) == bin && in_prefix(v, i)) {
-                const int n = atomicAdd(&sh.listed[which], 1);
-                if (n < kList) sh.list[n] = ((u64)float_order_key(v) << 32) | (uint32_t)~i;
-            }
+        each([&](const float (&v)[4], int i) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+                if (bin_of(v[k]) == bin && in_prefix(v[k], i + 32 * k)) {
+                    const int n = atomicAdd(&sh.listed[which], 1);
+                    if (n < kList) sh.list[n] = ((u64)float_order_key(v[k]) << 32) | (uint32_t) ~(i + 32 * k);
+                }
         });
         sync();
         int here = lane < P ? (int)dsmem_ld_u32(dsmem_map(&sh.listed[which], lane)) : 0, incl = here;
@@ -323,18 +386,19 @@ struct Row {
         cut_index = (int)~(uint32_t)sh.found[2];
     }
 
-    // The same for a bin with more elements than the list: its keys, 1024 bins at a
+    // The same for a bin with more elements than the list: its keys, 2048 bins at a
     // time, until one key is left, and among its elements by index.  `above`: the
     // weight before the bin.
     template <bool BY_MASS>
     __device__ void cut_in_bin(int bin, u64 target, u64 above) {
         uint32_t lo_key = 0xffffffffu, hi_key = 0;
-        each([&](float v, int i) {
-            const uint32_t k = float_order_key(v);
-            if (bin_of(v) == bin && in_prefix(v, i)) {
-                lo_key = min(lo_key, k);
-                hi_key = max(hi_key, k);
-            }
+        each([&](const float (&v)[4], int i) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+                if (bin_of(v[k]) == bin && in_prefix(v[k], i + 32 * k)) {
+                    lo_key = min(lo_key, float_order_key(v[k]));
+                    hi_key = max(hi_key, float_order_key(v[k]));
+                }
         });
         // both ends in one reduction: the high key, and the low key's complement
         const u64 ends = reduce(((u64)hi_key << 32) | (uint32_t)~lo_key, [](u64 a, u64 b) {
@@ -343,7 +407,6 @@ struct Row {
         });
         hi_key = (uint32_t)(ends >> 32);
         lo_key = ~(uint32_t)ends;
-        u64 b[2], before;
         while (lo_key < hi_key) {
             int shift = 0;
             while (((hi_key - lo_key) >> shift) >= (uint32_t)kRowBins) ++shift;
@@ -355,19 +418,19 @@ struct Row {
                     sh.count[i] = 0;
             }
             __syncthreads();
-            each([&](float v, int i) {
-                const uint32_t k = float_order_key(v);
-                if (k < lo_key || k > hi_key || !in_prefix(v, i)) return;
-                const int to = (int)((hi_key - k) >> shift);
-                if (BY_MASS)
-                    add_mass(to, fixed(v));
-                else
-                    atomicAdd(&sh.count[to], 1u);
+            each([&](const float (&v)[4], int i) {
+                int to[4];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const uint32_t key = float_order_key(v[k]);
+                    const bool in = key >= lo_key && key <= hi_key && in_prefix(v[k], i + 32 * k);
+                    to[k] = in ? (int)((hi_key - key) >> shift) : -1;
+                    if (!BY_MASS && in) atomicAdd(&sh.count[to[k]], 1u);
+                }
+                if (BY_MASS) add_masses(v, to);
             });
-            sync();
-            bins<BY_MASS>(b, before);
-            const int found = bin_at(b, before, above, target, &above);
-            if (found < 0) break;  // cannot be: the bin's weight reaches the target, and sums are exact
+            add_bins<BY_MASS>();  // the bin's weight reaches the target, and sums are exact: one is found
+            const int found = bin_at<BY_MASS>(target, &above);
             hi_key -= (uint32_t)found << shift;
             const uint32_t width = (1u << shift) - 1u;
             if (hi_key - lo_key > width) lo_key = hi_key - width;
@@ -377,7 +440,10 @@ struct Row {
         const u64 w = BY_MASS ? fixed(value) : 1ull;
         const u64 need = w ? (target - above + w - 1) / w : 1ull;
         int mine = 0;
-        each([&](float v, int i) { mine += v == value && in_prefix(v, i); });
+        each([&](const float (&v)[4], int i) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) mine += v[k] == value && in_prefix(v[k], i + 32 * k);
+        });
         for (int o = 16; o; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
         if (lane < P) dsmem_st_u32(dsmem_map(sh.ties + rank * kRowWarps + warp, lane), (unsigned int)mine);
         if (threadIdx.x < P) sh.tie_index[threadIdx.x] = 0;
@@ -419,12 +485,13 @@ __global__ void __launch_bounds__(kRowThreads) sample_rows_kernel(RowsParams p) 
         sh.mass[i] = 0;
         sh.count[i] = 0;
     }
+    if (threadIdx.x < kRoots) sh.root[threadIdx.x] = exp2((double)threadIdx.x / kRoots);
     if (threadIdx.x < 2) sh.listed[threadIdx.x] = 0;
     if (P > 1) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
     const float T = p.temperature ? p.temperature[row] : 1.0f;
     const int k = p.top_k ? p.top_k[row] : 0;
     const float top_p = p.top_p ? p.top_p[row] : 1.0f;
-    const double floor_w = p.min_p ? (double)fminf(fmaxf(p.min_p[row], 0.0f), 1.0f) : 0.0;
+    r.floor_w = p.min_p ? (double)fminf(fmaxf(p.min_p[row], 0.0f), 1.0f) : 0.0;
     const double u = fminf(fmaxf(p.uniform[row], 0.0f), 0.99999994f);
     float best = -INFINITY;
     int best_i = 0;
@@ -449,16 +516,20 @@ __global__ void __launch_bounds__(kRowThreads) sample_rows_kernel(RowsParams p) 
     r.top = float_from_order_key((uint32_t)(key >> 32));
     r.inv_t = 1.0 / (double)T;
     r.bin_scale = (float)((double)kRowBins / kBinSpan * r.inv_t);
+    // below this there is no weight; an infinite maximum shares it with its like alone
+    r.cut = r.top == INFINITY ? INFINITY : r.top - kNoWeight * T;
+    r.cut_index = r.cut > -INFINITY ? INT_MAX : -1;
 
     // 2. the kept prefix's last element: top-k's, and top-p's within it
-    u64 b[2], before, above;
+    u64 above = 0;
     if (k > 0 && k < p.V) {
-        r.each([&](float v, int) {
-            if (v > -INFINITY) atomicAdd(&sh.count[r.bin_of(v)], 1u);
+        r.each([&](const float (&v)[4], int i) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (r.in_prefix(v[j], i + 32 * j)) atomicAdd(&sh.count[r.bin_of(v[j])], 1u);
         });
-        r.sync();
-        if (r.template bins<false>(b, before) > (u64)k) {  // else all there is
-            const int bin = r.bin_at(b, before, 0, (u64)k, &above);
+        if (r.template add_bins<false>() > (u64)k) {  // else all there is
+            const int bin = r.template bin_at<false>((u64)k, &above);
             if (r.gather(bin, 0))
                 r.template cut_in_list<false>((u64)k - above);
             else
@@ -466,14 +537,17 @@ __global__ void __launch_bounds__(kRowThreads) sample_rows_kernel(RowsParams p) 
         }
     }
     if (!(top_p >= 1.0f)) {
-        r.each([&](float v, int i) {
-            if (r.in_prefix(v, i)) r.add_mass(r.bin_of(v), r.fixed(v));
+        r.each([&](const float (&v)[4], int i) {
+            int bin[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) bin[j] = r.in_prefix(v[j], i + 32 * j) ? r.bin_of(v[j]) : -1;
+            r.add_masses(v, bin);
         });
-        r.sync();
-        const u64 mass = r.template bins<true>(b, before);
+        const u64 mass = r.template add_bins<true>();
         const double want = ceil((double)top_p * (double)mass);
         const u64 target = want > 1.0 ? min((u64)want, mass) : 1ull;
-        const int bin = r.bin_at(b, before, 0, target, &above);
+        above = 0;
+        const int bin = r.template bin_at<true>(target, &above);
         if (r.gather(bin, 1))
             r.template cut_in_list<true>(target - above);
         else
@@ -481,17 +555,14 @@ __global__ void __launch_bounds__(kRowThreads) sample_rows_kernel(RowsParams p) 
     }
 
     // 3. the kept mass, run by run
-    const auto weight_of = [&](float v, int i) -> double {
-        if (!r.in_prefix(v, i)) return 0.0;
-        const double w = r.weight(v);
-        return w >= floor_w ? w : 0.0;
-    };
     double mass = 0.0, moment = 0.0;
-    r.each([&](float v, int i) {
-        const double w = weight_of(v, i);
-        if (w > 0.0) {
-            mass += w;
-            moment += w * r.exponent(v);
+    r.each([&](const float (&v)[4], int i) {
+        double w[4], y[4];
+        r.weights(v, i, w, y);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            mass += w[j];
+            moment += w[j] * y[j];
         }
     });
     for (int o = 16; o; o >>= 1) {
@@ -538,39 +609,42 @@ __global__ void __launch_bounds__(kRowThreads) sample_rows_kernel(RowsParams p) 
     run = __shfl_sync(0xffffffffu, run, src);
     run_before = __shfl_sync(0xffffffffu, run_before, src);
     if (run != me) return;
-    // 5. the element: 256 at a time by their sum, then 32 at a time by a scan
-    const auto weight_at = [&](int i) { return i < r.end ? weight_of(r.at(i), i) : 0.0; };
+    // 5. the element: 128 at a time by their sum, then 32 at a time by a scan
     int last = -1;
     double last_w = 0.0, running = run_before;
-    bool done = false;
-    for (int i0 = r.begin; i0 < r.end && !done; i0 += 256) {
-        double s = 0.0;
+    for (int i0 = r.begin; i0 < r.end; i0 += 128) {
+        float v[4];
+        double w[4], y[4];
 #pragma unroll
-        for (int j = 0; j < 256; j += 32) s += weight_at(i0 + j + r.lane);
+        for (int j = 0; j < 4; ++j) v[j] = i0 + 32 * j + r.lane < r.end ? r.at(i0 + 32 * j + r.lane) : -INFINITY;
+        r.weights(v, i0 + r.lane, w, y);
+        double s = (w[0] + w[1]) + (w[2] + w[3]);
         for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
         if (s == 0.0) continue;
         // what ends just short of the goal is searched too: a sum in another order
         // may end a rounding lower, and the run's last element is then the one
+        bool done = false;
         if (running + s >= goal * (1.0 - 1e-12)) {
             double upto = running;
-            for (int j = 0; j < 256 && i0 + j < r.end && !done; j += 32) {
-                const double w = weight_at(i0 + j + r.lane);
-                double c = w;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                double c = w[j];
                 for (int o = 1; o < 32; o <<= 1) {
                     const double t = __shfl_up_sync(0xffffffffu, c, o);
                     if (r.lane >= o) c += t;
                 }
-                const unsigned hit = __ballot_sync(0xffffffffu, w > 0.0 && upto + c > goal);
-                const unsigned any = __ballot_sync(0xffffffffu, w > 0.0);
+                const unsigned hit = __ballot_sync(0xffffffffu, w[j] > 0.0 && upto + c > goal);
+                const unsigned any = __ballot_sync(0xffffffffu, w[j] > 0.0);
                 const int pick = hit ? __ffs(hit) - 1 : any ? 31 - __clz(any) : -1;
-                if (pick >= 0) {
-                    last = i0 + j + pick;
-                    last_w = __shfl_sync(0xffffffffu, w, pick);
+                if (pick >= 0 && !done) {
+                    last = i0 + 32 * j + pick;
+                    last_w = __shfl_sync(0xffffffffu, w[j], pick);
                 }
-                done = hit != 0;
+                done |= hit != 0;
                 upto += __shfl_sync(0xffffffffu, c, 31);
             }
         }
+        if (done) break;
         running += s;
     }
     if (r.lane == 0) {
@@ -625,7 +699,7 @@ extern "C" tb_status tb_sample_rows_dev(void* stream, const float* logits, int64
     // elements to read, or while a CTA's part leaves no room for others on its SM
     int P = 1;
     while (P < kMaxCluster &&
-           (((long long)rows * P < 2ll * entry.num_sms && V / (2 * P) >= 2048) || V / P > 16 * 1024))
+           (((long long)rows * P < entry.num_sms && V / (2 * P) >= 2048) || V / P > 16 * 1024))
         P *= 2;
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
     cudaError_t e;
