@@ -26,6 +26,9 @@
 // over its keys.  Last come the kept masses and the search in the run that holds
 // the draw.  Bound by the steps' latency for few rows, by the fp64 exponentials
 // and the histogram's atomics for many.
+#include <cfloat>
+#include <climits>
+
 #include "tb_common.cuh"
 #include "tb_stream_entry.h"
 #include "tb_unit.cuh"
@@ -44,6 +47,7 @@ constexpr int kStagedMax = 44 * 1024;  // elements of a CTA that fit its shared 
 constexpr float kBinSpan = 24.0f;      // nats below the maximum that the histogram resolves
 constexpr float kNoWeight = 700.0f;    // nats below the maximum where weights end
 constexpr int kRoots = 64;
+constexpr int kBatch = 16;             // loads of a lane in flight while the row is read
 
 struct RowsParams {
     const float* logits;
@@ -79,6 +83,8 @@ struct __align__(16) RowShared {
     double root[kRoots];            // 2^(j / kRoots)
     double mass_of[kMaxCluster * kRowWarps], moment_of[kMaxCluster * kRowWarps];  // by run
     int ties[kMaxCluster * kRowWarps];
+    double chunk[kRowWarps], pick_weight;
+    int pick;
     u64 tie_index[kMaxCluster];
 };
 
@@ -100,14 +106,11 @@ __device__ __forceinline__ void dsmem_st_u32(uint32_t addr, unsigned int v) {
 }
 
 // -0 becomes +0 (equal values are ties) and NaN -inf.
-__device__ __forceinline__ float clean(float x) {
-    x += 0.0f;
-    return x == x ? x : -INFINITY;
-}
+__device__ __forceinline__ float clean(float x) { return fmaxf(x + 0.0f, -INFINITY); }
 
 constexpr __host__ __device__ int run_length(int V, int P) {
     const int runs = P * kRowWarps;
-    return ((V + runs - 1) / runs + 31) & ~31;
+    return ((V + runs - 1) / runs + 127) & ~127;
 }
 
 template <int P, bool STAGED>
@@ -116,8 +119,8 @@ struct Row {
     const RowsParams& p;
     RowShared& sh;
     const float* x;   // the row
-    float* kept;      // STAGED: the CTA's part of it
-    int cta_begin, begin, end;  // the CTA's first element, the warp's run
+    float* kept;      // STAGED: the warp's run of it, -inf behind the row's end
+    int base, n;      // the run's first element, and its elements
     int lane, warp, rank;
     int turn = 0, group_turn = 0;  // which of the alternating buffers is next
     u64 group[2], before_group;    // the lane's groups of bins, and what stands before them
@@ -129,15 +132,22 @@ struct Row {
     float cut = -INFINITY;
     int cut_index = -1;
 
-    __device__ Row(const RowsParams& p_, RowShared& s, float* stage, int row) : p(p_), sh(s), kept(stage) {
+    __device__ Row(const RowsParams& p_, RowShared& s, float* stage, int row) : p(p_), sh(s) {
         lane = threadIdx.x & 31;
         warp = threadIdx.x >> 5;
         rank = P == 1 ? 0 : (int)cluster_ctarank();
         x = p.logits + row * p.ld;
         const int len = run_length(p.V, P);
-        cta_begin = min(rank * kRowWarps * len, p.V);
-        begin = min((rank * kRowWarps + warp) * len, p.V);
-        end = min(begin + len, p.V);
+        base = (rank * kRowWarps + warp) * len;
+        n = min(max(p.V - base, 0), len);
+        kept = stage + warp * len;
+    }
+    // the run of the CTA's warp w, instead of its own
+    __device__ void turn_to(int w) {
+        const int len = run_length(p.V, P);
+        base += (w - warp) * len;
+        kept += (w - warp) * len;
+        n = min(max(p.V - base, 0), len);
     }
     static __device__ __forceinline__ void sync() {
         if (P == 1)
@@ -146,47 +156,76 @@ struct Row {
             cluster_sync();
     }
 
-    __device__ __forceinline__ float at(int i) const { return STAGED ? kept[i - cta_begin] : clean(x[i]); }
     __device__ __forceinline__ bool in_prefix(float v, int i) const { return v > cut || (v == cut && i <= cut_index); }
-    // f(values, index) over the warp's run, four at a time: of index + 32 k, and -inf
-    // behind the run's end
+    // the four elements that start at base + o; -inf behind the run's end
+    __device__ __forceinline__ void load4(int o, float (&v)[4]) const {
+        if (STAGED) {
+            const float4 f = *reinterpret_cast<const float4*>(kept + o);
+            v[0] = f.x, v[1] = f.y, v[2] = f.z, v[3] = f.w;
+        } else {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) v[k] = o + k < n ? clean(x[base + o + k]) : -INFINITY;
+        }
+    }
+    // f(values, index of the first) over the warp's run, a lane four consecutive
+    // elements at a time
     template <class F>
     __device__ __forceinline__ void each(F f) const {
-        for (int i = begin + lane; i - lane < end; i += 128) {
+        for (int o = 4 * lane; o - 4 * lane < n; o += 128) {
             float v[4];
-#pragma unroll
-            for (int k = 0; k < 4; ++k) v[k] = i + 32 * k < end ? at(i + 32 * k) : -INFINITY;
-            f(v, i);
+            load4(o, v);
+            f(v, base + o);
         }
     }
-    // the first reading, which stages the row
-    template <class F>
-    __device__ __forceinline__ void read(F f) {
-        int i = begin + lane;
-        for (; i + 224 < end; i += 256) {
-            float v[8];
+    // The first reading, which stages the row: the lane's largest element, and where
+    // asked for, the first index of that value.
+    __device__ __forceinline__ float read(bool want_index, int& index) {
+        float best = -INFINITY;
+        index = 0;
+        const float* run = x + base;
+        int o = lane;
+        float v[kBatch];
+        for (; o - lane + 32 * kBatch <= n; o += 32 * kBatch) {
 #pragma unroll
-            for (int k = 0; k < 8; ++k) v[k] = clean(x[i + 32 * k]);
+            for (int k = 0; k < kBatch; ++k) v[k] = clean(run[o + 32 * k]);
+            float m = v[0];
 #pragma unroll
-            for (int k = 0; k < 8; ++k) {
-                if (STAGED) kept[i + 32 * k - cta_begin] = v[k];
-                f(v[k], i + 32 * k);
+            for (int k = 1; k < kBatch; ++k) m = fmaxf(m, v[k]);
+            if (m > best) {
+                best = m;
+                if (want_index) {
+#pragma unroll
+                    for (int k = kBatch - 1; k >= 0; --k) index = v[k] == m ? base + o + 32 * k : index;
+                }
+            }
+            if (STAGED) {
+#pragma unroll
+                for (int k = 0; k < kBatch; ++k) kept[o + 32 * k] = v[k];
             }
         }
-        for (; i < end; i += 32) {
-            const float v = clean(x[i]);
-            if (STAGED) kept[i - cta_begin] = v;
-            f(v, i);
+        for (; o < ((n + 127) & ~127); o += 128) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) v[k] = o + 32 * k < n ? clean(run[o + 32 * k]) : -INFINITY;
+            const float m = fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3]));
+            if (m > best) {
+                best = m;
+#pragma unroll
+                for (int k = 3; k >= 0; --k) index = v[k] == m ? base + o + 32 * k : index;
+            }
+            if (STAGED) {
+#pragma unroll
+                for (int k = 0; k < 4; ++k) kept[o + 32 * k] = v[k];
+            }
         }
+        return best;
     }
-
     // exp(y) of y = (v - top) / T in [-701, 0] as 2^q 2^(j / 64) e^r, |r| <= ln 2 / 128,
     // the root of two from a table and e^r by its series to r^5 / 5! (the next term is
     // below 2^-54): the table-driven method of P. T. P. Tang, ACM TOMS 15 (1989).  exp()
     // itself has a branch for its ends, across which four elements do not overlap.
     __device__ __forceinline__ double weight(float v, double& y) const {
         const double ln2 = 0.6931471805599453094, ln2_rest = 2.319046813846299558e-17;
-        y = v == top ? 0.0 : ((double)v - (double)top) * inv_t;
+        y = ((double)fminf(v, FLT_MAX) - (double)fminf(top, FLT_MAX)) * inv_t;
         const double shift = 6755399441055744.0;  // 1.5 * 2^52: adding it rounds to a whole number
         const double sum = fma(y, kRoots / ln2, shift), t = sum - shift;
         const int n = __double2loint(sum);
@@ -209,24 +248,28 @@ struct Row {
         bool in[4];
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-            in[k] = in_prefix(v[k], i + 32 * k);
+            in[k] = in_prefix(v[k], i + k);
             w[k] = y[k] = 0.0;
         }
         if (in[0] || in[1] || in[2] || in[3]) {
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
-                const double e = weight(v[k], y[k]);
-                w[k] = in[k] && e >= floor_w ? e : 0.0;
-                y[k] = in[k] ? y[k] : 0.0;  // (else it may be anything)
+                const double e = weight(in[k] ? v[k] : top, y[k]);
+                w[k] = in[k] ? e : 0.0;
+            }
+            if (floor_w > 0.0) {
+#pragma unroll
+                for (int k = 0; k < 4; ++k) w[k] = w[k] >= floor_w ? w[k] : 0.0;
             }
         }
     }
     // Monotone in the value: 0 for the maximum, the last bin for all that lies
-    // kBinSpan nats or more below it.
-    __device__ __forceinline__ int bin_of(float v) const {
-        if (v == top) return 0;
-        return (int)fminf((top - v) * bin_scale, (float)(kRowBins - 1));  // (NaN: the last)
+    // kBinSpan nats or more below it (and for 0 * infinity).  As a float, the bin's
+    // number above 2^23, to which adding that rounds.
+    __device__ __forceinline__ float float_bin(float v) const {
+        return fminf((top - v) * bin_scale, (float)(kRowBins - 1)) + 8388608.0f;
     }
+    __device__ __forceinline__ int bin_of(float v) const { return __float_as_int(float_bin(v)) - 0x4b000000; }
 
     // Reduction over the cluster by an associative, commutative f with f(v, v) = v:
     // every thread gets the result.
@@ -333,12 +376,13 @@ struct Row {
     // The prefix's elements in a bin, from all CTAs, as sh.all; false: more than the
     // list holds.
     __device__ bool gather(int bin, int which) {
+        const float wanted = (float)bin + 8388608.0f;
         each([&](const float (&v)[4], int i) {
 #pragma unroll
             for (int k = 0; k < 4; ++k)
-                if (bin_of(v[k]) == bin && in_prefix(v[k], i + 32 * k)) {
+                if (float_bin(v[k]) == wanted && in_prefix(v[k], i + k)) {
                     const int n = atomicAdd(&sh.listed[which], 1);
-                    if (n < kList) sh.list[n] = ((u64)float_order_key(v[k]) << 32) | (uint32_t) ~(i + 32 * k);
+                    if (n < kList) sh.list[n] = ((u64)float_order_key(v[k]) << 32) | (uint32_t) ~(i + k);
                 }
         });
         sync();
@@ -392,10 +436,11 @@ struct Row {
     template <bool BY_MASS>
     __device__ void cut_in_bin(int bin, u64 target, u64 above) {
         uint32_t lo_key = 0xffffffffu, hi_key = 0;
+        const float wanted = (float)bin + 8388608.0f;
         each([&](const float (&v)[4], int i) {
 #pragma unroll
             for (int k = 0; k < 4; ++k)
-                if (bin_of(v[k]) == bin && in_prefix(v[k], i + 32 * k)) {
+                if (float_bin(v[k]) == wanted && in_prefix(v[k], i + k)) {
                     lo_key = min(lo_key, float_order_key(v[k]));
                     hi_key = max(hi_key, float_order_key(v[k]));
                 }
@@ -423,7 +468,7 @@ struct Row {
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
                     const uint32_t key = float_order_key(v[k]);
-                    const bool in = key >= lo_key && key <= hi_key && in_prefix(v[k], i + 32 * k);
+                    const bool in = key >= lo_key && key <= hi_key && in_prefix(v[k], i + k);
                     to[k] = in ? (int)((hi_key - key) >> shift) : -1;
                     if (!BY_MASS && in) atomicAdd(&sh.count[to[k]], 1u);
                 }
@@ -442,7 +487,7 @@ struct Row {
         int mine = 0;
         each([&](const float (&v)[4], int i) {
 #pragma unroll
-            for (int k = 0; k < 4; ++k) mine += v[k] == value && in_prefix(v[k], i + 32 * k);
+            for (int k = 0; k < 4; ++k) mine += v[k] == value && in_prefix(v[k], i + k);
         });
         for (int o = 16; o; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
         if (lane < P) dsmem_st_u32(dsmem_map(sh.ties + rank * kRowWarps + warp, lane), (unsigned int)mine);
@@ -453,14 +498,23 @@ struct Row {
         for (int i = lane; i < me; i += 32) rank_of += sh.ties[i];
         for (int o = 16; o; o >>= 1) rank_of += __shfl_xor_sync(0xffffffffu, rank_of, o);
         if (rank_of < need && rank_of + mine >= need) {
-            for (int i0 = begin; i0 < end; i0 += 32) {
-                const int i = i0 + lane;
-                const float v = i < end ? at(i) : -INFINITY;
-                const bool same = i < end && v == value && in_prefix(v, i);
-                const unsigned who = __ballot_sync(0xffffffffu, same);
-                if (same && rank_of + __popc(who & ((2u << lane) - 1u)) == need)
-                    for (int r = 0; r < P; ++r) dsmem_st_u64(dsmem_map(sh.tie_index + rank, r), (u64)i + 1);
-                rank_of += __popc(who);
+            for (int o = 4 * lane; o - 4 * lane < n; o += 128) {
+                float v[4];
+                load4(o, v);
+                int same = 0;
+#pragma unroll
+                for (int k = 0; k < 4; ++k) same += v[k] == value && in_prefix(v[k], base + o + k);
+                int incl = same;
+                for (int s = 1; s < 32; s <<= 1) {
+                    const int t = __shfl_up_sync(0xffffffffu, incl, s);
+                    if (lane >= s) incl += t;
+                }
+                u64 at = rank_of + incl - same;
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                    if (v[k] == value && in_prefix(v[k], base + o + k) && ++at == need)
+                        for (int r = 0; r < P; ++r) dsmem_st_u64(dsmem_map(sh.tie_index + rank, r), (u64)(base + o + k) + 1);
+                rank_of += __shfl_sync(0xffffffffu, incl, 31);
             }
         }
         sync();
@@ -474,7 +528,7 @@ struct Row {
 
 template <int P, bool STAGED>
 __global__ void __launch_bounds__(kRowThreads) sample_rows_kernel(RowsParams p) {
-    extern __shared__ float stage[];
+    extern __shared__ __align__(16) float stage[];
     __shared__ RowShared sh;
     const int row = blockIdx.x / P;
     Row<P, STAGED> r(p, sh, stage, row);
@@ -493,27 +547,22 @@ __global__ void __launch_bounds__(kRowThreads) sample_rows_kernel(RowsParams p) 
     const float top_p = p.top_p ? p.top_p[row] : 1.0f;
     r.floor_w = p.min_p ? (double)fminf(fmaxf(p.min_p[row], 0.0f), 1.0f) : 0.0;
     const double u = fminf(fmaxf(p.uniform[row], 0.0f), 0.99999994f);
-    float best = -INFINITY;
-    int best_i = 0;
-    r.read([&](float v, int i) {
-        if (v > best) {
-            best = v;
-            best_i = i;
-        }
-    });
+    const bool greedy = !(T > 0.0f) || k == 1;
+    int index;
+    const float best = r.read(greedy, index);
     // the others have started: their shared memory may be written
     if (P > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
-    const u64 key =
-        r.reduce(best > -INFINITY ? argmax_key(best, best_i) : 0ull, [](u64 a, u64 b) { return a > b ? a : b; });
-    if (key == 0 || !(T > 0.0f) || k == 1) {
+    const u64 key = r.reduce(argmax_key(best, index), [](u64 a, u64 b) { return a > b ? a : b; });
+    r.top = float_from_order_key((uint32_t)(key >> 32));
+    if (greedy || r.top == -INFINITY) {
         if (writer) {
-            p.token[row] = key ? (int)(0xffffffffu - (uint32_t)key) : -1;
-            if (p.prob) p.prob[row] = key ? 1.0f : 0.0f;
+            const bool any = r.top > -INFINITY;
+            p.token[row] = any ? (int)(0xffffffffu - (uint32_t)key) : -1;
+            if (p.prob) p.prob[row] = any ? 1.0f : 0.0f;
             if (p.entropy) p.entropy[row] = 0.0f;
         }
         return;  // (the others' writes came before the barrier)
     }
-    r.top = float_from_order_key((uint32_t)(key >> 32));
     r.inv_t = 1.0 / (double)T;
     r.bin_scale = (float)((double)kRowBins / kBinSpan * r.inv_t);
     // below this there is no weight; an infinite maximum shares it with its like alone
@@ -526,7 +575,7 @@ __global__ void __launch_bounds__(kRowThreads) sample_rows_kernel(RowsParams p) 
         r.each([&](const float (&v)[4], int i) {
 #pragma unroll
             for (int j = 0; j < 4; ++j)
-                if (r.in_prefix(v[j], i + 32 * j)) atomicAdd(&sh.count[r.bin_of(v[j])], 1u);
+                if (r.in_prefix(v[j], i + j)) atomicAdd(&sh.count[r.bin_of(v[j])], 1u);
         });
         if (r.template add_bins<false>() > (u64)k) {  // else all there is
             const int bin = r.template bin_at<false>((u64)k, &above);
@@ -540,7 +589,7 @@ __global__ void __launch_bounds__(kRowThreads) sample_rows_kernel(RowsParams p) 
         r.each([&](const float (&v)[4], int i) {
             int bin[4];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) bin[j] = r.in_prefix(v[j], i + 32 * j) ? r.bin_of(v[j]) : -1;
+            for (int j = 0; j < 4; ++j) bin[j] = r.in_prefix(v[j], i + j) ? r.bin_of(v[j]) : -1;
             r.add_masses(v, bin);
         });
         const u64 mass = r.template add_bins<true>();
@@ -608,48 +657,65 @@ __global__ void __launch_bounds__(kRowThreads) sample_rows_kernel(RowsParams p) 
     const int src = who ? __ffs(who) - 1 : 0;
     run = __shfl_sync(0xffffffffu, run, src);
     run_before = __shfl_sync(0xffffffffu, run_before, src);
-    if (run != me) return;
-    // 5. the element: 128 at a time by their sum, then 32 at a time by a scan
-    int last = -1;
-    double last_w = 0.0, running = run_before;
-    for (int i0 = r.begin; i0 < r.end; i0 += 128) {
-        float v[4];
+    // 5. the element, by the warps of the CTA that has the run: each scans the lanes'
+    // fours of 128 elements, and the first whose sum passes the goal has it
+    if (run / kRowWarps != r.rank) return;
+    r.turn_to(run % kRowWarps);
+    double running = run_before;
+    for (int first = 0; first < r.n; first += 128 * kRowWarps) {
+        const int o = first + 128 * r.warp + 4 * r.lane;
+        float v[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
         double w[4], y[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) v[j] = i0 + 32 * j + r.lane < r.end ? r.at(i0 + 32 * j + r.lane) : -INFINITY;
-        r.weights(v, i0 + r.lane, w, y);
-        double s = (w[0] + w[1]) + (w[2] + w[3]);
-        for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-        if (s == 0.0) continue;
-        // what ends just short of the goal is searched too: a sum in another order
-        // may end a rounding lower, and the run's last element is then the one
-        bool done = false;
-        if (running + s >= goal * (1.0 - 1e-12)) {
-            double upto = running;
+        if (o - 4 * r.lane < r.n) r.load4(o, v);
+        r.weights(v, r.base + o, w, y);
+        const double own = (w[0] + w[1]) + (w[2] + w[3]);
+        double incl4 = own;
+        for (int s = 1; s < 32; s <<= 1) {
+            const double t = __shfl_up_sync(0xffffffffu, incl4, s);
+            if (r.lane >= s) incl4 += t;
+        }
+        if (r.lane == 31) sh.chunk[r.warp] = incl4;
+        __syncthreads();
+        int chunk = -1, last = -1;
+        double before = running;
+        for (int c = 0; c < kRowWarps; ++c) {
+            const double sum = sh.chunk[c];
+            if (sum > 0.0 && chunk < 0) {
+                last = c;
+                if (running + sum > goal) {
+                    chunk = c;
+                    before = running;
+                }
+            }
+            running += sum;
+        }
+        // A sum in another order may end a rounding lower, so that the goal is not
+        // passed: the last element with a weight is then the one.
+        if (r.warp == (chunk >= 0 ? chunk : last)) {
+            double upto = before + (incl4 - own), pick_w = 0.0;
+            int pick = -1;  // the lane's first element that passes the goal, else its last one
+            bool hit = false;
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                double c = w[j];
-                for (int o = 1; o < 32; o <<= 1) {
-                    const double t = __shfl_up_sync(0xffffffffu, c, o);
-                    if (r.lane >= o) c += t;
+                upto += w[j];
+                if (w[j] > 0.0 && !hit) {
+                    pick = j;
+                    pick_w = w[j];
+                    hit = chunk >= 0 && upto > goal;
                 }
-                const unsigned hit = __ballot_sync(0xffffffffu, w[j] > 0.0 && upto + c > goal);
-                const unsigned any = __ballot_sync(0xffffffffu, w[j] > 0.0);
-                const int pick = hit ? __ffs(hit) - 1 : any ? 31 - __clz(any) : -1;
-                if (pick >= 0 && !done) {
-                    last = i0 + 32 * j + pick;
-                    last_w = __shfl_sync(0xffffffffu, w[j], pick);
-                }
-                done |= hit != 0;
-                upto += __shfl_sync(0xffffffffu, c, 31);
+            }
+            const unsigned hits = __ballot_sync(0xffffffffu, hit), any = __ballot_sync(0xffffffffu, pick >= 0);
+            if (r.lane == (hits ? __ffs(hits) - 1 : 31 - __clz(any))) {
+                sh.pick = r.base + o + pick;
+                sh.pick_weight = pick_w;
             }
         }
-        if (done) break;
-        running += s;
+        __syncthreads();
+        if (chunk >= 0) break;
     }
-    if (r.lane == 0) {
-        p.token[row] = last;
-        if (p.prob) p.prob[row] = (float)(last_w / all);
+    if (threadIdx.x == 0) {
+        p.token[row] = sh.pick;
+        if (p.prob) p.prob[row] = (float)(sh.pick_weight / all);
         if (p.entropy) p.entropy[row] = (float)fmax(log(all) - mom / all, 0.0);
     }
 }
