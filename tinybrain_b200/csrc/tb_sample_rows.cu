@@ -404,7 +404,8 @@ struct Row {
     }
     // The list's element where its running weight, in descending order, reaches
     // `target`, becomes the prefix's last; BY_MASS: of their masses, else counts.
-    // The weights of what stands above an element are added by 1 to 32 lanes.
+    // The weights of what stands above an element are added by 1 to 32 lanes; a long
+    // list is split over the cluster (300 elements: 5 us of a CTA's time otherwise).
     template <bool BY_MASS>
     __device__ void cut_in_list(u64 target) {
         const int n = sh.all_n;
@@ -413,19 +414,31 @@ struct Row {
                 sh.weight[i] = fixed(float_from_order_key((uint32_t)(sh.all[i] >> 32)));
             __syncthreads();
         }
+        const bool split = P > 1 && n > 64;
+        const int threads = split ? P * kRowThreads : kRowThreads;
         int lanes = 32;
-        while (lanes > 1 && n * lanes > kRowThreads) lanes >>= 1;
-        const int i = threadIdx.x / lanes;  // n <= kList = kRowThreads
-        const u64 e = i < n ? sh.all[i] : ~0ull;
-        u64 upto = 0;
-        for (int j = threadIdx.x % lanes; j < n; j += lanes)
-            upto += sh.all[j] >= e ? (BY_MASS ? sh.weight[j] : 1ull) : 0ull;
-        for (int o = 1; o < lanes; o <<= 1) upto += __shfl_xor_sync(0xffffffffu, upto, o);
-        if (i < n && threadIdx.x % lanes == 0) {
-            const u64 own = BY_MASS ? sh.weight[i] : 1ull;
-            if (upto - own < target && upto >= target) sh.found[2] = e;
+        while (lanes > 1 && n * lanes > threads) lanes >>= 1;
+        const int i = ((split ? rank * kRowThreads : 0) + threadIdx.x) / lanes;  // n <= kList = kRowThreads
+        if (__any_sync(0xffffffffu, i < n)) {
+            const u64 e = i < n ? sh.all[i] : ~0ull;
+            u64 upto = 0;
+#pragma unroll 4
+            for (int j = threadIdx.x % lanes; j < n; j += lanes)
+                upto += sh.all[j] >= e ? (BY_MASS ? sh.weight[j] : 1ull) : 0ull;
+            for (int o = 1; o < lanes; o <<= 1) upto += __shfl_xor_sync(0xffffffffu, upto, o);
+            if (i < n && threadIdx.x % lanes == 0) {
+                const u64 own = BY_MASS ? sh.weight[i] : 1ull;
+                if (upto - own < target && upto >= target) {
+                    sh.found[2] = e;
+                    if (split)
+                        for (int r = 0; r < P; ++r) dsmem_st_u64(dsmem_map(sh.found + 2, r), e);
+                }
+            }
         }
-        __syncthreads();
+        if (split)
+            sync();
+        else
+            __syncthreads();
         cut = float_from_order_key((uint32_t)(sh.found[2] >> 32));
         cut_index = (int)~(uint32_t)sh.found[2];
     }
