@@ -104,9 +104,16 @@ struct Shape {
     template <bool PRE>
     static constexpr size_t kSmem = (size_t)(kKStages<PRE> + kVStages<PRE>) * 2 * kHalf +
                                     (PRE ? 0 : (size_t)kSlots * kPageBytes);
-    // tensor memory columns
-    static constexpr int kS = 0, kO = 2 * NT, kQ = kO + 2 * D;  // S / P and O twice
-    static_assert(kQ + D <= 512, "tensor memory");
+    // tensor memory columns: S / P and O, each a few times, and Q
+    template <bool PRE>
+    static constexpr int kSBufs = PRE ? 3 : 2;
+    template <bool PRE>
+    static constexpr int kOBufs = PRE ? 1 : 2;
+    template <bool PRE>
+    static constexpr int kO = kSBufs<PRE> * NT;
+    template <bool PRE>
+    static constexpr int kQ = kO<PRE> + kOBufs<PRE> * D;
+    static_assert(kQ<false> + D <= 512 && kQ<true> + D <= 512, "tensor memory");
 };
 
 struct ChunkBars {
@@ -117,8 +124,8 @@ struct ChunkBars {
     uint64_t k_full[3], v_full[3];
     uint64_t k_empty[kEmptyRing], v_empty[kEmptyRing];  // by tile, see kEmptyRing
     uint64_t scales[kScaleRing];
-    uint64_t s_full[2], p_full[2];
-    uint64_t pv_done[2], q_full[kUnitRing], merge_full[4], merge_read[4], drained;
+    uint64_t s_full[3], p_full[3];
+    uint64_t pv_done[2], o_read[2], q_full[kUnitRing], merge_full[4], merge_read[4], drained;
 };
 
 // Operands made beforehand (chunk_operands_kernel): per sequence, KV head and
@@ -306,6 +313,8 @@ __global__ void __launch_bounds__(Roles<PRE>::kThreads, 1)
     constexpr int kIssueWarp = R::kIssueWarp, kLoadWarp = R::kLoadWarp, kConvertWarps = R::kConvertWarps;
     constexpr int kSoftmaxRegs = R::kSoftmaxRegs, kOtherRegs = R::kOtherRegs, kSoftmaxWarps = R::kSoftmaxWarps;
     constexpr int kGroups = R::kGroups;
+    constexpr int kSBufs = S::template kSBufs<PRE>, kOBufs = S::template kOBufs<PRE>;
+    constexpr int kO = S::template kO<PRE>, kQ = S::template kQ<PRE>;
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ ChunkShared sh;
     static_assert(S::template kSmem<PRE> + sizeof(ChunkShared) <= 227 * 1024, "shared memory");
@@ -325,6 +334,8 @@ __global__ void __launch_bounds__(Roles<PRE>::kThreads, 1)
             }
         }
         for (int i = 0; i < 3; ++i) {
+            mbar_init(b.s_full + i, 1);
+            mbar_init(b.p_full + i, 4);
             mbar_init(b.k_full + i, PRE ? 1 : PG);
             mbar_init(b.v_full + i, PRE ? 1 : PG);
         }
@@ -334,9 +345,8 @@ __global__ void __launch_bounds__(Roles<PRE>::kThreads, 1)
         }
         for (int i = 0; i < kScaleRing; ++i) mbar_init(b.scales + i, PRE ? 1 : 2 * PG);
         for (int i = 0; i < 2; ++i) {
-            mbar_init(b.s_full + i, 1);
-            mbar_init(b.p_full + i, 4);
             mbar_init(b.pv_done + i, 1);
+            mbar_init(b.o_read + i, 4);
         }
         for (int i = 0; i < kUnitRing; ++i) mbar_init(b.q_full + i, 4);
         for (int i = 0; i < 4; ++i) {
@@ -445,24 +455,28 @@ __global__ void __launch_bounds__(Roles<PRE>::kThreads, 1)
                 chunk_wait(&sh.dead, b.k_full + st, (uint32_t)(item / kKStages & 1), p.err);
                 tc_fence_after();
                 const uint32_t kb = k0 + st * 2 * S::kHalf;
-                tc_mma_split<NT, D>(tmem + S::kS + (uint32_t)(item & 1) * NT, tmem + S::kQ,
-                                    [](int s) { return 8 * s; }, D / 2, kb, kb + S::kHalf);
-                tc_commit(b.s_full + (item & 1));
+                tc_mma_split<NT, D>(tmem + (uint32_t)(item % kSBufs) * NT, tmem + kQ, [](int s) { return 8 * s; }, D / 2,
+                                    kb, kb + S::kHalf);
+                tc_commit(b.s_full + item % kSBufs);
                 tc_commit(b.k_empty + item % kEmptyRing);
             };
             for (int left = count; left > 0; at = 0) {
                 const int take = min(u.tiles - at, left);
-                issue_s(i, true, unit);
+                // S goes kAhead tiles ahead, over a P whose product has been issued before
+                constexpr int kAhead = kSBufs - 1;
+                for (int j = 0; j < kAhead && j < take; ++j) issue_s(i + j, j == 0, unit);
                 for (int j = 0; j < take; ++j, ++i) {
-                    if (j + 1 < take) issue_s(i + 1, false, unit);
+                    if (j + kAhead < take) issue_s(i + kAhead, false, unit);
                     const int st = i % kVStages;
                     chunk_wait(&sh.dead, b.v_full + st, (uint32_t)(i / kVStages & 1), p.err);
-                    chunk_wait(&sh.dead, b.p_full + (i & 1), (uint32_t)(i / 2 & 1), p.err);
+                    chunk_wait(&sh.dead, b.p_full + i % kSBufs, (uint32_t)(i / kSBufs & 1), p.err);
+                    // (of two buffers, O of two tiles before was read before P of this one arrived)
+                    if (kOBufs == 1 && i > 0)
+                        chunk_wait(&sh.dead, b.o_read + (i - 1 & 1), (uint32_t)((i - 1) / 2 & 1), p.err);
                     tc_fence_after();
                     const uint32_t vb = v0 + st * 2 * S::kHalf;
-                    // P: 16 columns of high, 16 of low halves per 32 positions.  O of two
-                    // tiles before was read before P of this one arrived.
-                    tc_mma_split<D, NT>(tmem + S::kO + (uint32_t)(i & 1) * D, tmem + S::kS + (uint32_t)(i & 1) * NT,
+                    // P: 16 columns of high, 16 of low halves per 32 positions
+                    tc_mma_split<D, NT>(tmem + kO + (uint32_t)(i % kOBufs) * D, tmem + (uint32_t)(i % kSBufs) * NT,
                                         [](int s) { return 32 * (s / 2) + 8 * (s % 2); }, 16, vb, vb + S::kHalf);
                     tc_commit(b.v_empty + i % kEmptyRing);
                     tc_commit(b.pv_done + (i & 1));
@@ -526,7 +540,7 @@ __global__ void __launch_bounds__(Roles<PRE>::kThreads, 1)
         const int group = warp >> 2, quad = warp & 3;
         const uint32_t lanes = (uint32_t)(quad * 32) << 16;
         const int G = p.H / p.Hkv, per = (kTileRows / G);
-        const uint32_t s0_addr = tmem + S::kS + lanes, o0_addr = tmem + S::kO + lanes;
+        const uint32_t s0_addr = tmem + lanes, o0_addr = tmem + kO + lanes;
         ChunkSplit split{0, 0, 0, -1};
         // A unit of at most 32 rows would leave three of a warpgroup's four warps
         // idle: its rows stand in all four lane groups, each of which takes a
@@ -539,7 +553,7 @@ __global__ void __launch_bounds__(Roles<PRE>::kThreads, 1)
             if (__any_sync(0xffffffffu, valid)) {
                 sh.q_scale[unit % kUnitRing][quad * 32 + lane] = load_queries<D>(
                     p, p.q + (w.first + (valid ? token : 0)) * p.ld_q + (size_t)(w.head * G + row % G) * D, valid,
-                    wide_q, tmem + S::kQ + lanes);
+                    wide_q, tmem + kQ + lanes);
                 tmem_st_wait();
             }
             tc_fence_before();
@@ -568,7 +582,7 @@ __global__ void __launch_bounds__(Roles<PRE>::kThreads, 1)
             const auto collect = [&](int item) {
                 warp_wait(sh, b.pv_done + (item & 1), (uint32_t)(item / 2 & 1), p.err);
                 tc_fence_after();
-                const uint32_t to = o0_addr + (uint32_t)(item & 1) * D;
+                const uint32_t to = o0_addr + (uint32_t)(item % kOBufs) * D;
                 if constexpr (D == 16) {
                     int v[16];
                     tmem_ld16(to, v);
@@ -594,13 +608,20 @@ __global__ void __launch_bounds__(Roles<PRE>::kThreads, 1)
                     }
                 }
             };
+            // after that, where there is one O: the next tile's product may go over it
+            const auto release = [&](int item) {
+                if (kOBufs > 1) return;
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(b.o_read + (item & 1));
+            };
             const int i0 = i;  // then this warpgroup's first tile of the unit:
             const int first = kGroups == 1 || (i0 & 1) == group ? i0 : i0 + 1;
             for (i = first; i < i0 + take; i += kGroups) {
-                const uint32_t ts = s0_addr + (uint32_t)(i & 1) * NT;
+                const uint32_t ts = s0_addr + (uint32_t)(i % kSBufs) * NT;
                 const int j = at + (i - i0), ring = i % kScaleRing;
-                lanes_wait(&sh.dead, lane == 0 ? b.scales + ring : lane == 1 ? b.s_full + (i & 1) : nullptr,
-                           (uint32_t)(lane == 0 ? i / kScaleRing : i / 2) & 1, p.err);
+                lanes_wait(&sh.dead, lane == 0 ? b.scales + ring : lane == 1 ? b.s_full + i % kSBufs : nullptr,
+                           (uint32_t)(lane == 0 ? i / kScaleRing : i / kSBufs) & 1, p.err);
                 tc_fence_after();
                 if (busy) {
                     const float *ks = sh.scale[ring], *ve = ks + 8;
@@ -650,6 +671,18 @@ __global__ void __launch_bounds__(Roles<PRE>::kThreads, 1)
                         }
                         return kPShift - (M == -INFINITY ? 0.0f : M);
                     };
+                    // the last tile's P V, and the sums to the new reference: one O is given back
+                    // before the weights are formed, of two the product has time until after
+                    const auto settle = [&] {
+                        if (i > first) {
+                            collect(i - kGroups);
+                            release(i - kGroups);
+                        }
+                        if (__any_sync(0xffffffffu, r != 1.0f)) {
+#pragma unroll
+                            for (int x = 0; x < D / 2; ++x) acc[x] = __fmul2_rn(acc[x], make_float2(r, r));
+                        }
+                    };
                     if (small) {  // the warp's quarter, kept in registers; zeros elsewhere
                         constexpr int W = NT / 4;
                         const int col = quad * W, g = col / 32;
@@ -669,6 +702,7 @@ __global__ void __launch_bounds__(Roles<PRE>::kThreads, 1)
                         float top = page_top(v, col / 16);
                         if constexpr (W == 32) top = fmaxf(top, page_top(v + 16, col / 16 + 1));
                         const float shift = refer(top);
+                        if (kOBufs == 1) settle();
                         uint32_t hi[W / 2], lo[W / 2];
                         page_weights(v, col / 16, shift, hi, lo);
                         if constexpr (W == 32) {
@@ -691,6 +725,7 @@ __global__ void __launch_bounds__(Roles<PRE>::kThreads, 1)
                             top = max3(top, page_top(v, 2 * g), page_top(v + 16, 2 * g + 1));
                         }
                         const float shift = refer(top);
+                        if (kOBufs == 1) settle();
 #pragma unroll 1
                         for (int g = 0; g < NT / 32; ++g) {
                             int v[32];
@@ -705,18 +740,16 @@ __global__ void __launch_bounds__(Roles<PRE>::kThreads, 1)
                         }
                     }
                     tmem_st_wait();
-                    if (i > first) collect(i - kGroups);
-                    if (__any_sync(0xffffffffu, r != 1.0f)) {
-#pragma unroll
-                        for (int x = 0; x < D / 2; ++x) acc[x] = __fmul2_rn(acc[x], make_float2(r, r));
-                    }
+                    if (kOBufs > 1) settle();
+                } else if (i > first) {
+                    release(i - kGroups);
                 }
                 // the odd sums of the last unit still stand where P V of this tile goes
                 if (group == 1 && i == first && merges > 0)
                     warp_wait(sh, b.merge_read + quad, (uint32_t)(merges - 1) & 1, p.err);
                 tc_fence_before();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(b.p_full + (i & 1));
+                if (lane == 0) mbar_arrive(b.p_full + i % kSBufs);
             }
             i = i0 + take;
             const Unit done = u;
@@ -728,11 +761,18 @@ __global__ void __launch_bounds__(Roles<PRE>::kThreads, 1)
                 // the warpgroup of the unit's last tile knows that its queries are read
                 if (kGroups == 1 || ((i - 1) & 1) == group) queries(u, unit + 1);
             }
-            if (busy && first < i) collect(kGroups == 1 || ((i - 1) & 1) == group ? i - 1 : i - 2);
+            if (first < i) {
+                const int mine = kGroups == 1 || ((i - 1) & 1) == group ? i - 1 : i - 2;
+                if (busy) collect(mine);
+                release(mine);
+            }
             wild |= __any_sync(0xffffffffu, huge);
             const bool merge = kGroups == 2 && ((i0 & 1) || take > 1);  // the odd warpgroup had a tile
             if (group == 1) {
                 if (merge) {
+                    // its sums go over O, which the even warpgroup may still be reading
+                    if (((i - 1) & 1) == 0) warp_wait(sh, b.o_read, (uint32_t)((i - 1) / 2) & 1, p.err);
+                    tc_fence_after();
                     if (busy) {
 #pragma unroll
                         for (int o = 0; o < D; o += 16) {
@@ -742,7 +782,7 @@ __global__ void __launch_bounds__(Roles<PRE>::kThreads, 1)
                                 w[2 * x] = __float_as_uint(acc[o / 2 + x].x);
                                 w[2 * x + 1] = __float_as_uint(acc[o / 2 + x].y);
                             }
-                            tmem_st16(o0_addr + D + o, w);
+                            tmem_st16(o0_addr + o, w);
                         }
                         sh.merge_m[quad * 32 + lane] = M;
                         sh.merge_l[quad * 32 + lane] = l;
@@ -811,7 +851,7 @@ __global__ void __launch_bounds__(Roles<PRE>::kThreads, 1)
                 for (int o = 0; o < D; o += 16) {
                     int v[16];
                     if (merge) {
-                        tmem_ld16(o0_addr + D + o, v);
+                        tmem_ld16(o0_addr + o, v);
                         tmem_ld_wait();
                     }
 #pragma unroll
