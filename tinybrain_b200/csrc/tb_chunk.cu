@@ -541,7 +541,7 @@ __global__ void __launch_bounds__(Roles<PRE>::kThreads, 1)
         const uint32_t lanes = (uint32_t)(quad * 32) << 16;
         const int G = p.H / p.Hkv, per = (kTileRows / G);
         const uint32_t s0_addr = tmem + lanes, o0_addr = tmem + kO + lanes;
-        ChunkSplit split{0, 0, 0, -1};
+        ChunkSplit split{-1};
         // A unit of at most 32 rows would leave three of a warpgroup's four warps
         // idle: its rows stand in all four lane groups, each of which takes a
         // quarter of a tile's positions (P is zero elsewhere).
@@ -802,7 +802,7 @@ __global__ void __launch_bounds__(Roles<PRE>::kThreads, 1)
                 part = partials + ((size_t)blockIdx.x * 2 + (from == 0)) * partial_floats(kTileRows, D);
                 if (from == 0) {  // goes on in the next CTAs: up to the one that holds its last tile
                     const int more = share.followers(done.tiles - take);
-                    split = ChunkSplit{done.s, done.tile, done.head, more};
+                    split = split_of<kTileRows>(p, done, more);
                 }
             }
             float w0 = 1.0f, w1 = 0.0f;
@@ -913,7 +913,7 @@ __global__ void __launch_bounds__(Roles<PRE>::kThreads, 1)
     } else if (count > 0) {
         set_registers_down<kOtherRegs>();  // idle
     } else if (tid == 0) {
-        splits[blockIdx.x] = ChunkSplit{0, 0, 0, -1};
+        splits[blockIdx.x] = ChunkSplit{-1};
     }
     tc_fence_before();
     __syncthreads();
@@ -1042,10 +1042,12 @@ cudaError_t chunk_kernel_attributes(size_t smem, int regs) {
     return cudaSuccess;
 }
 
+bool wide_output(const ChunkParams& p) { return p.ld_out % 4 == 0 && aligned_to(p.out, 16); }
+
 template <int D, bool PRE>
 cudaError_t launch_tiles(const ChunkParams& p, const ChunkPlan& plan, float* partials, ChunkSplit* splits,
                          const Operands& pre, cudaStream_t stream) {
-    const bool wide_q = p.ld_q % 4 == 0 && aligned_to(p.q, 16), wide_out = p.ld_out % 4 == 0 && aligned_to(p.out, 16);
+    const bool wide_q = p.ld_q % 4 == 0 && aligned_to(p.q, 16), wide_out = wide_output(p);
     cudaError_t e = chunk_kernel_attributes<chunk_tiles_kernel<D, PRE>>(Shape<D>::template kSmem<PRE>, Roles<PRE>::kLaunchRegs);
     if (e != cudaSuccess) return e;
     chunk_tiles_kernel<D, PRE><<<plan.ctas, Roles<PRE>::kThreads, Shape<D>::template kSmem<PRE>, stream>>>(p, partials, splits, pre,
@@ -1065,8 +1067,8 @@ cudaError_t launch_chunk(ChunkParams p, const ChunkPlan& plan, void* workspace, 
         if (e != cudaSuccess) return e;
         chunk_few_kernel<D><<<plan.few_ctas, Few<D>::kThreads, Few<D>::kSmem, stream>>>(p, partials, splits);
         e = cudaGetLastError();
-        if (e == cudaSuccess) e = launch_combine<D, kPageTokens, kFewRows>(p, plan.few_ctas * Few<D>::kWarps, partials,
-                                                                          splits, stream);
+        if (e == cudaSuccess)
+            e = launch_combine<D, kFewRows>(p, plan.few_ctas * Few<D>::kWarps, partials, splits, wide_output(p), stream);
         p.rows_above = kFewRows;
         p.rows_upto = INT_MAX;
     }
@@ -1086,7 +1088,7 @@ cudaError_t launch_chunk(ChunkParams p, const ChunkPlan& plan, void* workspace, 
         e = launch_tiles<D, false>(p, plan, partials, splits, pre, stream);
     }
     if (e != cudaSuccess) return e;
-    return launch_combine<D, Shape<D>::NT, kTileRows>(p, plan.ctas, partials, splits, stream);
+    return launch_combine<D, kTileRows>(p, plan.ctas, partials, splits, wide_output(p), stream);
 }
 
 }  // namespace

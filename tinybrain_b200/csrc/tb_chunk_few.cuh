@@ -145,7 +145,7 @@ __global__ void __launch_bounds__(Few<D>::kThreads, 1)
     share.index = warp * gridDim.x + blockIdx.x;
     share.shares = min((long long)gridDim.x * F::kWarps, (share.total + kFewPages - 1) / kFewPages);
     if (share.index >= share.shares) {
-        if (lane == 0) splits[share.index] = ChunkSplit{0, 0, 0, -1};
+        if (lane == 0) splits[share.index] = ChunkSplit{-1};
         return;
     }
     const long long begin = share.total * share.index / share.shares;
@@ -177,7 +177,7 @@ __global__ void __launch_bounds__(Few<D>::kThreads, 1)
         fetch = now;
     }
     const int G = p.H / p.Hkv, per = kFewRows / G;
-    ChunkSplit split{0, 0, 0, -1};
+    ChunkSplit split{-1};
 
     // K and V pages alternate through the ring; `fetch` runs ahead of `now`
     bool more = true;
@@ -381,7 +381,7 @@ __global__ void __launch_bounds__(Few<D>::kThreads, 1)
         float* part = nullptr;
         if (!whole) {
             part = partials + (share.index * 2 + (from == 0)) * partial_floats(kFewRows, D);
-            if (from == 0) split = ChunkSplit{u.s, u.tile, u.head, share.followers(u.tiles - now.end)};
+            if (from == 0) split = split_of<kFewRows>(p, u, share.followers(u.tiles - now.end));
         }
         if (wild) {
             for (int r = 0; r < rows; ++r)

@@ -232,9 +232,17 @@ __device__ __forceinline__ long long tiles_of_sequence(const ChunkParams& p, int
 
 // What a share leaves for chunk_combine_kernel: its last unit, if that begins
 // here and goes on in the next `more` shares.
-struct ChunkSplit {
-    int s, tile, head, more;
+struct alignas(16) ChunkSplit {
+    int more;   // -1: no unit
+    int head, row, rows;  // KV head, the output's row of the unit's first token, rows in use
+    int blank;  // rows in front that see no position
+    int unused[3];
 };
+template <int ROWS>
+__device__ __forceinline__ ChunkSplit split_of(const ChunkParams& p, const Unit& u, int more) {
+    const int G = p.H / p.Hkv, per = ROWS / G, t0 = u.tile * per;
+    return ChunkSplit{more, u.head, u.first + t0, min(per, u.n - t0) * G, max(u.n - u.len - t0, 0) * G, {0, 0, 0}};
+}
 // Partial sums of one unit in the workspace: O [rows][D], then M and l [rows].
 __host__ __device__ constexpr size_t partial_floats(int rows, int d) { return (size_t)rows * (d + 2); }
 
@@ -368,85 +376,132 @@ __device__ bool row_in_fp32(const ChunkParams& p, const Unit& u, int r, int t0, 
     return true;
 }
 
-// Block (c, y): 16 rows (or all, where there are fewer) of the unit that begins
-// in share c and goes on in the next ones.  A warp a row forms the maximum and the
-// sum; then 64 parts at a time their weights and the threads' sums.
-constexpr int kCombineThreads = 256;
-__host__ __device__ constexpr int combine_rows(int rows) { return rows < 16 ? rows : 16; }
-template <int D, int NT, int ROWS>
-__global__ void __launch_bounds__(kCombineThreads) chunk_combine_kernel(ChunkParams p, const float* partials,
-                                                                         const ChunkSplit* splits) {
-    constexpr int kRows = combine_rows(ROWS), kParts = 64, kEach = (kRows * D / 4 + kCombineThreads - 1) / kCombineThreads;
-    __shared__ float weight[kRows][kParts], top_of[kRows], norm[kRows];
-    pdl_wait();
-    const ChunkSplit s = splits[blockIdx.x];
-    if (s.more < 0) return;
-    Unit u;
-    u.s = s.s, u.tile = s.tile, u.head = s.head;
-    set_sequence(p, u);
-    const int G = p.H / p.Hkv, per = ROWS / G, r0 = blockIdx.y * kRows;
-    const int rows = min(min(per, u.n - u.tile * per) * G - r0, kRows);
-    if (rows <= 0) return;
-    const auto part = [&](int k) {
-        return partials + ((size_t)(blockIdx.x + k) * 2 + (k == 0)) * partial_floats(ROWS, D);
-    };
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    for (int r = warp; r < rows; r += kCombineThreads / 32) {
-        float top = -INFINITY, l = 0.0f;
-        for (int k = lane; k <= s.more; k += 32) top = fmaxf(top, part(k)[ROWS * D + r0 + r]);
-        for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-        const float off = top == -INFINITY ? 0.0f : top;
-        for (int k = lane; k <= s.more; k += 32)
-            l = fmaf(exp2f(part(k)[ROWS * D + r0 + r] - off), part(k)[ROWS * (D + 1) + r0 + r], l);
-        for (int o = 16; o; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
-        if (lane == 0) {
-            top_of[r] = off;
-            norm[r] = 1.0f / l;
-        }
-    }
+// Joins the parts of the units that several shares hold.  A block takes eight rows
+// of the units that begin in eight consecutive shares.  Of few parts a warp joins
+// a unit's alone; of many all warps do, one unit after the other (there are then
+// no more than two or three such units in eight shares).  A lane has four dims
+// of kEach rows, and reads the parts with their maxima and sums side by side: what
+// the call waits for here is a chain of loads (the share's record, the parts).
+constexpr int kCombineThreads = 256, kCombineWarps = 8, kCombineRows = 8;
+constexpr int kCombineAlone = 4;  // parts that a warp joins alone
+
+template <int D>
+struct CombineSum {
+    static constexpr int kEach = D / 16;
+    float top[kEach], l[kEach];
     float4 sum[kEach];
-#pragma unroll
-    for (int i = 0; i < kEach; ++i) sum[i] = make_float4(0, 0, 0, 0);
-    for (int k0 = 0; k0 <= s.more; k0 += kParts) {
-        const int parts = min(kParts, s.more + 1 - k0);
-        __syncthreads();
-        for (int e = threadIdx.x; e < rows * kParts; e += kCombineThreads) {
-            const int r = e / kParts, k = e % kParts;
-            if (k < parts) weight[r][k] = exp2f(part(k0 + k)[ROWS * D + r0 + r] - top_of[r]);
-        }
-        __syncthreads();
+    __device__ __forceinline__ void clear() {
 #pragma unroll
         for (int i = 0; i < kEach; ++i) {
-            const int e = threadIdx.x + i * kCombineThreads, r = e / (D / 4), d4 = e % (D / 4) * 4;
-            if (r >= rows) continue;
-#pragma unroll 8
-            for (int k = 0; k < parts; ++k) {
-                const float4 x = *reinterpret_cast<const float4*>(part(k0 + k) + (size_t)(r0 + r) * D + d4);
-                const float w = weight[r][k];
-                sum[i].x = fmaf(w, x.x, sum[i].x), sum[i].y = fmaf(w, x.y, sum[i].y);
-                sum[i].z = fmaf(w, x.z, sum[i].z), sum[i].w = fmaf(w, x.w, sum[i].w);
-            }
+            top[i] = -INFINITY;
+            l[i] = 0.0f;
+            sum[i] = make_float4(0, 0, 0, 0);
         }
     }
+    __device__ __forceinline__ void add(int i, float m, float ll, const float4& x) {
+        const float both = fmaxf(top[i], m), off = both == -INFINITY ? 0.0f : both;
+        const float a = exp2f(top[i] - off), b = exp2f(m - off);
+        top[i] = both;
+        l[i] = l[i] * a + ll * b;
+        sum[i].x = sum[i].x * a + x.x * b, sum[i].y = sum[i].y * a + x.y * b;
+        sum[i].z = sum[i].z * a + x.z * b, sum[i].w = sum[i].w * a + x.w * b;
+    }
+};
+
+template <int D, int ROWS>
+__global__ void __launch_bounds__(kCombineThreads, 2)
+    chunk_combine_kernel(ChunkParams p, const float* partials, const ChunkSplit* splits, int shares, bool wide_out) {
+    constexpr int kGroups = ROWS / kCombineRows, kEach = CombineSum<D>::kEach, kAcross = D / 4;
+    constexpr int kAtOnce = D == 128 ? 1 : D == 64 ? 2 : 4;  // parts in flight
+    __shared__ float4 sums[kCombineWarps][kEach][32];
+    __shared__ float tops[kCombineWarps][kCombineRows], ls[kCombineWarps][kCombineRows];
+    __shared__ ChunkSplit items[kCombineWarps];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, G = p.H / p.Hkv;
+    const int share0 = (int)blockIdx.x / kGroups * kCombineWarps, r0 = (int)blockIdx.x % kGroups * kCombineRows;
+    pdl_wait();
+    ChunkSplit s{-1, 0, 0, 0, 0, {0, 0, 0}};
+    if (share0 + warp < shares) s = splits[share0 + warp];
+    if (r0 >= s.rows) s.more = -1;
+    if (lane == 0) items[warp] = s;
+
+    CombineSum<D> sum;
+    const auto row_of = [&](int i) { return (lane + 32 * i) / kAcross; };
+    // adds parts k0, k0 + step, ... of the unit that begins in `share`
+    const auto join = [&](const ChunkSplit& t, int share, int k0, int step) {
+        sum.clear();
+        for (int k = k0; k <= t.more; k += kAtOnce * step) {
+            float m[kAtOnce][kEach], l[kAtOnce][kEach];
+            float4 x[kAtOnce][kEach];
 #pragma unroll
-    for (int i = 0; i < kEach; ++i) {
-        const int e = threadIdx.x + i * kCombineThreads, r = e / (D / 4), d4 = e % (D / 4) * 4;
-        if (r >= rows) continue;
-        const int token = u.tile * per + (r0 + r) / G;
-        float* dst = p.out + (u.first + token) * p.ld_out + (size_t)(u.head * G + (r0 + r) % G) * D + d4;
-        const bool some = u.len - u.n + token >= 0;  // else zeros, whatever the parts hold
-        dst[0] = some ? sum[i].x * norm[r] : 0.0f;
-        dst[1] = some ? sum[i].y * norm[r] : 0.0f;
-        dst[2] = some ? sum[i].z * norm[r] : 0.0f;
-        dst[3] = some ? sum[i].w * norm[r] : 0.0f;
+            for (int a = 0; a < kAtOnce; ++a) {
+                if (k + a * step > t.more) break;
+                const float* part = partials + ((size_t)(share + k + a * step) * 2 + (k + a * step == 0)) *
+                                                   partial_floats(ROWS, D);
+#pragma unroll
+                for (int i = 0; i < kEach; ++i) {
+                    const int r = r0 + row_of(i);
+                    if (r >= t.rows) continue;  // not written
+                    m[a][i] = part[ROWS * D + r];
+                    l[a][i] = part[ROWS * (D + 1) + r];
+                    x[a][i] = *reinterpret_cast<const float4*>(part + (size_t)r * D + (lane + 32 * i) % kAcross * 4);
+                }
+            }
+#pragma unroll
+            for (int a = 0; a < kAtOnce; ++a) {
+                if (k + a * step > t.more) break;
+#pragma unroll
+                for (int i = 0; i < kEach; ++i)
+                    if (r0 + row_of(i) < t.rows) sum.add(i, m[a][i], l[a][i], x[a][i]);
+            }
+        }
+    };
+    const auto write = [&](const ChunkSplit& t, int i, float l, const float4& v) {
+        const int r = r0 + row_of(i);
+        if (r >= t.rows) return;
+        float* dst = p.out + (t.row + r / G) * p.ld_out + (size_t)(t.head * G + r % G) * D + (lane + 32 * i) % kAcross * 4;
+        const float n = 1.0f / l;
+        float4 y = make_float4(v.x * n, v.y * n, v.z * n, v.w * n);
+        if (r < t.blank) y = make_float4(0, 0, 0, 0);  // whatever the parts hold
+        if (wide_out)
+            *reinterpret_cast<float4*>(dst) = y;
+        else
+            dst[0] = y.x, dst[1] = y.y, dst[2] = y.z, dst[3] = y.w;
+    };
+    if (s.more >= 0 && s.more < kCombineAlone) {
+        join(s, share0 + warp, 0, 1);
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) write(s, i, sum.l[i], sum.sum[i]);
+    }
+    __syncthreads();
+    for (int w = 0; w < kCombineWarps; ++w) {
+        const ChunkSplit t = items[w];
+        if (t.more < kCombineAlone) continue;
+        join(t, share0 + w, warp, kCombineWarps);
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) {
+            sums[warp][i][lane] = sum.sum[i];
+            if ((lane + 32 * i) % kAcross == 0) {
+                tops[warp][row_of(i)] = sum.top[i];
+                ls[warp][row_of(i)] = sum.l[i];
+            }
+        }
+        __syncthreads();
+        if (warp < kEach) {
+            const int r = row_of(warp);
+            sum.clear();
+#pragma unroll
+            for (int k = 0; k < kCombineWarps; ++k) sum.add(0, tops[k][r], ls[k][r], sums[k][warp][lane]);
+            write(t, warp, sum.l[0], sum.sum[0]);
+        }
+        __syncthreads();
     }
 }
 
-template <int D, int NT, int ROWS>
+template <int D, int ROWS>
 cudaError_t launch_combine(const ChunkParams& p, int shares, const float* partials, const ChunkSplit* splits,
-                           cudaStream_t stream) {
+                           bool wide_out, cudaStream_t stream) {
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3((unsigned)shares, ROWS / combine_rows(ROWS));
+    cfg.gridDim = dim3((unsigned)((shares + kCombineWarps - 1) / kCombineWarps * (ROWS / kCombineRows)));
     cfg.blockDim = dim3(kCombineThreads);
     cfg.stream = stream;
     cudaLaunchAttribute attr[1];
@@ -454,7 +509,7 @@ cudaError_t launch_combine(const ChunkParams& p, int shares, const float* partia
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, chunk_combine_kernel<D, NT, ROWS>, p, partials, splits);
+    return cudaLaunchKernelEx(&cfg, chunk_combine_kernel<D, ROWS>, p, partials, splits, shares, wide_out);
 }
 
 }  // namespace tb
