@@ -302,6 +302,17 @@ def test_chunk_attention(serving, H, kv, d, total, new):
     check_attend(serving, attend_case(len(total) + H + d, total, new, H, kv, d, extra_rows=2))
 
 
+@pytest.mark.parametrize("H,kv,d,total,new", [
+    (4, 4, 64, [2100], [1100]), (4, 4, 128, [1500], [1069]), (16, 2, 64, [2049, 300, 1025], [203, 5, 180]),
+    (8, 4, 128, [700, 1300], [520, 581]), (4, 4, 32, [1700], [1041]), (8, 8, 16, [1100], [1100])])
+def test_chunk_attention_of_long_prompts(serving, H, kv, d, total, new):
+    # 8 row tiles and more to a sequence, the last one of some rows, of several calls
+    c = attend_case(d + H, total, new, H, kv, d, evict=[(0, 3)])
+    for _ in range(3):
+        check_attend(serving, c)
+    serving.check_device()
+
+
 @pytest.mark.parametrize("H,kv,d", [(32, 4, 64), (8, 8, 128), (16, 4, 32)])
 def test_chunk_attention_long_and_ragged(serving, H, kv, d):
     g = np.random.default_rng(d)

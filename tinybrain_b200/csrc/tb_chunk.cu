@@ -211,12 +211,12 @@ __device__ __forceinline__ void convert_k(const float* src, int valid, uint8_t* 
     }
 }
 
-// V page -> columns (k) `page * 16 ..` of the V^T operand: a lane takes 8
-// consecutive tokens of a dim.
-template <int D>
+// V page -> columns (k) `page * 16 ..` of the V^T operand of NT columns: a lane
+// takes 8 consecutive tokens of a dim.
+template <int D, int NT>
 __device__ __forceinline__ void convert_v(const float* src, int valid, uint8_t* hi, uint8_t* lo, int page,
                                           float* exp_out) {
-    constexpr int NT = Shape<D>::NT, kTasks = D / 16;
+    constexpr int kTasks = D / 16;
     const int lane = threadIdx.x & 31;
     float x[kTasks][8];
     float m = 0.0f;
@@ -520,7 +520,7 @@ __global__ void __launch_bounds__(Roles<PRE>::kThreads, 1)
                     const float* src = reinterpret_cast<const float*>(pages + slot * S::kPageBytes);
                     uint8_t* op = (kv ? v_ops : k_ops) + st * 2 * S::kHalf;
                     if (kv)
-                        convert_v<D>(src, valid, op, op + S::kHalf, page, &sh.scale[ring][8 + page]);
+                        convert_v<D, NT>(src, valid, op, op + S::kHalf, page, &sh.scale[ring][8 + page]);
                     else
                         convert_k<D>(src, valid, op, op + S::kHalf, page, &sh.scale[ring][page]);
                     fence_proxy_async_shared();
@@ -611,6 +611,8 @@ __global__ void __launch_bounds__(Roles<PRE>::kThreads, 1)
             // after that, where there is one O: the next tile's product may go over it
             const auto release = [&](int item) {
                 if (kOBufs > 1) return;
+                // a warp without rows may not run ahead: its next arrival would count for this tile
+                if (!busy) warp_wait(sh, b.pv_done + (item & 1), (uint32_t)(item / 2 & 1), p.err);
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(b.o_read + (item & 1));
@@ -923,52 +925,55 @@ __global__ void __launch_bounds__(Roles<PRE>::kThreads, 1)
     }
 }
 
-// Operands of one tile of one KV head: a CTA of 8 warps, one or two pages each.
-constexpr int kOperandThreads = 256;
+// Operands of all K and V pages of a head: a warp a page, which it reads into
+// shared memory, converts in place (the halves take as many bytes as the page) and
+// writes to its part of the tile.  No warp waits for another; bound by HBM.
+constexpr int kOperandWarps = 8;
 template <int D>
-__global__ void __launch_bounds__(kOperandThreads) chunk_operands_kernel(ChunkParams p, Operands pre) {
+__global__ void __launch_bounds__(kOperandWarps * 32) chunk_operands_kernel(ChunkParams p, Operands pre) {
     using S = Shape<D>;
-    constexpr int PG = S::PG;
+    constexpr int PG = S::PG, kBlocks = 2 * PG / kOperandWarps;  // CTAs of a tile
+    static_assert(kBlocks * kOperandWarps == 2 * PG, "a tile's pages");
     extern __shared__ __align__(128) uint8_t smem[];
-    __shared__ uint64_t bar[kOperandThreads / 32];
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, tile = blockIdx.x, head = blockIdx.y;
+    __shared__ uint64_t bar[kOperandWarps];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, head = blockIdx.y, s = blockIdx.z;
+    const int tile = blockIdx.x / kBlocks, j = blockIdx.x % kBlocks * kOperandWarps + warp, page = j % PG;
     int first, n;
-    const int s = blockIdx.z;
     rows_of(p, s, first, n);
     const int len = p.total_lens[s], limit = min(len, p.stride * kPageTokens);
     if (n == 0 || tile * S::NT >= limit || len > pre.tiles * S::NT) return;
     const size_t t = operand_tile<D>(p, pre, s, head, tile);
-    if (lane == 0) {
-        mbar_init(bar + warp, 1);
-        fence_barrier_init();
-        fence_proxy_async_shared();
+    uint8_t* buf = smem + warp * S::kPageBytes;
+    const int pos = tile * S::NT + page * kPageTokens, id = pos < limit ? page_at(p, s, pos) : -1;
+    if (id >= 0) {
+        if (lane == 0) {
+            mbar_init(bar + warp, 1);
+            fence_barrier_init();
+            fence_proxy_async_shared();
+            mbar_arrive_expect_tx(bar + warp, S::kPageBytes);
+            bulk_g2s(buf, head_rows<D>(p, id, j / PG, head), S::kPageBytes, bar + warp);
+        }
+        __syncwarp();
+        mbar_wait(bar + warp, 0, p.err);
+    }
+    const int valid = id >= 0 ? min(limit - pos, kPageTokens) : 0;
+    const float* src = reinterpret_cast<const float*>(buf);
+    uint8_t* to = pre.ops + t * (4 * S::kHalf);
+    constexpr int kPart = S::kPageBytes / 2;  // of the high halves, then of the low ones
+    if (j < PG) {
+        convert_k<D>(src, valid, buf, buf + kPart, 0, pre.scales + t * 16 + page);
+        to += page * kPart;
+    } else {
+        convert_v<D, kPageTokens>(src, valid, buf, buf + kPart, 0, pre.scales + t * 16 + 8 + page);
+        to += 2 * S::kHalf + page * 256;
     }
     __syncwarp();
-    int phase = 0;
-    float* src = reinterpret_cast<float*>(smem + 4 * S::kHalf + warp * S::kPageBytes);
-    for (int j = warp; j < 2 * PG; j += kOperandThreads / 32) {
-        const int page = j % PG, pos = tile * S::NT + page * kPageTokens;
-        const int id = pos < limit ? page_at(p, s, pos) : -1;
-        if (id >= 0) {
-            if (lane == 0) {
-                mbar_arrive_expect_tx(bar + warp, S::kPageBytes);
-                bulk_g2s(src, head_rows<D>(p, id, j / PG, head), S::kPageBytes, bar + warp);
-            }
-            mbar_wait(bar + warp, phase, p.err);
-            phase ^= 1;
-        }
-        const int valid = id >= 0 ? min(limit - pos, kPageTokens) : 0;
-        if (j < PG)
-            convert_k<D>(src, valid, smem, smem + S::kHalf, page, pre.scales + t * 16 + page);
-        else
-            convert_v<D>(src, valid, smem + 2 * S::kHalf, smem + 3 * S::kHalf, page, pre.scales + t * 16 + 8 + page);
-        fence_proxy_async_shared();  // the page's buffer takes the next copy
-        __syncwarp();
+#pragma unroll 4
+    for (int i = lane; i < kPart / 16; i += 32) {
+        const int at = j < PG ? i * 16 : i / 16 * (16 * S::NT) + i % 16 * 16;  // V: 256 bytes of every 8 dims
+        *reinterpret_cast<uint4*>(to + at) = *reinterpret_cast<const uint4*>(buf + i * 16);
+        *reinterpret_cast<uint4*>(to + S::kHalf + at) = *reinterpret_cast<const uint4*>(buf + kPart + i * 16);
     }
-    __syncthreads();
-    const uint4* from = reinterpret_cast<const uint4*>(smem);
-    uint4* to = reinterpret_cast<uint4*>(pre.ops + t * (4 * S::kHalf));
-    for (int i = threadIdx.x; i < 4 * S::kHalf / 16; i += kOperandThreads) to[i] = from[i];
 }
 
 // The launches for a call's bounds, and their workspace: partial sums, what is
@@ -1077,11 +1082,12 @@ cudaError_t launch_chunk(ChunkParams p, const ChunkPlan& plan, void* workspace, 
     ChunkSplit* splits = reinterpret_cast<ChunkSplit*>(w + plan.splits);
     const Operands pre{w + plan.operands, reinterpret_cast<float*>(w + plan.scales), plan.operand_tiles};
     if (plan.operand_tiles) {
-        const size_t smem = 4 * Shape<D>::kHalf + (kOperandThreads / 32) * Shape<D>::kPageBytes;
+        const size_t smem = kOperandWarps * Shape<D>::kPageBytes;
         e = chunk_kernel_attributes<chunk_operands_kernel<D>>(smem, 0);
         if (e != cudaSuccess) return e;
-        chunk_operands_kernel<D><<<dim3((unsigned)plan.operand_tiles, (unsigned)p.Hkv, (unsigned)p.batch),
-                                   kOperandThreads, smem, stream>>>(p, pre);
+        const unsigned blocks = (unsigned)plan.operand_tiles * (2 * Shape<D>::PG / kOperandWarps);
+        chunk_operands_kernel<D><<<dim3(blocks, (unsigned)p.Hkv, (unsigned)p.batch), kOperandWarps * 32, smem, stream>>>(
+            p, pre);
         e = cudaGetLastError();
         if (e == cudaSuccess) e = launch_tiles<D, true>(p, plan, partials, splits, pre, stream);
     } else {
