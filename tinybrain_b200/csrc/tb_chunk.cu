@@ -1006,14 +1006,18 @@ ChunkPlan chunk_plan(long long rows, long long batch, long long max_new, long lo
     }
     const int few_shares = c.few_ctas * (d == 128 ? 8 : 16);
     if (many) c.ctas = ctas(per);
-    // Made beforehand where every K and V tile is read by kPreReuse row tiles or
-    // more (as far as the bounds tell) and the operands fit kPreBytes.  Measured:
-    // 1.6 row tiles (D = 128) 290 us without, 333 with; 4 (D = 64) 29 and 31; 128
-    // (D = 64) 750 and 400.
-    constexpr long long kPreReuse = 8, kPreBytes = 1ll << 30;
+    // Made beforehand where every K and V tile is read by so many row tiles or more
+    // (as far as the bounds tell), a CTA has some tiles to pay for the launch, and the
+    // operands fit kPreBytes.  Measured, us without / with:
+    //   D = 128: 2 row tiles 222 / 191 and 130 / 119, 4 370 / 282 and 199 / 140
+    //   D = 64:  2 row tiles 84 / 90 and 62 / 67, 4 80 / 77 and 217 / 187; of a CTA's
+    //            two tiles, 4 row tiles 36 / 38
+    const long long reuse = d == 128 ? 2 : 4;
+    constexpr long long kPreTiles = 4, kPreBytes = 1ll << 30;
     const long long tile_bytes = 8 * nt * d + 64;
     const bool fits = batch <= 65535 && len_tiles <= (1 << 24) && batch * Hkv * len_tiles <= kPreBytes / tile_bytes;
-    if (many && fits && rows / per >= kPreReuse * batch) c.operand_tiles = (int)len_tiles;
+    if (many && fits && rows / per >= reuse * batch && rows / per * most(Hkv) * len_tiles >= kPreTiles * kChunkCtas)
+        c.operand_tiles = (int)len_tiles;
     const long long all_tiles = batch * Hkv * c.operand_tiles;
     const auto up = [](size_t n) { return (n + 127) & ~(size_t)127; };
     c.splits = c.ctas * 2 * partial_floats(kTileRows, d) * sizeof(float);
