@@ -298,8 +298,9 @@ tb_status tb_paged_attention_chunk_dev(void *stream, const float *q_dev, int64_t
  * largest (<= 0 off).  The token is the first kept index whose running mass
  * exceeds uniform times the kept mass.  prob_dev and entropy_dev (NULL or
  * [rows]) get the token's probability and the entropy (nats) of the kept
- * distribution, as TokenOutput has them.  NaN counts as -inf; a row with
- * nothing above -inf gets token -1, probability and entropy 0.  The order of
+ * distribution, as TokenOutput has them.  NaN counts as -inf, a weight below
+ * e^-700 of the largest as 0; a row with nothing above -inf gets token -1,
+ * probability and entropy 0.  The order of
  * the steps is not tb_runner_set_sampler's, which follows the reference: there
  * the temperature comes last, top_p applies only without top_k, and there is
  * no min_p. */

@@ -302,6 +302,17 @@ def test_chunk_attention(serving, H, kv, d, total, new):
     check_attend(serving, attend_case(len(total) + H + d, total, new, H, kv, d, extra_rows=2))
 
 
+@pytest.mark.parametrize("H,kv,d", [(16, 2, 64), (8, 4, 128), (4, 4, 16), (32, 4, 32)])
+@pytest.mark.parametrize("hint", [None, 1])
+def test_chunk_attention_of_few_tokens_over_few_pages(serving, H, kv, d, hint):
+    # one CTA a unit: from no position to two pages a warp; with `hint` more units than the bounds tell
+    total = [1, 16, 17, 129, 255, 256, 3, 0, 200, 90]
+    new = [1, 0, 1, 1, 1, 1, 3, 0, 1, 1] if hint is None else [1, 0, 8, 5, 1, 3, 3, 0, 1, 7]
+    c = attend_case(d, total, new, H, kv, d, evict=[(3, 0), (3, 8), (8, 12)], extra_rows=2)
+    check_attend(serving, c, max_new=hint, max_len=hint and 256)
+    serving.check_device()
+
+
 @pytest.mark.parametrize("H,kv,d,total,new", [
     (4, 4, 64, [2100], [1100]), (4, 4, 128, [1500], [1069]), (16, 2, 64, [2049, 300, 1025], [203, 5, 180]),
     (8, 4, 128, [700, 1300], [520, 581]), (4, 4, 32, [1700], [1041]), (8, 8, 16, [1100], [1100])])

@@ -36,8 +36,8 @@ namespace {
 //   converters (8 warps) the K and the V page of 16 tokens at a time: a page's
 //              largest magnitude gives a power-of-two scale, the halves go to the
 //              operand tiles;
-//   issuer     one thread: S(i + 1) before P V(i), so the softmax of a tile runs
-//              while the tensor cores do the next S and the last P V;
+//   issuer     one thread: S(i + 1) (or i + 2) before P V(i), so the softmax of a tile
+//              runs while the tensor cores do the next S and the last P V;
 //   softmax    a warpgroup, a row a thread: base-2 softmax over the tile, P as
 //              halves over S in tensor memory, and the P V of the last tile added
 //              to the row's sums in registers, which are rescaled only where the
@@ -46,7 +46,17 @@ namespace {
 // the producer copies operand tiles, and a second softmax warpgroup takes the
 // odd tiles: one warp per scheduler waits for its own instructions, two fill
 // each other's gaps.  Each keeps its own maximum and sums, and at a unit's end
-// the odd one hands its to the even one, which writes the unit.
+// the odd one hands its to the even one, which writes the unit.  Tensor memory
+// then holds three S and one O: S runs two tiles ahead, so that a warpgroup finds
+// its next tile ready (two of each: 391 us for the prompt below), and O is read
+// before the weights of the next tile are formed.
+//
+// Bound by the softmax warps' instructions (a weight takes an exponential, two
+// conversions and some ten others).  Measured: 2048 tokens over 8192 positions, 32
+// query and 4 KV heads of 64, 322 us, 0.67 of the three products' time at the
+// measured 1679 TFLOP/s; 8 us for the operands.  Converted by the CTAs that read
+// them, 713 tokens of seven sequences of 664 to 1694, 32 heads of 128: 290 us; 64
+// tokens over 1920, 32 and 4 heads of 64: 29 us.
 //
 // With c the row's scale times the page's, a score is c S and a weighted value
 // 2^(c S - M) v = 2^(c S + e - M) (v 2^-e): the page's value exponent e enters
@@ -979,6 +989,7 @@ __global__ void __launch_bounds__(kOperandWarps * 32) chunk_operands_kernel(Chun
 // The launches for a call's bounds, and their workspace: partial sums, what is
 // split, and the operands where they are made beforehand.
 struct ChunkPlan {
+    bool whole;          // chunk_few_kernel by whole units
     int ctas, few_ctas;  // one per tile of work that the bounds allow, at most one per SM; 0: not launched
     int operand_tiles;   // of a sequence, 0: converted by the CTAs that read them
     size_t splits, few, few_splits, operands, scales, bytes;  // offsets, and all of it
@@ -990,6 +1001,7 @@ ChunkPlan chunk_plan(long long rows, long long batch, long long max_new, long lo
         const long long units = std::min(batch * ((std::min(max_new, rows) + tokens - 1) / tokens), batch + rows / tokens);
         return (int)std::max<long long>(1, most(most(units) * most(Hkv) * most(len_tiles)));
     };
+    constexpr int kWholePages = 2;
     ChunkPlan c{};
     // Sequences with at most eight rows of a KV head go to chunk_few_kernel.  Where
     // the bounds say that all have so few it takes them all, where they say that
@@ -1003,8 +1015,16 @@ ChunkPlan chunk_plan(long long rows, long long batch, long long max_new, long lo
         const auto many_pages = [](long long n) { return std::min<long long>(n, 1 << 16); };
         const long long pages = many_pages(units) * many_pages(Hkv) * many_pages((max_len + kPageTokens - 1) / kPageTokens);
         c.few_ctas = (int)std::max<long long>(1, most((pages + kFewPages - 1) / kFewPages));
+        // A CTA takes whole units, and nothing is left to join, where a warp then has
+        // kWholePages or fewer.  Measured, us by shares / by units, one sequence of 4 KV
+        // heads of 64: 129 tokens (1 page) 16.9 / 10.2, 256 (1) 13.0 / 11.7, 512 (2) 13.4 /
+        // 14.3, 1024 (4) 14.6 / 19.4; 9 sequences of 16 heads: 512 18.7 / 16.3, 1024 28 / 22.
+        const int warps = d == 128 ? 8 : 16;
+        c.whole = !many && units <= kChunkCtas && units * Hkv <= kChunkCtas &&
+                  max_len <= (long long)kWholePages * warps * kPageTokens;
+        if (c.whole) c.few_ctas = (int)(units * Hkv);
     }
-    const int few_shares = c.few_ctas * (d == 128 ? 8 : 16);
+    const int few_shares = c.whole ? 0 : c.few_ctas * (d == 128 ? 8 : 16);
     if (many) c.ctas = ctas(per);
     // Made beforehand where every K and V tile is read by so many row tiles or more
     // (as far as the bounds tell), a CTA has some tiles to pay for the launch, and the
@@ -1072,9 +1092,15 @@ cudaError_t launch_chunk(ChunkParams p, const ChunkPlan& plan, void* workspace, 
         float* partials = reinterpret_cast<float*>(w + plan.few);
         ChunkSplit* splits = reinterpret_cast<ChunkSplit*>(w + plan.few_splits);
         p.rows_upto = plan.ctas ? kFewRows : INT_MAX;
-        e = chunk_kernel_attributes<chunk_few_kernel<D>>(Few<D>::kSmem, 0);
+        if (plan.whole) {
+            e = chunk_kernel_attributes<chunk_few_kernel<D, true>>(Few<D>::kSmem, 0);
+            if (e != cudaSuccess) return e;
+            chunk_few_kernel<D, true><<<plan.few_ctas, Few<D>::kThreads, Few<D>::kSmem, stream>>>(p, nullptr, nullptr);
+            return cudaGetLastError();
+        }
+        e = chunk_kernel_attributes<chunk_few_kernel<D, false>>(Few<D>::kSmem, 0);
         if (e != cudaSuccess) return e;
-        chunk_few_kernel<D><<<plan.few_ctas, Few<D>::kThreads, Few<D>::kSmem, stream>>>(p, partials, splits);
+        chunk_few_kernel<D, false><<<plan.few_ctas, Few<D>::kThreads, Few<D>::kSmem, stream>>>(p, partials, splits);
         e = cudaGetLastError();
         if (e == cudaSuccess)
             e = launch_combine<D, kFewRows>(p, plan.few_ctas * Few<D>::kWarps, partials, splits, wide_output(p), stream);
@@ -1143,7 +1169,8 @@ extern "C" tb_status tb_paged_attention_chunk_dev(void* stream, const float* q, 
     TB_ENTRY_CHECK(aligned_to(pool, 16), "kv_pool must be 16-byte aligned");
     if (rows == 0) return TB_OK;
     const ChunkPlan plan = chunk_plan(rows, batch, max_new, max_len, H, Hkv, d);
-    TB_ENTRY_CHECK(workspace && aligned_to(workspace, 16) && workspace_bytes >= (int64_t)plan.bytes,
+    TB_ENTRY_CHECK(plan.bytes == 0 ||
+                       (workspace && aligned_to(workspace, 16) && workspace_bytes >= (int64_t)plan.bytes),
                    "the workspace must be 16-byte aligned and hold %lld bytes", (long long)plan.bytes);
     StreamEntry entry(pool, "kv_pool");
     if (entry.status != TB_OK) return entry.status;

@@ -5,7 +5,8 @@
 // empty, and making its operands costs more than the products.  Here every warp
 // takes an equal share of all pages of all units, streams them through its own
 // ring of bulk copies and waits for no other warp; units that several warps hold
-// are joined by chunk_combine_kernel.  (Sixteen warps on one unit, joined at its
+// are joined by chunk_combine_kernel.  WHOLE, for little work: the warps of a CTA
+// share a unit's pages and join them at its end, without the second launch.  (Sixteen warps on one unit, joined at its
 // end, spent a fifth of their time at that barrier.)  Per page of 16 tokens:
 //   scores  mma.sync m16n8k8 on the fp32 page as it lies: A = 16 tokens, B = the
 //           rows' queries from registers, both split into a TF32 high part and
@@ -14,6 +15,9 @@
 //           it by 2^8 (one vote a page);
 //   sums    V in plain fp32 FMAs: a lane holds D / 32 dims of all rows, a row of
 //           V is one conflict-free load, the weights are broadcast loads.
+// Bound by issue slots beside HBM.  Measured: 64 sequences of 512 to 4224 tokens, 32
+// query and 4 KV heads of 64, 73 us for 290 MB, 4.0 TB/s; WHOLE, one token over 129
+// positions, 10 us with its launch.
 // The dims of a lane in the scores' products are four neighbours: k is a label,
 // the same for A and B.
 #pragma once
@@ -95,7 +99,7 @@ struct WarpPages {
     __device__ __forceinline__ int id() const { return __shfl_sync(0xffffffffu, ids, page - base); }
 };
 
-template <int D>
+template <int D, bool WHOLE>
 __global__ void __launch_bounds__(Few<D>::kThreads, 1)
     chunk_few_kernel(ChunkParams p, float* partials, ChunkSplit* splits) {
     using F = Few<D>;
@@ -112,14 +116,21 @@ __global__ void __launch_bounds__(Few<D>::kThreads, 1)
         fence_proxy_async_shared();
     }
 
-    // ---- the warp's share of all units' pages: shares w, w + CTAs, ... fall to one CTA,
-    //      so that few pages spread over the SMs ----
+    // ---- the work: the warp's share of all units' pages (shares w, w + CTAs, ... fall to
+    //      one CTA, so that few pages spread over the SMs), or WHOLE the CTA's units ----
+    const int G = p.H / p.Hkv, per = kFewRows / G;
     const int run = (p.batch + F::kThreads - 1) / F::kThreads;
+    const auto work_of = [&](int s) -> long long {
+        if (!WHOLE) return tiles_of_sequence<kPageTokens, kFewRows>(p, s);
+        int first, n;
+        rows_of(p, s, first, n);
+        return (long long)((n + per - 1) / per) * p.Hkv;
+    };
     long long mine = 0;
     {
         const int s0 = min(tid * run, p.batch), s1 = min(s0 + run, p.batch);
         for (int s = s0; s < s1; ++s) {
-            mine += tiles_of_sequence<kPageTokens, kFewRows>(p, s);
+            mine += work_of(s);
             int first, n;
             rows_of(p, s, first, n);
             if (n && p.total_lens[s] > p.stride * kPageTokens) record_error(p.err, kDevBadPage);
@@ -141,17 +152,15 @@ __global__ void __launch_bounds__(Few<D>::kThreads, 1)
     sh.before[tid] = upto - mine;
     sh.mine[tid] = mine;
     __syncthreads();
-    pdl_launch_dependents();
-    share.index = warp * gridDim.x + blockIdx.x;
+    if (!WHOLE) pdl_launch_dependents();
+    share.index = WHOLE ? blockIdx.x : warp * gridDim.x + blockIdx.x;
     share.shares = min((long long)gridDim.x * F::kWarps, (share.total + kFewPages - 1) / kFewPages);
-    if (share.index >= share.shares) {
-        if (lane == 0) splits[share.index] = ChunkSplit{-1};
+    if (share.index >= (WHOLE ? share.total : share.shares)) {
+        if (!WHOLE && lane == 0) splits[share.index] = ChunkSplit{-1};
         return;
     }
-    const long long begin = share.total * share.index / share.shares;
-    share.end = share.total * (share.index + 1) / share.shares;
     WarpPages fetch, now;
-    {
+    const auto seek = [&](long long begin) {  // the unit that holds it, and the place in its sequence's work
         int holder = 0;
         for (int t = lane; t < F::kThreads; t += 32) {
             const bool has = sh.before[t] <= begin && begin < sh.before[t] + sh.mine[t];
@@ -161,11 +170,18 @@ __global__ void __launch_bounds__(Few<D>::kThreads, 1)
         long long at = begin - sh.before[holder];
         Unit& u = now.u;
         for (u.s = holder * run;; ++u.s) {
-            const long long here = run == 1 ? LLONG_MAX : tiles_of_sequence<kPageTokens, kFewRows>(p, u.s);
+            const long long here = run == 1 ? LLONG_MAX : work_of(u.s);
             if (at < here) break;
             at -= here;
         }
         set_sequence(p, u);
+        return at;
+    };
+    if (!WHOLE) {
+        const long long begin = share.total * share.index / share.shares;
+        share.end = share.total * (share.index + 1) / share.shares;
+        long long at = seek(begin);
+        Unit& u = now.u;
         for (u.tile = 0;; ++u.tile) {
             set_tile<kPageTokens, kFewRows>(p, u);
             if (at < (long long)u.tiles * p.Hkv) break;
@@ -176,11 +192,10 @@ __global__ void __launch_bounds__(Few<D>::kThreads, 1)
         now.piece(p, (int)(at % u.tiles));
         fetch = now;
     }
-    const int G = p.H / p.Hkv, per = kFewRows / G;
     ChunkSplit split{-1};
 
     // K and V pages alternate through the ring; `fetch` runs ahead of `now`
-    bool more = true;
+    bool more = !WHOLE;
     int fetch_kv = 0, fetch_slot = 0, held = 0;  // held: pages fetched and not yet read
     int slot = 0, phase = 0;
     const auto fill = [&]() {
@@ -216,9 +231,25 @@ __global__ void __launch_bounds__(Few<D>::kThreads, 1)
         }
         fill();
     };
-    fill();
+    // a WHOLE unit's partial sums, one warp's after the other's, over the ring
+    float* const parts = reinterpret_cast<float*>(smem);
+    constexpr int kPartStride = F::kSmem / F::kWarps / sizeof(float);
+    static_assert(kPartStride >= (int)partial_floats(kFewRows, D), "a warp's sums in its ring");
 
     do {
+        if (WHOLE) {  // pages T w / warps to T (w + 1) / warps of the CTA's unit
+            const long long at = seek(share.index);
+            Unit& u = now.u;
+            u.tile = (int)(at / p.Hkv);
+            u.head = (int)(at % p.Hkv);
+            set_tile<kPageTokens, kFewRows>(p, u);
+            const int begin = (int)((long long)u.tiles * warp / F::kWarps);
+            now.left = (int)((long long)u.tiles * (warp + 1) / F::kWarps) - begin;
+            more = now.left > 0;
+            now.piece(p, begin);
+            fetch = now;
+        }
+        fill();
         const Unit& u = now.u;
         const int from = now.page;
         // the rows' queries, times log2(e) / sqrt(D): B fragments (k = dims, n = rows)
@@ -379,11 +410,14 @@ __global__ void __launch_bounds__(Few<D>::kThreads, 1)
         wild = __any_sync(0xffffffffu, wild);
         const bool whole = from == 0 && now.end == u.tiles;
         float* part = nullptr;
-        if (!whole) {
+        if (WHOLE) {
+            part = parts + warp * kPartStride;
+        } else if (!whole) {
             part = partials + (share.index * 2 + (from == 0)) * partial_floats(kFewRows, D);
             if (from == 0) split = split_of<kFewRows>(p, u, share.followers(u.tiles - now.end));
         }
-        if (wild) {
+        if (WHOLE && from == now.end) {  // no page
+        } else if (wild) {
             for (int r = 0; r < rows; ++r)
                 row_in_fp32<D, kFewRows>(p, u, r, from * kPageTokens, now.end * kPageTokens, part, 0.0f);
         } else {
@@ -410,8 +444,35 @@ __global__ void __launch_bounds__(Few<D>::kThreads, 1)
                 }
             }
         }
-    } while (now.next_piece(p));
-    if (lane == 0) splits[share.index] = split;
+        if (WHOLE) {
+            __syncthreads();
+            for (int e = tid; e < kFewRows * D / 4; e += F::kThreads) {
+                const int r = e / (D / 4), d4 = e % (D / 4) * 4;
+                if (r >= rows) continue;
+                CombineSum<D> sum;
+                sum.clear();
+#pragma unroll 4
+                for (int w = 0; w < F::kWarps; ++w) {
+                    const float* at = parts + w * kPartStride;
+                    if ((long long)u.tiles * w / F::kWarps < (long long)u.tiles * (w + 1) / F::kWarps)
+                        sum.add(0, at[kFewRows * D + r], at[kFewRows * (D + 1) + r],
+                                *reinterpret_cast<const float4*>(at + r * D + d4));
+                }
+                const float f = 1.0f / sum.l[0];
+                const bool some = held_tokens + r / G + 1 > 0;
+                float* dst = p.out + (u.first + u.tile * per + r / G) * p.ld_out + (size_t)(u.head * G + r % G) * D + d4;
+                dst[0] = some ? sum.sum[0].x * f : 0.0f;
+                dst[1] = some ? sum.sum[0].y * f : 0.0f;
+                dst[2] = some ? sum.sum[0].z * f : 0.0f;
+                dst[3] = some ? sum.sum[0].w * f : 0.0f;
+            }
+            share.index += gridDim.x;
+            if (share.index >= share.total) break;
+            fence_proxy_async_shared();  // the ring takes copies again
+            __syncthreads();
+        }
+    } while (WHOLE || now.next_piece(p));
+    if (!WHOLE && lane == 0) splits[share.index] = split;
     if (sh.dead) land_copies();
 }
 

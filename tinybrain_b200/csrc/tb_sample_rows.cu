@@ -20,12 +20,17 @@
 // A row is read once, by a cluster of P CTAs (P = 1, 2, 4, 8) that keep it in
 // shared memory, each of their warps a run of consecutive elements.  A truncated
 // row then takes one histogram of 2048 bins over (m - x) / T -- counts for top-k,
-// masses for top-p -- and the elements of the one bin that holds the boundary,
-// which every CTA ranks for itself (no sort: a select needs the boundary, not the
-// order).  A bin of more elements than the list holds is narrowed by histograms
-// over its keys.  Last come the kept masses and the search in the run that holds
-// the draw.  Bound by the steps' latency for few rows, by the fp64 exponentials
-// and the histogram's atomics for many.
+// then masses of what that leaves for top-p -- and the elements of the one bin
+// that holds the boundary, which are ranked (no sort: a select needs the boundary,
+// not the order).  A bin of more elements than the list holds is narrowed by
+// histograms over its keys.  Last come the kept masses, run by run, and the search
+// in the run that holds the draw.  What the CTAs tell one another they push into
+// each other's shared memory ahead of a barrier, after which it is read locally.
+//
+// Bound by the barriers' and reads' latency for few rows, by instruction issue for
+// many.  Measured: one row of 32000 11 us, 64 rows 24 us; 256 rows of 131072, each
+// with its own settings, 162 us (0.8 TB/s); greedy alone 43 us, without truncation
+// 113, top-p 0.9 254.
 #include <cfloat>
 #include <climits>
 
@@ -775,7 +780,9 @@ extern "C" tb_status tb_sample_rows_dev(void* stream, const float* logits, int64
     const RowsParams p{logits, ld, V, std::ldexp(1.0, 62 - log_v), temperature, top_k, top_p, min_p, uniform, token,
                        prob, entropy};
     // CTAs of a row: while the rows leave SMs idle and a CTA would still have 2048
-    // elements to read, or while a CTA's part leaves no room for others on its SM
+    // elements to read, or while a CTA's part leaves no room for others on its SM.
+    // Measured, us: one row of 32000 P = 1 31, 2 21, 4 16, 8 14; 64 rows 62, 41, 35,
+    // 43; 256 rows of 131072 P = 4 267, 8 222
     int P = 1;
     while (P < kMaxCluster &&
            (((long long)rows * P < entry.num_sms && V / (2 * P) >= 2048) || V / P > 16 * 1024))
