@@ -8,8 +8,6 @@
 // Rows of an evicted page (table entry -1) are zeros, as in the decode
 // attention (ModelRunner.swift:519-579 over KVCache.swift's pages).
 #include "tb_chunk_mma.cuh"
-#include <atomic>
-
 #include "tb_chunk_few.cuh"
 #include "tb_chunk_units.cuh"
 
@@ -1049,35 +1047,13 @@ ChunkPlan chunk_plan(long long rows, long long batch, long long max_new, long lo
     return c;
 }
 
-// Once per kernel and device (the calls cost more than a launch).  K names the
-// kernel: each has its own record.
-template <auto K>
-cudaError_t chunk_kernel_attributes(size_t smem, int regs) {
-    static std::atomic<uint64_t> done{0};
-    int dev = 0;
-    cudaError_t e = cudaGetDevice(&dev);
-    if (e != cudaSuccess || (dev < 64 && done.load(std::memory_order_relaxed) >> dev & 1)) return e;
-    e = cudaFuncSetAttribute(K, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-    if (e != cudaSuccess) return e;
-    if (regs) {
-        // setmaxnreg moves registers within what the CTA was launched with: with
-        // fewer than planned the softmax warps would wait for them
-        cudaFuncAttributes a{};
-        e = cudaFuncGetAttributes(&a, K);
-        if (e != cudaSuccess) return e;
-        if (a.numRegs != regs) return cudaErrorNotSupported;
-    }
-    if (dev < 64) done.fetch_or(1ull << dev, std::memory_order_relaxed);
-    return cudaSuccess;
-}
-
 bool wide_output(const ChunkParams& p) { return p.ld_out % 4 == 0 && aligned_to(p.out, 16); }
 
 template <int D, bool PRE>
 cudaError_t launch_tiles(const ChunkParams& p, const ChunkPlan& plan, float* partials, ChunkSplit* splits,
                          const Operands& pre, cudaStream_t stream) {
     const bool wide_q = p.ld_q % 4 == 0 && aligned_to(p.q, 16), wide_out = wide_output(p);
-    cudaError_t e = chunk_kernel_attributes<chunk_tiles_kernel<D, PRE>>(Shape<D>::template kSmem<PRE>, Roles<PRE>::kLaunchRegs);
+    cudaError_t e = kernel_attributes<chunk_tiles_kernel<D, PRE>>(Shape<D>::template kSmem<PRE>, Roles<PRE>::kLaunchRegs);
     if (e != cudaSuccess) return e;
     chunk_tiles_kernel<D, PRE><<<plan.ctas, Roles<PRE>::kThreads, Shape<D>::template kSmem<PRE>, stream>>>(p, partials, splits, pre,
                                                                                                wide_q, wide_out);
@@ -1093,12 +1069,12 @@ cudaError_t launch_chunk(ChunkParams p, const ChunkPlan& plan, void* workspace, 
         ChunkSplit* splits = reinterpret_cast<ChunkSplit*>(w + plan.few_splits);
         p.rows_upto = plan.ctas ? kFewRows : INT_MAX;
         if (plan.whole) {
-            e = chunk_kernel_attributes<chunk_few_kernel<D, true>>(Few<D>::kSmem, 0);
+            e = kernel_attributes<chunk_few_kernel<D, true>>(Few<D>::kSmem);
             if (e != cudaSuccess) return e;
             chunk_few_kernel<D, true><<<plan.few_ctas, Few<D>::kThreads, Few<D>::kSmem, stream>>>(p, nullptr, nullptr);
             return cudaGetLastError();
         }
-        e = chunk_kernel_attributes<chunk_few_kernel<D, false>>(Few<D>::kSmem, 0);
+        e = kernel_attributes<chunk_few_kernel<D, false>>(Few<D>::kSmem);
         if (e != cudaSuccess) return e;
         chunk_few_kernel<D, false><<<plan.few_ctas, Few<D>::kThreads, Few<D>::kSmem, stream>>>(p, partials, splits);
         e = cudaGetLastError();
@@ -1113,7 +1089,7 @@ cudaError_t launch_chunk(ChunkParams p, const ChunkPlan& plan, void* workspace, 
     const Operands pre{w + plan.operands, reinterpret_cast<float*>(w + plan.scales), plan.operand_tiles};
     if (plan.operand_tiles) {
         const size_t smem = kOperandWarps * Shape<D>::kPageBytes;
-        e = chunk_kernel_attributes<chunk_operands_kernel<D>>(smem, 0);
+        e = kernel_attributes<chunk_operands_kernel<D>>(smem);
         if (e != cudaSuccess) return e;
         const unsigned blocks = (unsigned)plan.operand_tiles * (2 * Shape<D>::PG / kOperandWarps);
         chunk_operands_kernel<D><<<dim3(blocks, (unsigned)p.Hkv, (unsigned)p.batch), kOperandWarps * 32, smem, stream>>>(

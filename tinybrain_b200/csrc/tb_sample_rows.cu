@@ -753,9 +753,7 @@ cudaError_t launch_rows(const RowsParams& p, int rows, cudaStream_t stream) {
     cfg.attrs = attr;
     cfg.numAttrs = 1;
     cudaError_t e = cudaSuccess;
-    if (smem + sizeof(RowShared) > 48 * 1024)  // what needs no asking
-        e = cudaFuncSetAttribute(sample_rows_kernel<P, STAGED>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                 kStagedMax * (int)sizeof(float));
+    if (STAGED) e = kernel_attributes<sample_rows_kernel<P, STAGED>>(kStagedMax * sizeof(float));
     if (e == cudaSuccess) e = cudaLaunchKernelEx(&cfg, sample_rows_kernel<P, STAGED>, p);
     return e;
 }

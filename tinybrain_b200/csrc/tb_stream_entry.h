@@ -5,6 +5,7 @@
 // (tb_paged_attention_noalloc_status).
 #pragma once
 
+#include <atomic>
 #include "../../include/tinybrain_cuda.h"
 #include "tb_kernels.h"
 
@@ -65,6 +66,29 @@ inline tb_status launch_status(cudaError_t e, const char* what) {
     if (e == cudaSuccess) return TB_OK;
     return (tb_status)report_error(e == cudaErrorNotSupported ? TB_ERR_UNSUPPORTED : TB_ERR_CUDA, "%s: %s", what,
                                    cudaGetErrorString(e));
+}
+
+// Lets kernel K have `smem` bytes of dynamic shared memory, once per kernel and
+// device (the calls cost more than a launch); K names the kernel, each has its own
+// record.  regs: the registers of a thread that K must have been built with.
+template <auto K>
+cudaError_t kernel_attributes(size_t smem, int regs = 0) {
+    static std::atomic<uint64_t> done{0};
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess || (dev < 64 && done.load(std::memory_order_relaxed) >> dev & 1)) return e;
+    e = cudaFuncSetAttribute(K, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (e != cudaSuccess) return e;
+    if (regs) {
+        // setmaxnreg moves registers within what the CTA was launched with: with
+        // fewer than planned the warps that ask for more would wait for them
+        cudaFuncAttributes a{};
+        e = cudaFuncGetAttributes(&a, K);
+        if (e != cudaSuccess) return e;
+        if (a.numRegs != regs) return cudaErrorNotSupported;
+    }
+    if (dev < 64) done.fetch_or(1ull << dev, std::memory_order_relaxed);
+    return cudaSuccess;
 }
 
 inline bool aligned_to(const void* p, size_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
