@@ -198,22 +198,29 @@ __global__ void __launch_bounds__(Few<D>::kThreads, 1)
     bool more = !WHOLE;
     int fetch_kv = 0, fetch_slot = 0, held = 0;  // held: pages fetched and not yet read
     int slot = 0, phase = 0;
-    const auto fill = [&]() {
-        while (more && held < kRing && !sh.dead) {
-            const int id = fetch.id();
-            if (lane == 0) {
-                uint64_t* bar = &sh.full[warp][fetch_slot];
-                sh.id[warp][fetch_slot] = id;
-                mbar_arrive_expect_tx(bar, id >= 0 ? F::kPageBytes : 0);
-                if (id >= 0)
-                    bulk_g2s(ring + fetch_slot * F::kPageBytes, head_rows<D>(p, id, fetch_kv, fetch.u.head),
-                             F::kPageBytes, bar);
-            }
-            ++held;
-            if (++fetch_slot == kRing) fetch_slot = 0;
-            if (fetch_kv) more = fetch.next_page(p);
-            fetch_kv ^= 1;
+    const size_t page_floats = (size_t)p.num_layers * 2 * p.Hkv * (kPageTokens * D);
+    const float* fetch_at = nullptr;  // page 0's rows of fetch's head, K
+    int fetch_id = -1;
+    const auto fetch_next = [&]() {
+        if (fetch_kv == 0) {
+            fetch_id = fetch.id();
+            fetch_at = head_rows<D>(p, 0, 0, fetch.u.head);
         }
+        if (lane == 0) {
+            uint64_t* bar = &sh.full[warp][fetch_slot];
+            sh.id[warp][fetch_slot] = fetch_id;
+            mbar_arrive_expect_tx(bar, fetch_id >= 0 ? F::kPageBytes : 0);
+            if (fetch_id >= 0)
+                bulk_g2s(ring + fetch_slot * F::kPageBytes,
+                         fetch_at + fetch_id * page_floats + (fetch_kv ? p.Hkv * (kPageTokens * D) : 0), F::kPageBytes,
+                         bar);
+        }
+        if (++fetch_slot == kRing) fetch_slot = 0;
+        if (fetch_kv) more = fetch.next_page(p);
+        fetch_kv ^= 1;
+    };
+    const auto fill = [&]() {
+        for (; more && held < kRing; ++held) fetch_next();
     };
     // the next page in the ring; its pool page (-1: zeros)
     const auto take_page = [&](const float*& rows) {
@@ -224,12 +231,14 @@ __global__ void __launch_bounds__(Few<D>::kThreads, 1)
     };
     const auto done_page = [&]() {
         __syncwarp();
-        --held;
         if (++slot == kRing) {
             slot = 0;
             phase ^= 1;
         }
-        fill();
+        if (more && !sh.dead)
+            fetch_next();
+        else
+            --held;
     };
     // a WHOLE unit's partial sums, one warp's after the other's, over the ring
     float* const parts = reinterpret_cast<float*>(smem);
