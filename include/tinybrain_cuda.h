@@ -242,7 +242,7 @@ typedef enum {
  * A step that does not fit takes no page and has no rows: info_dev holds 0, 0
  * and the status, row_offsets_dev zeros, total_lens_dev the cached lengths, and
  * the rest stays as it was.  The pages taken are the caller's to remove from
- * its list. */
+ * its list.  No output may overlap an input. */
 tb_status tb_page_tables_build_dev(void *stream, const int32_t *cached_lens_dev, const int32_t *new_lens_dev,
                                    int32_t batch, const int32_t *free_pages_dev, int32_t num_free,
                                    int32_t *page_table_dev, int32_t ptab_stride, int32_t max_rows,
@@ -274,7 +274,7 @@ tb_status tb_rope_append_paged_dev(void *stream, const float *q_dev, int64_t ld_
  * (its new tokens included, already in the cache) attends over positions
  * 0 .. total - n + i, scaled by 1 / sqrt(head_dim); rows of evicted pages are
  * zeros, as in tb_paged_attention_dev, and a row with no position gets zeros.
- * `rows` is what q_dev and out_dev hold; max_new and max_len bound a sequence's
+ * `rows` is what q_dev and out_dev hold (out_dev may be q_dev); max_new and max_len bound a sequence's
  * new tokens and length for the launch's shape only (larger ones stay right).
  * The workspace is tb_paged_attention_chunk_workspace bytes of device memory,
  * 16-byte aligned, for this call's use until it has run: calls that may overlap

@@ -101,6 +101,19 @@ def test_page_tables(serving, batch, most, longest, room):
         assert (o[name][rows:] == -7).all(), name  # behind the last row
 
 
+@pytest.mark.parametrize("cut", [(1, 0), (0, 3), (2, 1)])
+def test_page_tables_from_lengths_at_any_address(serving, cut):
+    cached, new, free, table = tables_case(8, 2100, 7, 60)
+    want_table, off, total, *_ = tables_numpy(cached, new, free, table)
+    lens = [torch.cat([torch.zeros(k, dtype=torch.int32, device="cuda"), dev(x)])[k:] for k, x in zip(cut, (cached, new))]
+    o = tables_device(serving, cached, new, free, table, int(new.sum()))
+    again = {n: torch.full_like(o[n], -7) for n in ("offsets", "total", "seq", "pos", "slot", "info")}
+    t = dev(table)
+    serving.build_page_tables(*lens, dev(free), t, *again.values())
+    assert all(torch.equal(again[n], o[n]) for n in again) and torch.equal(t, o["table"])
+    assert o["offsets"].tolist() == off.tolist() and np.array_equal(t.cpu().numpy(), want_table)
+
+
 @pytest.mark.parametrize("fault", ["pages", "rows", "negative", "negative_new", "long"])
 def test_page_tables_that_do_not_fit_take_nothing(serving, fault):
     cached, new, free, table = tables_case(5, 300, 30, 60, slack=0)
@@ -300,6 +313,16 @@ HEADS = [(32, 4, 64), (8, 8, 128), (16, 4, 32), (4, 4, 16), (8, 1, 128), (8, 1, 
     ([640, 1, 64, 33], [64, 1, 64, 1])])
 def test_chunk_attention(serving, H, kv, d, total, new):
     check_attend(serving, attend_case(len(total) + H + d, total, new, H, kv, d, extra_rows=2))
+
+
+@pytest.mark.parametrize("H,kv,d,total,new", [
+    (8, 1, 64, [200, 90], [1, 1]), (8, 1, 64, [4100, 90], [1, 1]), (8, 2, 128, [300, 1500], [70, 3]),
+    (16, 2, 64, [900], [300])])
+def test_chunk_attention_may_write_over_its_queries(serving, H, kv, d, total, new):
+    c = attend_case(H + d, total, new, H, kv, d)
+    q = dev(c["q"])
+    apart = attend_device(serving, c)
+    assert torch.equal(attend_device(serving, c, out=q, q=q), apart)
 
 
 @pytest.mark.parametrize("H,kv,d", [(16, 2, 64), (8, 4, 128), (4, 4, 16), (32, 4, 32)])

@@ -66,6 +66,15 @@ def test_c_entries_refuse_bad_arguments(call, kw):
     assert call(**kw) == INVALID
 
 
+def test_lengths_may_not_be_written_while_they_are_read():
+    at = lambda n: C.c_void_p(4096 + n)  # noqa: E731
+    apart = dict(cached=at(0), new=at(8), offsets=at(16), total=at(32))  # two sequences: 8, 8, 12 and 8 bytes
+    for clash in (dict(total=at(0)), dict(total=at(4)), dict(total=at(12)), dict(offsets=at(8)), dict(offsets=at(-8))):
+        assert tables(**{**apart, **clash}) == INVALID
+        assert "overlap" in _lib.last_error()
+    assert tables(**apart) != 0 and "overlap" not in _lib.last_error()  # no device here, or not device memory
+
+
 def test_unsupported_geometry_is_refused():
     assert attend(d=48, H=8, ld_q=384, ld_out=384) == 4
     assert attend(H=258, Hkv=2, ld_q=1 << 20, ld_out=1 << 20) == 4
