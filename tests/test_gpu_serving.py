@@ -448,6 +448,52 @@ def test_chunk_attention_bounds_only_shape_the_launch(serving, max_new, max_len)
     check_attend(serving, c, max_new=max_new, max_len=max_len)
 
 
+@pytest.mark.parametrize("H,kv,d", [(12, 4, 64), (16, 8, 64), (8, 8, 128)])
+@pytest.mark.parametrize("value", [np.nan, np.inf, 3e30])
+def test_chunk_attention_of_long_prompts_with_values_out_of_range(serving, H, kv, d, value):
+    # a token of the chunk, an evicted page's old memory and what lies behind the last token; three query heads to a
+    # KV head leave rows of a tile empty
+    total, new, t = [1503], [700], 1100
+    c = attend_case(11, total, new, H, kv, d, evict=[(0, 9)])
+    want = attend_numpy(c)
+    c["pool"][list(set(range(len(c["pool"]))) - set(c["table"][c["table"] >= 0].tolist()))] = value
+    c["pool"][c["table"][0, 1503 // PAGE], :, :, :, 1503 % PAGE:] = value
+    c["pool"][c["table"][0, t // PAGE], 1, :, :, t % PAGE] = value
+    out = attend_device(serving, c).cpu().numpy()
+    first = t - (1503 - 700)
+    assert rel_l2(out[:first], want[:first]) <= ATTN_TOL
+    if not np.isfinite(value):
+        assert not np.isfinite(out[first:]).any()
+    serving.check_device()
+
+
+@pytest.mark.parametrize("max_len", [1, 1000, 5000])
+def test_chunk_attention_of_long_prompts_beyond_their_bounds(serving, max_len):
+    c = attend_case(12, [1503], [700], 16, 8, 64)
+    check_attend(serving, c, max_len=max_len)
+    q, out = (torch.zeros(701, 1024 + k, device="cuda") for k in (3, 1))  # rows at any address
+    q[:700, 3:] = dev(c["q"])
+    attend_device(serving, c, out=out[:, 1:], q=q[:, 3:], max_len=max_len)
+    assert rel_l2(out[:700, 1:].cpu().numpy(), attend_numpy(c)) <= ATTN_TOL
+    assert (out[700:] == 0).all() and (out[:, 0] == 0).all()
+
+
+@pytest.mark.parametrize("value", [np.nan, np.inf])
+def test_chunk_attention_of_few_tokens_ignores_what_is_masked(serving, value):
+    c = attend_case(13, [37, 1, 250, 16], [1, 1, 1, 1], 16, 2, 64, evict=[(2, 2)])
+    want = attend_numpy(c)
+    c["pool"][list(set(range(len(c["pool"]))) - set(c["table"][c["table"] >= 0].tolist()))] = value
+    for s, L in enumerate((37, 1, 250)):
+        c["pool"][c["table"][s, L // PAGE], :, :, :, L % PAGE:] = value
+    assert rel_l2(attend_device(serving, c).cpu().numpy(), want) <= ATTN_TOL
+    c["pool"][c["table"][2, 5], 1, 1, 0, 3] = value  # visible to one KV head of one sequence
+    out = attend_device(serving, c).cpu().numpy().reshape(4, 16, 64)
+    hit = np.zeros((4, 16, 64), bool)
+    hit[2, :8] = True
+    assert not np.isfinite(out[hit]).any()
+    assert rel_l2(np.where(hit, 0, out), np.where(hit, 0, want.reshape(4, 16, 64))) <= ATTN_TOL
+
+
 def test_chunk_attention_strided_rows(serving):
     c = attend_case(10, [90, 33], [40, 1], 8, 2, 64)
     wide = torch.zeros(41, 3 * 512 + 1, device="cuda")
@@ -632,6 +678,32 @@ def test_sample_boundary_among_many_like_values(serving, kind, s, V):
     if kind == "far below":
         x[:, V // 3] = 5.0
     check_sample(serving, x, np.array([0.0, 0.4, 0.97], np.float32), **s)
+
+
+def test_sample_settings_that_are_no_numbers(serving):
+    x, _ = rows_like_a_model(5, 6, 700)
+    nan = np.float32(np.nan)
+    top = np.where(np.isnan(x), -np.inf, x).argmax(1).tolist()
+    f = lambda v: dev(np.full(6, v, np.float32))  # noqa: E731
+    assert serving.sample_rows(dev(x), f(0.9), temperature=f(nan))[0].tolist() == top  # not above 0: the maximum
+    assert serving.sample_rows(dev(x), f(0.9), temperature=f(-1.0))[0].tolist() == top
+    assert serving.sample_rows(dev(x), f(0.9), top_p=f(nan))[0].tolist() == top  # the shortest prefix
+    assert serving.sample_rows(dev(x), f(0.9), min_p=f(7.0))[0].tolist() == top
+    first = check_sample(serving, x, np.zeros(6, np.float32))
+    assert serving.sample_rows(dev(x), f(nan))[0].tolist() == first.tolist()
+    assert serving.sample_rows(dev(x), f(-3.0), min_p=f(nan))[0].tolist() == first.tolist()
+
+
+def test_sample_the_largest_vocabulary(serving):
+    V = 1 << 24
+    x = torch.zeros(2, V, device="cuda")
+    x[0, V - 1], x[1, 5] = 20.0, 30.0
+    z = torch.tensor([0.999, 0.5], device="cuda")
+    assert serving.sample_rows(x, z)[0].tolist() == [V - 1, 5]
+    k = torch.tensor([3, 1000], dtype=torch.int32, device="cuda")  # ties of zeros: the lowest indices
+    p = torch.tensor([1.0, 0.9999999], device="cuda")
+    t = torch.tensor([1e6, 1e6], device="cuda")
+    assert serving.sample_rows(x, z, top_k=k, top_p=p, temperature=t)[0].tolist() == [V - 1, 499]
 
 
 def test_sample_ends_of_the_unit_interval(serving):
