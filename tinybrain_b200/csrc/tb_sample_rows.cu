@@ -272,7 +272,9 @@ struct Row {
     // kBinSpan nats or more below it (and for 0 * infinity).  As a float, the bin's
     // number above 2^23, to which adding that rounds.
     __device__ __forceinline__ float float_bin(float v) const {
-        return fminf((top - v) * bin_scale, (float)(kRowBins - 1)) + 8388608.0f;
+        float b = fminf((top - v) * bin_scale, (float)(kRowBins - 1));
+        if (!STAGED) b = fmaxf(b, 0.0f);  // a row that changes while it is read must not leave the bins
+        return b + 8388608.0f;
     }
     __device__ __forceinline__ int bin_of(float v) const { return __float_as_int(float_bin(v)) - 0x4b000000; }
 
@@ -470,7 +472,7 @@ struct Row {
         });
         hi_key = (uint32_t)(ends >> 32);
         lo_key = ~(uint32_t)ends;
-        while (lo_key < hi_key) {
+        for (int round = 0; lo_key < hi_key && round < 3; ++round) {  // 2^32 keys, 2^21, 2^10
             int shift = 0;
             while (((hi_key - lo_key) >> shift) >= (uint32_t)kRowBins) ++shift;
             sync();  // the bins have been read
