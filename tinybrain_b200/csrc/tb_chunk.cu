@@ -81,9 +81,8 @@ struct Roles {
 };
 constexpr int kTileRows = 128;
 constexpr int kScaleRing = 8;     // tiles whose page scales are kept, at least two more than operand tiles
-// Barriers that free the operand tiles, more than there are tiles: a converter
-// warp may have no K (or V) page in a tile, and a phase two back on the same
-// barrier would then look like the one it waits for.
+// Barriers that free the operand tiles, more than there are tiles: a phase two back
+// on the same barrier looks like the one that a warp waits for.
 constexpr int kEmptyRing = 4;
 constexpr int kUnitRing = 4;      // units whose queries' scales are kept: with units of one tile, one
                                   // softmax warpgroup can be two units ahead of the other
@@ -125,9 +124,9 @@ struct Shape {
 };
 
 struct ChunkBars {
-    // By fill: a slot's fills come from two producers and go to converters that may be
-    // two tiles apart, so one barrier's parity would not tell a fill from the one two
-    // before it.  With two, that one is four fills and at least two V tiles back.
+    // By fill: a slot's fills come from two producers and go to converters that may be a
+    // tile apart, so one barrier's parity would not tell a fill from the one two before
+    // it.  With two, that one is four fills and at least two V tiles back.
     uint64_t slot_full[2][64], slot_empty[2][64];
     uint64_t k_full[3], v_full[3];
     uint64_t k_empty[kEmptyRing], v_empty[kEmptyRing];  // by tile, see kEmptyRing
@@ -153,6 +152,7 @@ struct ChunkShared {
     ChunkBars bars;
     alignas(16) float scale[kScaleRing][16];  // of a tile's pages: K factors, then V exponents
     int slot_page[64];
+    uint32_t page_top[2][8];  // of K and V pages that two warps convert
     ShareShared share;
     uint32_t tmem;
     float q_scale[kUnitRing][kTileRows];              // of the units' rows
@@ -185,33 +185,47 @@ __device__ __forceinline__ void split4(const float4& a, float s, uint2& hi, uint
     split_pair(y.x, y.y, hi.y, lo.y);
 }
 
+// The largest magnitude of a page that PARTS warps convert, each its dims: they
+// tell one another (tops[page][part]) and meet at the page's named barrier.
+template <int PARTS>
+struct PageTop {
+    volatile uint32_t* tops;
+    __device__ __forceinline__ uint32_t operator()(uint32_t bits, int page, int part) const {
+        if (PARTS == 1) return bits;
+        if ((threadIdx.x & 31) == 0) tops[page * PARTS + part] = bits;
+        named_bar_sync(2 + page, 32 * PARTS);
+        for (int k = 0; k < PARTS; ++k) bits = max(bits, tops[page * PARTS + k]);
+        return bits;
+    }
+};
+
 // K page -> rows `page * 16 ..` of the K operand, four dims of a token at a
 // time.  Lane (r, q) of a step takes dims 4 g .. of token r + 8 (q & 1) with g
 // staggered over the lanes, so that the reads (rows of D floats, 16 bytes a
 // lane) and the writes (8 bytes of a core matrix's 16-byte rows) fall into
 // different banks.
-template <int D>
-__device__ __forceinline__ void convert_k(const float* src, int valid, uint8_t* hi, uint8_t* lo, int page,
-                                          float* scale_out) {
-    constexpr int C = D / 4, kTasks = C / 2;  // 16-byte columns of a token, steps of a lane
+template <int D, int PARTS>
+__device__ __forceinline__ void convert_k(const float* src, int valid, uint8_t* hi, uint8_t* lo, int page, int part,
+                                          PageTop<PARTS> both, float* scale_out) {
+    constexpr int C = D / 4 / PARTS, kTasks = C / 2;  // 16-byte columns of a token, steps of a lane
     const int lane = threadIdx.x & 31, r = lane & 15;
     const int g0 = (lane & 7) + ((lane >> 3) & 1) + (lane >> 4) * kTasks;
     const float* row = src + r * D;
     float4 x[kTasks];
 #pragma unroll
     for (int t = 0; t < kTasks; ++t)
-        x[t] = r < valid ? lds128f(row + ((g0 + t) % C) * 4) : make_float4(0, 0, 0, 0);
+        x[t] = r < valid ? lds128f(row + (part * C + (g0 + t) % C) * 4) : make_float4(0, 0, 0, 0);
     float m = 0.0f;
 #pragma unroll
     for (int t = 0; t < kTasks; ++t) m = max_abs(max_abs(m, x[t].x, x[t].y), x[t].z, x[t].w);
-    const uint32_t bits = warp_max_bits(m);
+    const uint32_t bits = both(warp_max_bits(m), page, part);
     const int e = block_exponent(bits);
     const float s = exp2_int(-e);
-    if (lane == 0) *scale_out = bits >= kWildBits ? kWildMark : exp2_int(e);
+    if (lane == 0 && part == 0) *scale_out = bits >= kWildBits ? kWildMark : exp2_int(e);
     const int at0 = (page * 2 + (r >> 3)) * (D * 16) + (r & 7) * 16;
 #pragma unroll
     for (int t = 0; t < kTasks; ++t) {
-        const int g = (g0 + t) % C, at = at0 + (g >> 1) * 128 + (g & 1) * 8;
+        const int g = part * C + (g0 + t) % C, at = at0 + (g >> 1) * 128 + (g & 1) * 8;
         uint2 h, l;
         split4(x[t], s, h, l);
         *reinterpret_cast<uint2*>(hi + at) = h;
@@ -221,16 +235,16 @@ __device__ __forceinline__ void convert_k(const float* src, int valid, uint8_t* 
 
 // V page -> columns (k) `page * 16 ..` of the V^T operand of NT columns: a lane
 // takes 8 consecutive tokens of a dim.
-template <int D, int NT>
-__device__ __forceinline__ void convert_v(const float* src, int valid, uint8_t* hi, uint8_t* lo, int page,
-                                          float* exp_out) {
-    constexpr int kTasks = D / 16;
+template <int D, int NT, int PARTS>
+__device__ __forceinline__ void convert_v(const float* src, int valid, uint8_t* hi, uint8_t* lo, int page, int part,
+                                          PageTop<PARTS> both, float* exp_out) {
+    constexpr int kDims = D / PARTS, kTasks = kDims / 16;
     const int lane = threadIdx.x & 31;
     float x[kTasks][8];
     float m = 0.0f;
 #pragma unroll
     for (int t = 0; t < kTasks; ++t) {
-        const int task = lane + 32 * t, n = task % D, kc = task / D;
+        const int task = lane + 32 * t, n = part * kDims + task % kDims, kc = task / kDims;
 #pragma unroll
         for (int j = 0; j < 8; ++j) x[t][j] = kc * 8 + j < valid ? src[(kc * 8 + j) * D + n] : 0.0f;
     }
@@ -238,13 +252,13 @@ __device__ __forceinline__ void convert_v(const float* src, int valid, uint8_t* 
     for (int t = 0; t < kTasks; ++t)
 #pragma unroll
         for (int j = 0; j < 8; j += 2) m = max_abs(m, x[t][j], x[t][j + 1]);
-    const uint32_t bits = warp_max_bits(m);
+    const uint32_t bits = both(warp_max_bits(m), page, part);
     const int e = block_exponent(bits);
     const float s = exp2_int(-e);
-    if (lane == 0) *exp_out = bits >= kWildBits ? kWildMark : (float)e;
+    if (lane == 0 && part == 0) *exp_out = bits >= kWildBits ? kWildMark : (float)e;
 #pragma unroll
     for (int t = 0; t < kTasks; ++t) {
-        const int task = lane + 32 * t, n = task % D, kc = task / D;
+        const int task = lane + 32 * t, n = part * kDims + task % kDims, kc = task / kDims;
         uint2 h0, l0, h1, l1;
         split4(make_float4(x[t][0], x[t][1], x[t][2], x[t][3]), s, h0, l0);
         split4(make_float4(x[t][4], x[t][5], x[t][6], x[t][7]), s, h1, l1);
@@ -254,50 +268,56 @@ __device__ __forceinline__ void convert_v(const float* src, int valid, uint8_t* 
     }
 }
 
-template <int D>
-__device__ __forceinline__ void load_row4(const float* q, bool wide, int i, float (&x)[4]) {
+// N values of a query row, all loads in flight (a branch at each would make them wait
+// for one another: 11 us a unit of head dim 128 instead of 3).
+template <int N>
+__device__ __forceinline__ void load_row(const float* q, bool wide, float (&x)[N]) {
     if (wide) {
-        const float4 f = *reinterpret_cast<const float4*>(q + i);
-        x[0] = f.x, x[1] = f.y, x[2] = f.z, x[3] = f.w;
+#pragma unroll
+        for (int j = 0; j < N; j += 4) {
+            const float4 f = *reinterpret_cast<const float4*>(q + j);
+            x[j] = f.x, x[j + 1] = f.y, x[j + 2] = f.z, x[j + 3] = f.w;
+        }
     } else {
-        x[0] = q[i], x[1] = q[i + 1], x[2] = q[i + 2], x[3] = q[i + 3];
+#pragma unroll
+        for (int j = 0; j < N; ++j) x[j] = q[j];
     }
 }
 
 // The unit's query rows as halves in tensor memory; the thread's row factor
-// (2^e log2(e) / sqrt(D)) is the result, negative for a row without operands.
+// (2^e log2(e) / sqrt(D)) is the result, negative for a row without operands.  What
+// rows that are not the unit's (q is then a neighbour's) or have no operands hold
+// reaches no other row.
 template <int D>
-__device__ __forceinline__ float load_queries(const ChunkParams& p, const float* q, bool valid, bool wide,
-                                              uint32_t tq) {
+__device__ __forceinline__ float load_queries(const float* q, bool wide, uint32_t tq) {
+    constexpr int N = D < 64 ? D : D == 64 ? 64 : 32;  // at a time; one that holds the row reads it once
+    constexpr int W = D < 32 ? D : 32;
+    float x[N];
     float top = 0.0f;
-    if (valid) {
-#pragma unroll 8
-        for (int i = 0; i < D; i += 4) {
-            float x[4];
-            load_row4<D>(q, wide, i, x);
-            top = max_abs(max_abs(top, x[0], x[1]), x[2], x[3]);
-        }
+#pragma unroll 1
+    for (int i = 0; i < D; i += N) {
+        load_row(q + i, wide, x);
+#pragma unroll
+        for (int j = 0; j < N; j += 2) top = max_abs(top, x[j], x[j + 1]);
     }
     const uint32_t m = __float_as_uint(top) & 0x7fffffffu;
     const int e = m < kWildQueryBits ? block_exponent(m) : 0;
     const float s = exp2_int(-e);
-    constexpr int W = D < 32 ? D : 32;
 #pragma unroll 1
-    for (int i = 0; i < D; i += W) {
-        uint32_t hi[W / 2], lo[W / 2];
+    for (int i = 0; i < D; i += N) {
+        if (N < D) load_row(q + i, wide, x);
 #pragma unroll
-        for (int j = 0; j < W; j += 4) {
-            float x[4] = {0, 0, 0, 0};
-            if (valid && m < kWildQueryBits) load_row4<D>(q, wide, i + j, x);
-            split_pair(x[0] * s, x[1] * s, hi[j / 2], lo[j / 2]);
-            split_pair(x[2] * s, x[3] * s, hi[j / 2 + 1], lo[j / 2 + 1]);
-        }
-        if constexpr (W == 32) {
-            tmem_st16(tq + i / 2, hi);
-            tmem_st16(tq + D / 2 + i / 2, lo);
-        } else {
-            tmem_st8(tq + i / 2, hi);
-            tmem_st8(tq + D / 2 + i / 2, lo);
+        for (int c = 0; c < N; c += W) {
+            uint32_t hi[W / 2], lo[W / 2];
+#pragma unroll
+            for (int j = 0; j < W; j += 2) split_pair(x[c + j] * s, x[c + j + 1] * s, hi[j / 2], lo[j / 2]);
+            if constexpr (W == 32) {
+                tmem_st16(tq + (i + c) / 2, hi);
+                tmem_st16(tq + D / 2 + (i + c) / 2, lo);
+            } else {
+                tmem_st8(tq + (i + c) / 2, hi);
+                tmem_st8(tq + D / 2 + (i + c) / 2, lo);
+            }
         }
     }
     return m < kWildQueryBits ? exp2_int(e) * (1.4426950408889634f * rsqrtf((float)D)) : -1.0f;
@@ -338,14 +358,14 @@ __global__ void __launch_bounds__(Roles<PRE>::kThreads, 1)
         for (int i = 0; i < S::kSlots; ++i) {
             for (int f = 0; f < 2; ++f) {
                 mbar_init(b.slot_full[f] + i, 1);
-                mbar_init(b.slot_empty[f] + i, 1);
+                mbar_init(b.slot_empty[f] + i, 8 / PG);
             }
         }
         for (int i = 0; i < 3; ++i) {
             mbar_init(b.s_full + i, 1);
             mbar_init(b.p_full + i, 4);
-            mbar_init(b.k_full + i, PRE ? 1 : PG);
-            mbar_init(b.v_full + i, PRE ? 1 : PG);
+            mbar_init(b.k_full + i, PRE ? 1 : 8);
+            mbar_init(b.v_full + i, PRE ? 1 : 8);
         }
         for (int i = 0; i < kEmptyRing; ++i) {
             mbar_init(b.k_empty + i, 1);
@@ -501,18 +521,17 @@ __global__ void __launch_bounds__(Roles<PRE>::kThreads, 1)
         }
         __syncwarp();
     } else if (!PRE && count > 0 && warp >= kSoftmaxWarps && warp < kIssueWarp) {
-        // ---- converters: a warp takes the same pages of every tile (of every second one where a
-        //      tile has only four) ----
+        // ---- converters: a warp takes the same page of every tile, or of a tile of four
+        //      pages half the dims of one (one K operand tile: the next tile's conversion
+        //      waits for this one's, and a page by one warp takes 5600 cycles of D = 128) ----
         set_registers_down<kOtherRegs>();
-        constexpr int kStep = 8 / PG;
-        const int cw = warp - kSoftmaxWarps, page = cw % PG;
-        int i = 0, mine = cw / PG;  // the CTA's tile, and the warp's next one
+        constexpr int kParts = 8 / PG;
+        const int cw = warp - kSoftmaxWarps, page = cw % PG, part = cw / PG;
+        int i = 0;  // the CTA's tile
         int left = count;
         for (; left > 0; at = 0) {
             const int take = min(u.tiles - at, left);
             for (int j = at; j < at + take; ++j, ++i) {
-                if (i != mine) continue;
-                mine += kStep;
                 const int ring = i % kScaleRing, valid_here = u.limit - (j * NT + page * kPageTokens);
                 const int job = i * (2 * PG) + page;
                 for (int kv = 0; kv < 2; ++kv) {
@@ -528,12 +547,14 @@ __global__ void __launch_bounds__(Roles<PRE>::kThreads, 1)
                     const float* src = reinterpret_cast<const float*>(pages + slot * S::kPageBytes);
                     uint8_t* op = (kv ? v_ops : k_ops) + st * 2 * S::kHalf;
                     if (kv)
-                        convert_v<D, NT>(src, valid, op, op + S::kHalf, page, &sh.scale[ring][8 + page]);
+                        convert_v<D, NT, kParts>(src, valid, op, op + S::kHalf, page, part, {sh.page_top[1]},
+                                                 &sh.scale[ring][8 + page]);
                     else
-                        convert_k<D>(src, valid, op, op + S::kHalf, page, &sh.scale[ring][page]);
+                        convert_k<D, kParts>(src, valid, op, op + S::kHalf, page, part, {sh.page_top[0]},
+                                             &sh.scale[ring][page]);
                     fence_proxy_async_shared();
                     __syncwarp();
-                    if (lane < 3)
+                    if (lane < (part == 0 ? 3 : 2))
                         mbar_arrive(lane == 0   ? (kv ? b.v_full : b.k_full) + st
                                     : lane == 1 ? b.slot_empty[fill & 1] + slot
                                                 : b.scales + ring);
@@ -560,8 +581,8 @@ __global__ void __launch_bounds__(Roles<PRE>::kThreads, 1)
             const bool valid = row < per * G && token < w.n;
             if (__any_sync(0xffffffffu, valid)) {
                 sh.q_scale[unit % kUnitRing][quad * 32 + lane] = load_queries<D>(
-                    p, p.q + (w.first + (valid ? token : 0)) * p.ld_q + (size_t)(w.head * G + row % G) * D, valid,
-                    wide_q, tmem + kQ + lanes);
+                    p.q + (w.first + (valid ? token : 0)) * p.ld_q + (size_t)(w.head * G + row % G) * D, wide_q,
+                    tmem + kQ + lanes);
                 tmem_st_wait();
             }
             tc_fence_before();
@@ -969,10 +990,10 @@ __global__ void __launch_bounds__(kOperandWarps * 32) chunk_operands_kernel(Chun
     uint8_t* to = pre.ops + t * (4 * S::kHalf);
     constexpr int kPart = S::kPageBytes / 2;  // of the high halves, then of the low ones
     if (j < PG) {
-        convert_k<D>(src, valid, buf, buf + kPart, 0, pre.scales + t * 16 + page);
+        convert_k<D, 1>(src, valid, buf, buf + kPart, 0, 0, {}, pre.scales + t * 16 + page);
         to += page * kPart;
     } else {
-        convert_v<D, kPageTokens>(src, valid, buf, buf + kPart, 0, pre.scales + t * 16 + 8 + page);
+        convert_v<D, kPageTokens, 1>(src, valid, buf, buf + kPart, 0, 0, {}, pre.scales + t * 16 + 8 + page);
         to += 2 * S::kHalf + page * 256;
     }
     __syncwarp();
