@@ -338,9 +338,10 @@ def test_chunk_attention_of_few_tokens_over_few_pages(serving, H, kv, d, hint):
 
 @pytest.mark.parametrize("H,kv,d,total,new", [
     (4, 4, 64, [2100], [1100]), (4, 4, 128, [1500], [1069]), (16, 2, 64, [2049, 300, 1025], [203, 5, 180]),
-    (8, 4, 128, [700, 1300], [520, 581]), (4, 4, 32, [1700], [1041]), (8, 8, 16, [1100], [1100])])
+    (8, 4, 128, [700, 1300], [520, 581]), (4, 4, 32, [1700], [1041]), (8, 8, 16, [1100], [1100]),
+    (8, 2, 128, [1500], [701])])
 def test_chunk_attention_of_long_prompts(serving, H, kv, d, total, new):
-    # 8 row tiles and more to a sequence, the last one of some rows, of several calls
+    # many row tiles to a sequence, the last one of some rows, in several calls
     c = attend_case(d + H, total, new, H, kv, d, evict=[(0, 3)])
     for _ in range(3):
         check_attend(serving, c)
@@ -448,7 +449,7 @@ def test_chunk_attention_bounds_only_shape_the_launch(serving, max_new, max_len)
     check_attend(serving, c, max_new=max_new, max_len=max_len)
 
 
-@pytest.mark.parametrize("H,kv,d", [(12, 4, 64), (16, 8, 64), (8, 8, 128)])
+@pytest.mark.parametrize("H,kv,d", [(12, 4, 64), (16, 8, 64), (8, 8, 128), (8, 2, 128)])
 @pytest.mark.parametrize("value", [np.nan, np.inf, 3e30])
 def test_chunk_attention_of_long_prompts_with_values_out_of_range(serving, H, kv, d, value):
     # a token of the chunk, an evicted page's old memory and what lies behind the last token; three query heads to a

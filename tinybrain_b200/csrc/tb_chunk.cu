@@ -51,10 +51,11 @@ namespace {
 //
 // Bound by the softmax warps' instructions (a weight takes an exponential, two
 // conversions and some ten others).  Measured: 2048 tokens over 8192 positions, 32
-// query and 4 KV heads of 64, 322 us, 0.67 of the three products' time at the
+// query and 4 KV heads of 64, 314 us, 0.68 of the three products' time at the
 // measured 1679 TFLOP/s; 8 us for the operands.  Converted by the CTAs that read
-// them, 713 tokens of seven sequences of 664 to 1694, 32 heads of 128: 290 us; 64
-// tokens over 1920, 32 and 4 heads of 64: 29 us.
+// them, 713 tokens of seven sequences of 664 to 1694, 32 heads of 128: 166 us; 64
+// tokens over 1920, 32 and 4 heads of 64: 24 us, of which 4 pass before the share
+// is known and 5 in reading the queries.
 //
 // With c the row's scale times the page's, a score is c S and a weighted value
 // 2^(c S - M) v = 2^(c S + e - M) (v 2^-e): the page's value exponent e enters
@@ -1048,10 +1049,11 @@ ChunkPlan chunk_plan(long long rows, long long batch, long long max_new, long lo
     // Made beforehand where every K and V tile is read by so many row tiles or more
     // (as far as the bounds tell), a CTA has some tiles to pay for the launch, and the
     // operands fit kPreBytes.  Measured, us without / with:
-    //   D = 128: 2 row tiles 222 / 191 and 130 / 119, 4 370 / 282 and 199 / 140
-    //   D = 64:  2 row tiles 84 / 90 and 62 / 67, 4 80 / 77 and 217 / 187; of a CTA's
-    //            two tiles, 4 row tiles 36 / 38
-    const long long reuse = d == 128 ? 2 : 4;
+    //   D = 128: 4 row tiles 226 / 253 and 125 / 132, 8 204 / 188 and 539 / 603, 16 342 / 286
+    //   D = 64:  2 row tiles 78 / 87 and 56 / 62, 4 120 / 115 and 208 / 182, 8 190 / 165;
+    //            of a CTA's two tiles, 4 row tiles 30 / 33
+    //   D = 32:  4 row tiles 97 / 78
+    const long long reuse = d == 128 ? 12 : 4;
     constexpr long long kPreTiles = 4, kPreBytes = 1ll << 30;
     const long long tile_bytes = 8 * nt * d + 64;
     const bool fits = batch <= 65535 && len_tiles <= (1 << 24) && batch * Hkv * len_tiles <= kPreBytes / tile_bytes;
