@@ -274,11 +274,13 @@ tb_status tb_rope_append_paged_dev(void *stream, const float *q_dev, int64_t ld_
  * (its new tokens included, already in the cache) attends over positions
  * 0 .. total - n + i, scaled by 1 / sqrt(head_dim); rows of evicted pages are
  * zeros, as in tb_paged_attention_dev, and a row with no position gets zeros.
- * `rows` is what q_dev and out_dev hold (out_dev may be q_dev); max_new and max_len bound a sequence's
- * new tokens and length for the launch's shape only (larger ones stay right).
- * The workspace is tb_paged_attention_chunk_workspace bytes of device memory,
- * 16-byte aligned, for this call's use until it has run: calls that may overlap
- * need their own.  head_dim 16, 32, 64 or 128; num_heads / num_kv_heads <= 128. */
+ * `rows` is what q_dev and out_dev hold (out_dev may be q_dev); max_new and
+ * max_len bound a sequence's new tokens and length for the launch's shape only
+ * (larger ones stay right).
+ * The workspace is tb_paged_attention_chunk_workspace bytes of device memory for
+ * the same bounds (where that is 0, NULL will do), 16-byte aligned, for this
+ * call's use until it has run: calls that may overlap need their own.  head_dim
+ * 16, 32, 64 or 128; num_heads / num_kv_heads <= 128. */
 tb_status tb_paged_attention_chunk_workspace(int32_t rows, int32_t batch, int32_t max_new, int32_t max_len,
                                              int32_t num_heads, int32_t num_kv_heads, int32_t head_dim,
                                              int64_t *bytes);

@@ -80,6 +80,21 @@ def test_unsupported_geometry_is_refused():
     assert attend(H=258, Hkv=2, ld_q=1 << 20, ld_out=1 << 20) == 4
 
 
+def test_the_workspace_is_asked_for_where_it_is_used():
+    few, many = dict(rows=1, batch=1, max_new=1, max_len=64), dict(rows=1, batch=1, max_new=1, max_len=1 << 20)
+
+    def need(rows, batch, max_new, max_len):
+        n = C.c_int64(-1)
+        _lib.call("tb_paged_attention_chunk_workspace", rows, batch, max_new, max_len, 8, 2, 32, C.byref(n))
+        return n.value
+
+    assert need(**few) == 0 and need(**many) > 0
+    assert attend(**few, ws=None, ws_bytes=0) != 0 and "workspace" not in _lib.last_error()  # no device here
+    assert attend(**many, ws=None, ws_bytes=0) == INVALID and "workspace" in _lib.last_error()
+    assert attend(**many, ws_bytes=need(**many) - 1) == INVALID and "workspace" in _lib.last_error()
+    assert attend(**many, ws=C.c_void_p(72)) == INVALID and "workspace" in _lib.last_error()
+
+
 def test_no_rows_is_no_work():
     assert append(rows=0) == 0 and attend(rows=0) == 0 and sample(rows=0) == 0
 
