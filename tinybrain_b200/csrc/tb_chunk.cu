@@ -51,11 +51,11 @@ namespace {
 //
 // Bound by the softmax warps' instructions (a weight takes an exponential, two
 // conversions and some ten others).  Measured: 2048 tokens over 8192 positions, 32
-// query and 4 KV heads of 64, 314 us, 0.68 of the three products' time at the
+// query and 4 KV heads of 64, 305 us, 0.70 of the three products' time at the
 // measured 1679 TFLOP/s; 8 us for the operands.  Converted by the CTAs that read
-// them, 713 tokens of seven sequences of 664 to 1694, 32 heads of 128: 166 us; 64
-// tokens over 1920, 32 and 4 heads of 64: 24 us, of which 4 pass before the share
-// is known and 5 in reading the queries.
+// them, 713 tokens of seven sequences of 664 to 1694, 32 heads of 128: 165 us; 64
+// tokens over 1920, 32 and 4 heads of 64: 23 us, of which 4 pass before the share
+// is known and 2 in reading the queries.
 //
 // With c the row's scale times the page's, a score is c S and a weighted value
 // 2^(c S - M) v = 2^(c S + e - M) (v 2^-e): the page's value exponent e enters
@@ -269,59 +269,76 @@ __device__ __forceinline__ void convert_v(const float* src, int valid, uint8_t* 
     }
 }
 
-// N values of a query row, all loads in flight (a branch at each would make them wait
-// for one another: 11 us a unit of head dim 128 instead of 3).
+// A thread's 4 of every 16 values of a query row (N of them in all), all loads in
+// flight: a branch at each would make them wait for one another.
 template <int N>
 __device__ __forceinline__ void load_row(const float* q, bool wide, float (&x)[N]) {
     if (wide) {
 #pragma unroll
         for (int j = 0; j < N; j += 4) {
-            const float4 f = *reinterpret_cast<const float4*>(q + j);
+            const float4 f = *reinterpret_cast<const float4*>(q + 4 * j);
             x[j] = f.x, x[j + 1] = f.y, x[j + 2] = f.z, x[j + 3] = f.w;
         }
     } else {
 #pragma unroll
-        for (int j = 0; j < N; ++j) x[j] = q[j];
+        for (int j = 0; j < N; ++j) x[j] = q[j / 4 * 16 + j % 4];
     }
 }
 
-// The unit's query rows as halves in tensor memory; the thread's row factor
-// (2^e log2(e) / sqrt(D)) is the result, negative for a row without operands.  What
-// rows that are not the unit's (q is then a neighbour's) or have no operands hold
-// reaches no other row.
-template <int D>
-__device__ __forceinline__ float load_queries(const float* q, bool wide, uint32_t tq) {
-    constexpr int N = D < 64 ? D : D == 64 ? 64 : 32;  // at a time; one that holds the row reads it once
-    constexpr int W = D < 32 ? D : 32;
-    float x[N];
-    float top = 0.0f;
+// A warp's 32 query rows (row(r): where row r is) as halves in tensor memory, 16 at a
+// time, four threads to a row, so that a load touches 8 rows and not 32 (a thread a
+// row: 311 us for the prompt above instead of 305).  scale[r] becomes the row's factor
+// (2^e log2(e) / sqrt(D)), negative for a row without operands.  What rows that are
+// not the unit's (row() is then a neighbour's) or have no operands hold reaches no
+// other row.
+template <int D, class Row>
+__device__ __forceinline__ void load_queries(Row row, bool wide, uint32_t tq, float* scale) {
+    constexpr int N = D < 64 ? D : 64, M = N / 4;  // dims at a time; all of them are read once
+    const int lane = threadIdx.x & 31, own = lane / 4, dims = 4 * (lane % 4);
 #pragma unroll 1
-    for (int i = 0; i < D; i += N) {
-        load_row(q + i, wide, x);
-#pragma unroll
-        for (int j = 0; j < N; j += 2) top = max_abs(top, x[j], x[j + 1]);
-    }
-    const uint32_t m = __float_as_uint(top) & 0x7fffffffu;
-    const int e = m < kWildQueryBits ? block_exponent(m) : 0;
-    const float s = exp2_int(-e);
+    for (int half = 0; half < 2; ++half) {
+        const float* q[2] = {row(16 * half + own) + dims, row(16 * half + own + 8) + dims};
+        float x[2][M], s[2];
+        float top[2] = {0.0f, 0.0f};
 #pragma unroll 1
-    for (int i = 0; i < D; i += N) {
-        if (N < D) load_row(q + i, wide, x);
+        for (int i = 0; i < D; i += N) {
+            load_row(q[0] + i, wide, x[0]);
+            load_row(q[1] + i, wide, x[1]);
 #pragma unroll
-        for (int c = 0; c < N; c += W) {
-            uint32_t hi[W / 2], lo[W / 2];
+            for (int a = 0; a < 2; ++a)
 #pragma unroll
-            for (int j = 0; j < W; j += 2) split_pair(x[c + j] * s, x[c + j + 1] * s, hi[j / 2], lo[j / 2]);
-            if constexpr (W == 32) {
-                tmem_st16(tq + (i + c) / 2, hi);
-                tmem_st16(tq + D / 2 + (i + c) / 2, lo);
-            } else {
-                tmem_st8(tq + (i + c) / 2, hi);
-                tmem_st8(tq + D / 2 + (i + c) / 2, lo);
+                for (int j = 0; j < M; j += 2) top[a] = max_abs(top[a], x[a][j], x[a][j + 1]);
+        }
+#pragma unroll
+        for (int a = 0; a < 2; ++a) {
+            for (int o = 1; o < 4; o <<= 1)
+                top[a] = max_abs(top[a], __shfl_xor_sync(0xffffffffu, top[a], o), 0.0f);
+            const uint32_t m = __float_as_uint(top[a]) & 0x7fffffffu;
+            const int e = m < kWildQueryBits ? block_exponent(m) : 0;
+            s[a] = exp2_int(-e);
+            if (dims == 0)
+                scale[16 * half + own + 8 * a] =
+                    m < kWildQueryBits ? exp2_int(e) * (1.4426950408889634f * rsqrtf((float)D)) : -1.0f;
+        }
+        const uint32_t to = tq + ((uint32_t)(16 * half) << 16);
+#pragma unroll 1
+        for (int i = 0; i < D; i += N) {
+            if (N < D) {
+                load_row(q[0] + i, wide, x[0]);
+                load_row(q[1] + i, wide, x[1]);
             }
+            uint32_t hi[M], lo[M];
+#pragma unroll
+            for (int j = 0; j < M; j += 4)
+#pragma unroll
+                for (int a = 0; a < 2; ++a) {
+                    split_pair(x[a][j] * s[a], x[a][j + 1] * s[a], hi[j + 2 * a], lo[j + 2 * a]);
+                    split_pair(x[a][j + 2] * s[a], x[a][j + 3] * s[a], hi[j + 2 * a + 1], lo[j + 2 * a + 1]);
+                }
+            tmem_st_rows<N / 16>(to + i / 2, hi);
+            tmem_st_rows<N / 16>(to + D / 2 + i / 2, lo);
         }
     }
-    return m < kWildQueryBits ? exp2_int(e) * (1.4426950408889634f * rsqrtf((float)D)) : -1.0f;
 }
 
 // A unit's rows of one warp in fp32 (pages or queries without fp16 operands).
@@ -577,13 +594,14 @@ __global__ void __launch_bounds__(Roles<PRE>::kThreads, 1)
         // quarter of a tile's positions (P is zero elsewhere).
         const auto small_unit = [&](const Unit& w) { return min(per, w.n - w.tile * per) * G <= 32; };
         const auto queries = [&](const Unit& w, int unit) {
-            const int row = small_unit(w) ? lane : quad * 32 + lane;
-            const int token = w.tile * per + row / G;
-            const bool valid = row < per * G && token < w.n;
-            if (__any_sync(0xffffffffu, valid)) {
-                sh.q_scale[unit % kUnitRing][quad * 32 + lane] = load_queries<D>(
-                    p.q + (w.first + (valid ? token : 0)) * p.ld_q + (size_t)(w.head * G + row % G) * D, wide_q,
-                    tmem + kQ + lanes);
+            const int row0 = small_unit(w) ? 0 : quad * 32, used = min(per, w.n - w.tile * per) * G;
+            if (row0 < used) {
+                load_queries<D>(
+                    [&](int r) {  // (rows that are not the unit's: its first)
+                        const int row = row0 + r < used ? row0 + r : 0;
+                        return p.q + (w.first + w.tile * per + row / G) * p.ld_q + (size_t)(w.head * G + row % G) * D;
+                    },
+                    wide_q, tmem + kQ + lanes, sh.q_scale[unit % kUnitRing] + quad * 32);
                 tmem_st_wait();
             }
             tc_fence_before();
