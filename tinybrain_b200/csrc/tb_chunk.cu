@@ -31,8 +31,8 @@ namespace {
 // Roles:
 //   producers  (2 warps: K, V) a lane per page of a tile: page table, then a bulk
 //              copy of the page's rows of this head into a ring of fp32 pages;
-//   converters (8 warps) the K and the V page of 16 tokens at a time: a page's
-//              largest magnitude gives a power-of-two scale, the halves go to the
+//   converters (8 warps) the K and the V page of 16 tokens at a time (of D = 128 two
+//              warps a page, half the dims each): a page's largest magnitude gives a power-of-two scale, the halves go to the
 //              operand tiles;
 //   issuer     one thread: S(i + 1) (or i + 2) before P V(i), so the softmax of a tile
 //              runs while the tensor cores do the next S and the last P V;
@@ -356,7 +356,7 @@ __global__ void __launch_bounds__(Roles<PRE>::kThreads, 1)
     using R = Roles<PRE>;
     constexpr int NT = S::NT, PG = S::PG, kChunkThreads = R::kThreads;
     constexpr int kKStages = S::template kKStages<PRE>, kVStages = S::template kVStages<PRE>;
-    constexpr int kIssueWarp = R::kIssueWarp, kLoadWarp = R::kLoadWarp, kConvertWarps = R::kConvertWarps;
+    constexpr int kIssueWarp = R::kIssueWarp, kLoadWarp = R::kLoadWarp;
     constexpr int kSoftmaxRegs = R::kSoftmaxRegs, kOtherRegs = R::kOtherRegs, kSoftmaxWarps = R::kSoftmaxWarps;
     constexpr int kGroups = R::kGroups;
     constexpr int kSBufs = S::template kSBufs<PRE>, kOBufs = S::template kOBufs<PRE>;
