@@ -32,8 +32,8 @@ namespace {
 //   producers  (2 warps: K, V) a lane per page of a tile: page table, then a bulk
 //              copy of the page's rows of this head into a ring of fp32 pages;
 //   converters (8 warps) the K and the V page of 16 tokens at a time (of D = 128 two
-//              warps a page, half the dims each): a page's largest magnitude gives a power-of-two scale, the halves go to the
-//              operand tiles;
+//              warps a page, half the dims each): a page's largest magnitude gives
+//              a power-of-two scale, the halves go to the operand tiles;
 //   issuer     one thread: S(i + 1) (or i + 2) before P V(i), so the softmax of a tile
 //              runs while the tensor cores do the next S and the last P V;
 //   softmax    a warpgroup, a row a thread: base-2 softmax over the tile, P as
