@@ -1,0 +1,81 @@
+"""Chunk attention where its tiles, scales and masks can go wrong.
+
+The reference is the definition in 64 bits (include/tinybrain_cuda.h).  Tolerance:
+a score is off by 5.2e-6 at most for q, k ~ N(0, 1) (test_gpu_serving.py's bound),
+a weight by as much relative to itself, and the sums add a few 2^-22: 1e-5 in
+relative L2, over the call and, four times that, over every row and head by itself.
+Nothing in that depends on the size of the values, so rows are held to their own norm.
+"""
+import numpy as np
+import pytest
+
+from tests.helpers import rel_l2
+from tests.test_gpu_serving import ATTN_TOL, PAGE, attend_case, attend_device, dev, serving  # noqa: F401
+
+torch = pytest.importorskip("torch")
+pytestmark = pytest.mark.gpu
+
+
+def attend_exact(c):
+    """The definition in 64 bits, a sequence and head at a time; rows without a position are zeros."""
+    H, kv, d = c["H"], c["kv"], c["d"]
+    q, pool = dev(c["q"]).double(), dev(c["pool"])[:, c["layer"]].double()
+    out = torch.zeros(int(c["offsets"][-1]), H, d, dtype=torch.float64, device="cuda")
+    for s, (L, n) in enumerate(zip(c["total"].tolist(), c["new"].tolist())):
+        if not n or L <= 0:
+            continue
+        ids = dev(c["table"][s, :-(-L // PAGE)].astype(np.int64))
+        pages = torch.where((ids >= 0)[:, None, None, None, None], pool[ids.clamp(min=0)], 0.0)  # [pages, 2, kv, 16, d]
+        K, V = (pages[:, x].transpose(0, 1).reshape(kv, -1, d)[:, :L] for x in (0, 1))
+        a, z = int(c["offsets"][s]), max(n - L, 0)  # the first z rows have no position
+        limit = torch.arange(L - n + z, L, device="cuda")
+        later = torch.arange(L, device="cuda")[None] > limit[:, None]
+        for h in range(H):
+            sc = (q[a + z:a + n, h * d:(h + 1) * d] @ K[h * kv // H].T) / d ** 0.5
+            out[a + z:a + n, h] = torch.softmax(sc.masked_fill(later, -np.inf), 1) @ V[h * kv // H]
+    return out.reshape(-1, H * d).cpu().numpy()
+
+
+def check(serving, c, tol=ATTN_TOL, **kw):  # noqa: F811
+    out = attend_device(serving, c, **kw).cpu().numpy()
+    n, want = int(c["offsets"][-1]), attend_exact(c)
+    assert np.isfinite(out[:n]).all()
+    assert rel_l2(out[:n], want) <= tol
+    a, b = (x.reshape(-1, c["d"]).astype(np.float64) for x in (out[:n], want))
+    big = np.linalg.norm(b, axis=1)
+    off = np.linalg.norm(a - b, axis=1)
+    assert np.all(off <= 4 * tol * np.maximum(big, 0.02 * big.max())), (off / np.maximum(big, 0.02 * big.max())).max()
+    assert (out[n:] == -7).all()
+    serving.check_device()
+    return out
+
+
+def cut(G, k, kv=1):
+    """k row tiles of whole tokens and one token more."""
+    return k * (128 // G) + 1
+
+
+# Before these were right, the smallest of them walked out of the lengths and the table.
+@pytest.mark.parametrize("H,kv,d,total,new", [
+    (7, 1, 64, [73], [73]), (28, 4, 128, [512], [512]), (28, 4, 128, [343], [343]), (40, 8, 64, [201], [201]),
+    (24, 8, 64, [2048], [2048]), (12, 2, 32, [1100], [cut(6, 30)]), (24, 2, 16, [900], [cut(12, 40)]),
+    (14, 2, 64, [900], [577]), (20, 1, 64, [400], [cut(20, 22)]), (100, 1, 32, [200], [200]), (11, 1, 128, [300], [cut(11, 20)]),
+    (28, 4, 128, [8192], [2048])])
+def test_head_groups_that_do_not_divide_a_tile(serving, H, kv, d, total, new):  # noqa: F811
+    check(serving, attend_case(H + d, total, new, H, kv, d, extra_rows=2))
+
+
+@pytest.mark.parametrize("G,kv,d", [(3, 4, 64), (5, 2, 64), (6, 2, 32), (7, 4, 64), (12, 1, 128), (20, 2, 16), (48, 1, 64)])
+def test_head_groups_that_do_not_divide_a_tile_ragged(serving, G, kv, d):  # noqa: F811
+    g = np.random.default_rng(G)
+    new = [cut(G, int(k)) for k in g.integers(1, 9, 16)]
+    new[3], new[7] = 0, 1
+    total = [n + int(h) for n, h in zip(new, g.integers(0, 400, 16))]
+    check(serving, attend_case(G, total, new, G * kv, kv, d, evict=[(0, 0)], extra_rows=1))
+
+
+@pytest.mark.parametrize("G,kv,d", [(3, 4, 64), (5, 2, 32), (6, 2, 128), (7, 4, 64)])
+@pytest.mark.parametrize("max_new,max_len", [(1, 1), (1, 4096), (2, 500)])
+def test_head_groups_with_more_tokens_than_the_bounds_tell(serving, G, kv, d, max_new, max_len):  # noqa: F811
+    for total, new in (([40], [9]), ([300, 5, 77], [63, 5, 3]), ([30] * 16, list(range(16)))):
+        check(serving, attend_case(G + len(new), total, new, G * kv, kv, d), max_new=max_new, max_len=max_len)

@@ -166,11 +166,11 @@ __global__ void __launch_bounds__(Few<D>::kThreads, 1)
             const bool has = sh.before[t] <= begin && begin < sh.before[t] + sh.mine[t];
             if (has) holder = t + 1;
         }
-        holder = __reduce_max_sync(0xffffffffu, holder) - 1;
+        holder = max(__reduce_max_sync(0xffffffffu, holder) - 1, 0);
         long long at = begin - sh.before[holder];
         Unit& u = now.u;
-        for (u.s = holder * run;; ++u.s) {
-            const long long here = run == 1 ? LLONG_MAX : work_of(u.s);
+        for (u.s = min(holder * run, p.batch - 1);; ++u.s) {
+            const long long here = run == 1 || u.s + 1 >= p.batch ? LLONG_MAX : work_of(u.s);
             if (at < here) break;
             at -= here;
         }
