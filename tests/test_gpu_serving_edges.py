@@ -79,3 +79,16 @@ def test_head_groups_that_do_not_divide_a_tile_ragged(serving, G, kv, d):  # noq
 def test_head_groups_with_more_tokens_than_the_bounds_tell(serving, G, kv, d, max_new, max_len):  # noqa: F811
     for total, new in (([40], [9]), ([300, 5, 77], [63, 5, 3]), ([30] * 16, list(range(16)))):
         check(serving, attend_case(G + len(new), total, new, G * kv, kv, d), max_new=max_new, max_len=max_len)
+
+
+@pytest.mark.parametrize("H,kv,d,total,new", [
+    (8, 2, 64, [300, 40], [150, 40]), (16, 2, 128, [200], [33]), (4, 4, 32, [500], [500]), (8, 8, 64, [1500], [1100]),
+    (32, 4, 64, [300, 17], [1, 1])])
+@pytest.mark.parametrize("q,k", [(1e-20, 1e-20), (1e-30, 1e-30), (1e-12, 1e-25), (0.0, 1e-30), (0.0, 0.0), (1e10, 1e-10),
+                                 (1e-16, 1e16), (1e15, 1e-15)])
+def test_queries_and_keys_of_any_size(serving, H, kv, d, total, new, q, k):  # noqa: F811
+    # the scores keep their bound (their size is that of q times k); of next to none the result is the mean
+    c = attend_case(d, total, new, H, kv, d)
+    c["q"] *= np.float32(q)
+    c["pool"][:, :, 0] *= np.float32(k)
+    check(serving, c)

@@ -220,7 +220,7 @@ __device__ __forceinline__ void convert_k(const float* src, int valid, uint8_t* 
 #pragma unroll
     for (int t = 0; t < kTasks; ++t) m = max_abs(max_abs(m, x[t].x, x[t].y), x[t].z, x[t].w);
     const uint32_t bits = both(warp_max_bits(m), page, part);
-    const int e = block_exponent(bits);
+    const int e = block_exponent(bits, kLowestFactor);
     const float s = exp2_int(-e);
     if (lane == 0 && part == 0) *scale_out = bits >= kWildBits ? kWildMark : exp2_int(e);
     const int at0 = (page * 2 + (r >> 3)) * (D * 16) + (r & 7) * 16;
@@ -254,7 +254,7 @@ __device__ __forceinline__ void convert_v(const float* src, int valid, uint8_t* 
 #pragma unroll
         for (int j = 0; j < 8; j += 2) m = max_abs(m, x[t][j], x[t][j + 1]);
     const uint32_t bits = both(warp_max_bits(m), page, part);
-    const int e = block_exponent(bits);
+    const int e = block_exponent(bits, kLowestValue);
     const float s = exp2_int(-e);
     if (lane == 0 && part == 0) *exp_out = bits >= kWildBits ? kWildMark : (float)e;
 #pragma unroll
@@ -314,7 +314,7 @@ __device__ __forceinline__ void load_queries(Row row, bool wide, uint32_t tq, fl
             for (int o = 1; o < 4; o <<= 1)
                 top[a] = max_abs(top[a], __shfl_xor_sync(0xffffffffu, top[a], o), 0.0f);
             const uint32_t m = __float_as_uint(top[a]) & 0x7fffffffu;
-            const int e = m < kWildQueryBits ? block_exponent(m) : 0;
+            const int e = m < kWildQueryBits ? block_exponent(m, kLowestFactor) : 0;
             s[a] = exp2_int(-e);
             if (dims == 0)
                 scale[16 * half + own + 8 * a] =
