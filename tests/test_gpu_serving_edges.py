@@ -92,3 +92,39 @@ def test_queries_and_keys_of_any_size(serving, H, kv, d, total, new, q, k):  # n
     c["q"] *= np.float32(q)
     c["pool"][:, :, 0] *= np.float32(k)
     check(serving, c)
+
+
+TILE = {16: 8, 32: 8, 64: 8, 128: 4}  # pages of a tile
+
+
+@pytest.mark.parametrize("H,kv,d,total,new", [
+    (8, 2, 64, [1000], [30]), (8, 4, 128, [1000], [100]), (16, 1, 16, [1000], [64]), (8, 8, 64, [1500], [1100]),
+    (2, 2, 128, [2100], [2000]), (32, 4, 64, [1000], [1])])
+@pytest.mark.parametrize("size", [1.0, 1e-2, 1e-5, 1e-12, 1e-30, 1e5])
+@pytest.mark.parametrize("where", ["first", "later", "tile", "most"])
+@pytest.mark.parametrize("how", ["evicted", "zeros", "zero values"])
+def test_pages_of_zeros_beside_values_of_any_size(serving, H, kv, d, total, new, size, where, how):  # noqa: F811
+    c = attend_case(d + H, total, new, H, kv, d)
+    c["pool"][:, :, 1] *= np.float32(size)
+    n = total[0] // PAGE
+    at = {"first": [0], "later": [TILE[d] + 3, n - 2], "tile": list(range(2 * TILE[d], 3 * TILE[d])),
+          "most": list(range(n - 1))}[where]
+    if how == "evicted":
+        c["table"][0, at] = -1
+    else:
+        c["pool"][c["table"][0, at], :, (0 if how == "zeros" else 1):] = 0
+    check(serving, c)
+
+
+@pytest.mark.parametrize("max_len", [1, None])
+def test_a_long_context_of_zero_values(serving, max_len):  # noqa: F811
+    # scores that rise to just below what moves the reference maximum, over pages without
+    # values: the row sums grow as far as they can.  Operands made beforehand, or not.
+    d, L, n = 16, 40000, 4736
+    c = attend_case(3, [L], [n], 4, 4, d)
+    c["q"][:] = 1.0
+    c["pool"][:, :, 0] = np.float32(5.45 / 4)  # d = 16: 5.45 nats, 2^7.86
+    c["pool"][c["table"][0, :8], :, 0] = 0
+    c["pool"][c["table"][0, :-60], :, 1] = 0
+    c["pool"][:, :, 1] *= np.float32(1e-3)
+    check(serving, c, max_len=max_len)

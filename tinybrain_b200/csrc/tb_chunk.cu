@@ -91,6 +91,9 @@ constexpr uint32_t kWildBits = (127u + 20u) << 23;    // a K or V value of 2^20
 constexpr uint32_t kWildQueryBits = (127u + 40u) << 23;
 constexpr float kPShift = 6.0f;   // P = 2^(6 + score - M), M within 2^8 of the maximum: at most 2^14
 constexpr float kLazy = 8.0f;
+// The row sums count in 2^kSumShift: over pages of zeros a term is up to 2^(14 + 100),
+// and 2^31 of them have to fit; the smallest sum is 2^(6 - 6 - kSumShift).
+constexpr float kSumShift = 32.0f, kSumScale = 1.0f / 4294967296.0f;
 constexpr float kWildMark = 3e38f;
 constexpr float kHuge = 1048576.0f;  // a score whose rounding could carry P out of fp16's range
 
@@ -346,7 +349,7 @@ template <int D>
 __device__ __noinline__ void rows_without_operands(const ChunkParams& p, const Unit& u, int t0, int t1, float* partial) {
     const int first = (threadIdx.x >> 5) * 32;
     for (int r = first; r < first + 32; ++r)  // the even warpgroup's warps 0 to 3
-        if (!row_in_fp32<D, kTileRows>(p, u, r, t0, t1, partial, kPShift)) break;
+        if (!row_in_fp32<D, kTileRows>(p, u, r, t0, t1, partial, kPShift, kSumScale)) break;
 }
 
 template <int D, bool PRE>
@@ -708,7 +711,7 @@ __global__ void __launch_bounds__(Roles<PRE>::kThreads, 1)
                             sum = __fadd2_rn(sum, w);
                             split_pair(w.x, w.y, hi[x / 2], lo[x / 2]);
                         }
-                        l = fmaf(sum.x + sum.y, ex2(-e), l);
+                        l = fmaf(sum.x + sum.y, ex2(-e - kSumShift), l);
                     };
                     float r = 1.0f;
                     // takes the block's maximum into the reference; the result is P's shift
@@ -888,7 +891,7 @@ __global__ void __launch_bounds__(Roles<PRE>::kThreads, 1)
                 for (int k = 0; k < 4; ++k) l = fmaf(ex2(sh.quad_m[k * 32 + lane] - off), sh.quad_l[k * 32 + lane], l);
             }
             if (!part) {
-                const float inv = sees > 0 ? 1.0f / l : 0.0f;
+                const float inv = sees > 0 ? kSumScale / l : 0.0f;
                 w0 = sees > 0 ? w0 * inv : 0.0f;
                 w1 = sees > 0 ? w1 * inv : 0.0f;
             }
@@ -1120,7 +1123,8 @@ cudaError_t launch_chunk(ChunkParams p, const ChunkPlan& plan, void* workspace, 
         chunk_few_kernel<D, false><<<plan.few_ctas, Few<D>::kThreads, Few<D>::kSmem, stream>>>(p, partials, splits);
         e = cudaGetLastError();
         if (e == cudaSuccess)
-            e = launch_combine<D, kFewRows>(p, plan.few_ctas * Few<D>::kWarps, partials, splits, wide_output(p), stream);
+            e = launch_combine<D, kFewRows>(p, plan.few_ctas * Few<D>::kWarps, partials, splits, wide_output(p), 1.0f,
+                                            stream);
         p.rows_above = kFewRows;
         p.rows_upto = INT_MAX;
     }
@@ -1141,7 +1145,7 @@ cudaError_t launch_chunk(ChunkParams p, const ChunkPlan& plan, void* workspace, 
         e = launch_tiles<D, false>(p, plan, partials, splits, pre, stream);
     }
     if (e != cudaSuccess) return e;
-    return launch_combine<D, kTileRows>(p, plan.ctas, partials, splits, wide_output(p), stream);
+    return launch_combine<D, kTileRows>(p, plan.ctas, partials, splits, wide_output(p), kSumScale, stream);
 }
 
 }  // namespace

@@ -428,7 +428,7 @@ __global__ void __launch_bounds__(Few<D>::kThreads, 1)
         if (WHOLE && from == now.end) {  // no page
         } else if (wild) {
             for (int r = 0; r < rows; ++r)
-                row_in_fp32<D, kFewRows>(p, u, r, from * kPageTokens, now.end * kPageTokens, part, 0.0f);
+                row_in_fp32<D, kFewRows>(p, u, r, from * kPageTokens, now.end * kPageTokens, part, 0.0f, 1.0f);
         } else {
 #pragma unroll
             for (int r = 0; r < kFewRows; ++r) {

@@ -107,15 +107,19 @@ __device__ __forceinline__ void split_pair(float a, float b, uint32_t& hi, uint3
 }
 
 // The exponent e with max 2^-e in [2^14, 2^15), from the bits of a block's
-// largest magnitude, but no lower than `lowest`; 0 for a block of zeros.  Below
+// largest magnitude, but no lower than `lowest` (which zeros get).  Below
 // 2^15 2^lowest a block keeps the absolute step of that size.
 __device__ __forceinline__ int block_exponent(uint32_t max_bits, int lowest) {
-    return max_bits ? max((int)(max_bits >> 23) - 127 - 14, lowest) : 0;
+    return max((int)(max_bits >> 23) - 127 - 14, lowest);
 }
 // Of queries and keys: the product of the two scales, times log2(e) / sqrt(D), is
 // then a normal number, so that it times a masked score of -inf stays -inf (0 * inf
 // made NaN of the rows).  What is lost of a score is below 2^-85 of the other factor.
 constexpr int kLowestFactor = -60;
+// Of values.  A page of zeros (an evicted one) must not stand above a page that has
+// values: the weights' reference is the largest score + value exponent, and a page
+// of zeros taken as 2^15 pushed all others' weights down into fp16's subnormals
+// (values of 1e-3: error 8e-4 instead of 8e-8).
 constexpr int kLowestValue = -100;
 __device__ __forceinline__ float exp2_int(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }  // |e| <= 126
 // Largest magnitude of three, NaN if one is (one instruction).

@@ -232,10 +232,11 @@ __device__ __forceinline__ Share find_share(const ChunkParams& p, ShareShared& s
 }
 
 // Row r of a unit over positions [t0, t1) in fp32 by one warp, to the output or
-// to the unit's partial sums (whose weights carry 2^shift).  false: the unit has
-// no such row.
+// to the unit's partial sums (whose weights carry 2^shift, and whose row sums are
+// multiplied by sum_scale).  false: the unit has no such row.
 template <int D, int ROWS>
-__device__ bool row_in_fp32(const ChunkParams& p, const Unit& u, int r, int t0, int t1, float* partial, float shift) {
+__device__ bool row_in_fp32(const ChunkParams& p, const Unit& u, int r, int t0, int t1, float* partial, float shift,
+                            float sum_scale) {
     const int G = p.H / p.Hkv, per = ROWS / G, lane = threadIdx.x & 31, token = u.tile * per + r / G;
     if (r >= per * G || token >= u.n) return false;
     const int h = u.head * G + r % G, sees = min(u.len - u.n + token + 1, u.limit);
@@ -252,7 +253,7 @@ __device__ bool row_in_fp32(const ChunkParams& p, const Unit& u, int r, int t0, 
     }
     if (partial && lane == 0) {
         partial[ROWS * D + r] = sum.m * 1.4426950408889634f + shift;
-        partial[ROWS * (D + 1) + r] = sum.l;
+        partial[ROWS * (D + 1) + r] = sum.l * sum_scale;
     }
     return true;
 }
@@ -291,7 +292,8 @@ struct CombineSum {
 
 template <int D, int ROWS>
 __global__ void __launch_bounds__(kCombineThreads, 2)
-    chunk_combine_kernel(ChunkParams p, const float* partials, const ChunkSplit* splits, int shares, bool wide_out) {
+    chunk_combine_kernel(ChunkParams p, const float* partials, const ChunkSplit* splits, int shares, bool wide_out,
+                         float sum_scale) {
     constexpr int kGroups = ROWS / kCombineRows, kEach = CombineSum<D>::kEach, kAcross = D / 4;
     constexpr int kAtOnce = D == 128 ? 1 : D == 64 ? 2 : 4;  // parts in flight
     __shared__ float4 sums[kCombineWarps][kEach][32];
@@ -340,7 +342,7 @@ __global__ void __launch_bounds__(kCombineThreads, 2)
         const int r = r0 + row_of(i);
         if (r >= t.rows) return;
         float* dst = p.out + (t.row + r / G) * p.ld_out + (size_t)(t.head * G + r % G) * D + (lane + 32 * i) % kAcross * 4;
-        const float n = 1.0f / l;
+        const float n = sum_scale / l;  // the parts' sums are multiplied by it
         float4 y = make_float4(v.x * n, v.y * n, v.z * n, v.w * n);
         if (r < t.blank) y = make_float4(0, 0, 0, 0);  // whatever the parts hold
         if (wide_out)
@@ -380,7 +382,7 @@ __global__ void __launch_bounds__(kCombineThreads, 2)
 
 template <int D, int ROWS>
 cudaError_t launch_combine(const ChunkParams& p, int shares, const float* partials, const ChunkSplit* splits,
-                           bool wide_out, cudaStream_t stream) {
+                           bool wide_out, float sum_scale, cudaStream_t stream) {
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3((unsigned)((shares + kCombineWarps - 1) / kCombineWarps * (ROWS / kCombineRows)));
     cfg.blockDim = dim3(kCombineThreads);
@@ -390,7 +392,7 @@ cudaError_t launch_combine(const ChunkParams& p, int shares, const float* partia
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, chunk_combine_kernel<D, ROWS>, p, partials, splits, shares, wide_out);
+    return cudaLaunchKernelEx(&cfg, chunk_combine_kernel<D, ROWS>, p, partials, splits, shares, wide_out, sum_scale);
 }
 
 }  // namespace tb
