@@ -128,3 +128,17 @@ def test_a_long_context_of_zero_values(serving, max_len):  # noqa: F811
     c["pool"][c["table"][0, :-60], :, 1] = 0
     c["pool"][:, :, 1] *= np.float32(1e-3)
     check(serving, c, max_len=max_len)
+
+
+@pytest.mark.parametrize("H,kv,d,total,new", [
+    (8, 1, 64, [8192, 0], [2048, 64]), (8, 1, 64, [0, 8192, 30], [300, 2048, 200]), (4, 4, 128, [0, 4000], [40, 3200]),
+    (4, 2, 32, [2000, 0, 0], [2000, 1, 700]), (8, 1, 64, [300, 0], [70, 64]), (8, 1, 64, [300, 0], [1, 1])])
+@pytest.mark.parametrize("fill", [0, 0xFF, 0x7F])
+def test_rows_without_a_position_are_zeros_whatever_the_workspace_holds(serving, H, kv, d, total, new, fill):  # noqa: F811
+    c = attend_case(d, total, new, H, kv, d)
+    need = serving.paged_attention_chunk_workspace(sum(new), len(new), max(new), max(total), H, kv, d)
+    w = torch.full((need,), fill, dtype=torch.uint8, device="cuda")
+    out = check(serving, c, workspace=w)
+    for s, (L, n) in enumerate(zip(total, new)):
+        a = int(c["offsets"][s])
+        assert (out[a:a + max(n - L, 0)] == 0).all()

@@ -890,10 +890,11 @@ __global__ void __launch_bounds__(Roles<PRE>::kThreads, 1)
                 l = 0.0f;
                 for (int k = 0; k < 4; ++k) l = fmaf(ex2(sh.quad_m[k * 32 + lane] - off), sh.quad_l[k * 32 + lane], l);
             }
+            const bool blank = !part && sees <= 0;  // zeros, whatever the sums hold
             if (!part) {
-                const float inv = sees > 0 ? kSumScale / l : 0.0f;
-                w0 = sees > 0 ? w0 * inv : 0.0f;
-                w1 = sees > 0 ? w1 * inv : 0.0f;
+                const float inv = kSumScale / l;
+                w0 *= inv;
+                w1 *= inv;
             }
             float* dst = part ? part + (size_t)row * D
                               : p.out + (done.first + (valid ? token : 0)) * p.ld_out +
@@ -913,7 +914,7 @@ __global__ void __launch_bounds__(Roles<PRE>::kThreads, 1)
                         if (merge)
                             y = __ffma2_rn(make_float2(__int_as_float(v[2 * x]), __int_as_float(v[2 * x + 1])),
                                            make_float2(w1, w1), y);
-                        acc[o / 2 + x] = y;
+                        acc[o / 2 + x] = blank ? make_float2(0.0f, 0.0f) : y;
                     }
                     if (small) {  // the first warp adds the others', 16 dims at a time
                         if (o) named_bar_sync(1, 128);
@@ -992,7 +993,8 @@ __global__ void __launch_bounds__(kOperandWarps * 32) chunk_operands_kernel(Chun
     int first, n;
     rows_of(p, s, first, n);
     const int len = p.total_lens[s], limit = min(len, p.stride * kPageTokens);
-    if (n == 0 || tile * S::NT >= limit || len > pre.tiles * S::NT) return;
+    // (the units of a sequence without a position read its first tile too)
+    if (n == 0 || tile * S::NT >= max(limit, 1) || len > pre.tiles * S::NT) return;
     const size_t t = operand_tile<D>(p, pre, s, head, tile);
     uint8_t* buf = smem + warp * S::kPageBytes;
     const int pos = tile * S::NT + page * kPageTokens, id = pos < limit ? page_at(p, s, pos) : -1;
