@@ -1007,7 +1007,7 @@ __global__ void __launch_bounds__(kOperandWarps * 32) chunk_operands_kernel(Chun
             bulk_g2s(buf, head_rows<D>(p, id, j / PG, head), S::kPageBytes, bar + warp);
         }
         __syncwarp();
-        mbar_wait(bar + warp, 0, p.err);
+        if (!mbar_wait(bar + warp, 0, p.err)) land_copies();
     }
     const int valid = id >= 0 ? min(limit - pos, kPageTokens) : 0;
     const float* src = reinterpret_cast<const float*>(buf);
