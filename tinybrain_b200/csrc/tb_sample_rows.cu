@@ -35,6 +35,7 @@
 #include <climits>
 
 #include "tb_common.cuh"
+#include "tb_sample_cut.h"
 #include "tb_stream_entry.h"
 #include "tb_unit.cuh"
 
@@ -50,7 +51,6 @@ constexpr int kMaxCluster = 8;
 constexpr int kList = 512;           // boundary elements that a CTA notes, and that are ranked
 constexpr int kStagedMax = 44 * 1024;  // elements of a CTA that fit its shared memory
 constexpr float kBinSpan = 24.0f;      // nats below the maximum that the histogram resolves
-constexpr float kNoWeight = 700.0f;    // nats below the maximum where weights end
 constexpr int kRoots = 64;
 constexpr int kBatch = 16;             // loads of a lane in flight while the row is read
 
@@ -224,7 +224,7 @@ struct Row {
         }
         return best;
     }
-    // exp(y) of y = (v - top) / T in [-701, 0] as 2^q 2^(j / 64) e^r, |r| <= ln 2 / 128,
+    // exp(y) of y = (v - top) / T in [-700, 0] (lowest_weighted) as 2^q 2^(j / 64) e^r, |r| <= ln 2 / 128,
     // the root of two from a table and e^r by its series to r^5 / 5! (the next term is
     // below 2^-54): the table-driven method of P. T. P. Tang, ACM TOMS 15 (1989).  exp()
     // itself has a branch for its ends, across which four elements do not overlap.
@@ -561,6 +561,10 @@ __global__ void __launch_bounds__(kRowThreads) sample_rows_kernel(RowsParams p) 
     }
     if (threadIdx.x < kRoots) sh.root[threadIdx.x] = exp2((double)threadIdx.x / kRoots);
     if (threadIdx.x < 2) sh.listed[threadIdx.x] = 0;
+    if (threadIdx.x == 0) {
+        sh.pick = -1;
+        sh.pick_weight = 0.0;
+    }
     if (P > 1) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
     const float T = p.temperature ? p.temperature[row] : 1.0f;
     const int k = p.top_k ? p.top_k[row] : 0;
@@ -586,7 +590,7 @@ __global__ void __launch_bounds__(kRowThreads) sample_rows_kernel(RowsParams p) 
     r.inv_t = 1.0 / (double)T;
     r.bin_scale = (float)((double)kRowBins / kBinSpan * r.inv_t);
     // below this there is no weight; an infinite maximum shares it with its like alone
-    r.cut = r.top == INFINITY ? INFINITY : r.top - kNoWeight * T;
+    r.cut = r.top == INFINITY ? INFINITY : lowest_weighted(r.top, T);
     r.cut_index = r.cut > -INFINITY ? INT_MAX : -1;
 
     // 2. the kept prefix's last element: top-k's, and top-p's within it
@@ -675,7 +679,8 @@ __global__ void __launch_bounds__(kRowThreads) sample_rows_kernel(RowsParams p) 
     }
     const unsigned who = __ballot_sync(0xffffffffu, run >= 0);
     const int src = who ? __ffs(who) - 1 : 0;
-    run = __shfl_sync(0xffffffffu, run, src);
+    // (one always has it, unless the row changes while it is read: no run before the first then)
+    run = max(__shfl_sync(0xffffffffu, run, src), 0);
     run_before = __shfl_sync(0xffffffffu, run_before, src);
     // 5. the element, by the warps of the CTA that has the run: each scans the lanes'
     // fours of 128 elements, and the first whose sum passes the goal has it
