@@ -91,9 +91,11 @@ constexpr uint32_t kWildBits = (127u + 20u) << 23;    // a K or V value of 2^20
 constexpr uint32_t kWildQueryBits = (127u + 40u) << 23;
 constexpr float kPShift = 6.0f;   // P = 2^(6 + score - M), M within 2^8 of the maximum: at most 2^14
 constexpr float kLazy = 8.0f;
-// The row sums count in 2^kSumShift: over pages of zeros a term is up to 2^(14 + 100),
-// and 2^31 of them have to fit; the smallest sum is 2^(6 - 6 - kSumShift).
-constexpr float kSumShift = 32.0f, kSumScale = 1.0f / 4294967296.0f;
+// The pages' value exponents are kept with 32 added (the reference maximum has it too,
+// so P does not), and the row sums thus count in 2^32: over pages of zeros a term is up
+// to 2^(14 + 100), and 2^31 of them have to fit; the smallest sum is 2^(6 - 6 - 32).
+constexpr int kSumShift = 32;
+constexpr float kSumScale = 1.0f / 4294967296.0f;
 constexpr float kWildMark = 3e38f;
 constexpr float kHuge = 1048576.0f;  // a score whose rounding could carry P out of fp16's range
 
@@ -259,7 +261,7 @@ __device__ __forceinline__ void convert_v(const float* src, int valid, uint8_t* 
     const uint32_t bits = both(warp_max_bits(m), page, part);
     const int e = block_exponent(bits, kLowestValue);
     const float s = exp2_int(-e);
-    if (lane == 0 && part == 0) *exp_out = bits >= kWildBits ? kWildMark : (float)e;
+    if (lane == 0 && part == 0) *exp_out = bits >= kWildBits ? kWildMark : (float)(e + kSumShift);
 #pragma unroll
     for (int t = 0; t < kTasks; ++t) {
         const int task = lane + 32 * t, n = part * kDims + task % kDims, kc = task / kDims;
@@ -349,7 +351,7 @@ template <int D>
 __device__ __noinline__ void rows_without_operands(const ChunkParams& p, const Unit& u, int t0, int t1, float* partial) {
     const int first = (threadIdx.x >> 5) * 32;
     for (int r = first; r < first + 32; ++r)  // the even warpgroup's warps 0 to 3
-        if (!row_in_fp32<D, kTileRows>(p, u, r, t0, t1, partial, kPShift, kSumScale)) break;
+        if (!row_in_fp32<D, kTileRows>(p, u, r, t0, t1, partial, kPShift + kSumShift, kSumScale)) break;
 }
 
 template <int D, bool PRE>
@@ -711,7 +713,7 @@ __global__ void __launch_bounds__(Roles<PRE>::kThreads, 1)
                             sum = __fadd2_rn(sum, w);
                             split_pair(w.x, w.y, hi[x / 2], lo[x / 2]);
                         }
-                        l = fmaf(sum.x + sum.y, ex2(-e - kSumShift), l);
+                        l = fmaf(sum.x + sum.y, ex2(-e), l);
                     };
                     float r = 1.0f;
                     // takes the block's maximum into the reference; the result is P's shift
