@@ -142,3 +142,12 @@ def test_rows_without_a_position_are_zeros_whatever_the_workspace_holds(serving,
     for s, (L, n) in enumerate(zip(total, new)):
         a = int(c["offsets"][s])
         assert (out[a:a + max(n - L, 0)] == 0).all()
+
+
+def test_rows_without_operands_over_a_long_context(serving):  # noqa: F811
+    # bounds of one token launch one CTA; its first unit is summed in fp32 for longer than its other warps'
+    # limit of 2 s, and a second unit follows.  (What makes it so is a key of 2^21, which the queries do not see.)
+    c = attend_case(5, [131072], [9], 16, 1, 128, layers=1)
+    c["q"].reshape(9, 16, 128)[:, :, 0] = 0
+    c["pool"][c["table"][0, 0], 0, 0, 0, 0, 0] = 2.0 ** 21
+    check(serving, c, max_new=1, max_len=1)

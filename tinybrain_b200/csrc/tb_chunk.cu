@@ -166,7 +166,7 @@ struct ChunkShared {
     float quad_m[kTileRows], quad_l[kTileRows];       // the even warpgroup's warps', in small units
     float quad_sum[3][32][17];
     int merge_wild[4], quad_wild[4];
-    volatile int dead;  // a wait ran out: nobody waits any more
+    ChunkWatch watch;
 };
 
 // What frees the operand tile that position tile i goes to: the product with its
@@ -176,7 +176,7 @@ __device__ __forceinline__ uint64_t* free_bar(uint64_t* ring, int i, int stages)
 }
 __device__ __forceinline__ uint32_t free_parity(int i, int stages) { return (uint32_t)((i - stages) / kEmptyRing & 1); }
 __device__ __forceinline__ void warp_wait(ChunkShared& sh, uint64_t* bar, uint32_t parity, int* err) {
-    if ((threadIdx.x & 31) == 0) chunk_wait(&sh.dead, bar, parity, err);
+    if ((threadIdx.x & 31) == 0) chunk_wait(&sh.watch, bar, parity, err);
     __syncwarp();
 }
 
@@ -348,10 +348,14 @@ __device__ __forceinline__ void load_queries(Row row, bool wide, uint32_t tq, fl
 
 // A unit's rows of one warp in fp32 (pages or queries without fp16 operands).
 template <int D>
-__device__ __noinline__ void rows_without_operands(const ChunkParams& p, const Unit& u, int t0, int t1, float* partial) {
+__device__ __noinline__ void rows_without_operands(const ChunkParams& p, const Unit& u, int t0, int t1, float* partial,
+                                                   ChunkWatch* watch) {
     const int first = (threadIdx.x >> 5) * 32;
-    for (int r = first; r < first + 32; ++r)  // the even warpgroup's warps 0 to 3
+    for (int r = first; r < first + 32; ++r) {  // the even warpgroup's warps 0 to 3
+        const unsigned long long since = global_timer_ns();
         if (!row_in_fp32<D, kTileRows>(p, u, r, t0, t1, partial, kPShift + kSumShift, kSumScale)) break;
+        if ((threadIdx.x & 31) == 0) atomicAdd(&watch->limit, global_timer_ns() - since);
+    }
 }
 
 template <int D, bool PRE>
@@ -377,7 +381,7 @@ __global__ void __launch_bounds__(Roles<PRE>::kThreads, 1)
     ChunkBars& b = sh.bars;
 
     if (tid == 0) {
-        sh.dead = 0;
+        watch_init(sh.watch);
         for (int i = 0; i < S::kSlots; ++i) {
             for (int f = 0; f < 2; ++f) {
                 mbar_init(b.slot_full[f] + i, 1);
@@ -426,26 +430,26 @@ __global__ void __launch_bounds__(Roles<PRE>::kThreads, 1)
         if constexpr (PRE) {
             int i = 0;
             if (lane == 0) {
-                for (int left = count; left > 0 && !sh.dead; at = 0) {
+                for (int left = count; left > 0 && !sh.watch.dead; at = 0) {
                     const int take = min(u.tiles - at, left);
                     for (int j = at; j < at + take; ++j, ++i) {
                         const int sk = i % kKStages, sv = i % kVStages, ring = i % kScaleRing;
                         const bool made = u.len <= pre.tiles * NT;  // a longer one goes without operands
                         const size_t t = made ? operand_tile<D>(p, pre, u.s, u.head, j) : 0;
                         const uint8_t* src = pre.ops + t * (4 * S::kHalf);
-                        if (i >= kKStages && !chunk_wait(&sh.dead, free_bar(b.k_empty, i, kKStages), free_parity(i, kKStages), p.err)) break;
+                        if (i >= kKStages && !chunk_wait(&sh.watch, free_bar(b.k_empty, i, kKStages), free_parity(i, kKStages), p.err)) break;
                         mbar_arrive_expect_tx(b.scales + ring, 64);
                         bulk_g2s(sh.scale[ring], pre.scales + t * 16, 64, b.scales + ring);
                         mbar_arrive_expect_tx(b.k_full + sk, 2 * S::kHalf);
                         bulk_g2s(k_ops + sk * 2 * S::kHalf, src, 2 * S::kHalf, b.k_full + sk);
-                        if (i >= kVStages && !chunk_wait(&sh.dead, free_bar(b.v_empty, i, kVStages), free_parity(i, kVStages), p.err)) break;
+                        if (i >= kVStages && !chunk_wait(&sh.watch, free_bar(b.v_empty, i, kVStages), free_parity(i, kVStages), p.err)) break;
                         mbar_arrive_expect_tx(b.v_full + sv, 2 * S::kHalf);
                         bulk_g2s(v_ops + sv * 2 * S::kHalf, src + 2 * S::kHalf, 2 * S::kHalf, b.v_full + sv);
                     }
                     left -= take;
                     if (left > 0) next_unit<NT, kTileRows>(p, u);
                 }
-                if (sh.dead) land_copies();
+                if (sh.watch.dead) land_copies();
             }
             __syncwarp();
         } else {
@@ -461,7 +465,7 @@ __global__ void __launch_bounds__(Roles<PRE>::kThreads, 1)
             return mine && pos < u.limit ? p.table[(size_t)u.s * p.stride + pos / kPageTokens] : -1;
         };
         int left = count, j = at, end_j = at + min(u.tiles - at, left), page = entry(j);
-        while (left > 0 && !sh.dead) {
+        while (left > 0 && !sh.watch.dead) {
             const int id = checked_page(p, page);
             const float* src = head_rows<D>(p, max(id, 0), kv, u.head);
             if (--left > 0) {
@@ -476,9 +480,9 @@ __global__ void __launch_bounds__(Roles<PRE>::kThreads, 1)
             for (int g = 0; g < PG; g += 4) {
                 const bool turn = lane >= g && lane < g + 4;
                 const int last = fill - 1;
-                lanes_wait(&sh.dead, turn && fill ? b.slot_empty[last & 1] + slot : nullptr, (uint32_t)(last >> 1) & 1,
+                lanes_wait(&sh.watch, turn && fill ? b.slot_empty[last & 1] + slot : nullptr, (uint32_t)(last >> 1) & 1,
                            p.err);
-                if (turn && !sh.dead) {
+                if (turn && !sh.watch.dead) {
                     sh.slot_page[slot] = id;
                     uint64_t* full = b.slot_full[fill & 1] + slot;
                     mbar_arrive_expect_tx(full, id >= 0 ? S::kPageBytes : 0);
@@ -492,7 +496,7 @@ __global__ void __launch_bounds__(Roles<PRE>::kThreads, 1)
                 ++fill;
             }
         }
-        if (sh.dead) land_copies();
+        if (sh.watch.dead) land_copies();
         }
     } else if (count > 0 && warp == kIssueWarp) {
         // ---- issuer ----
@@ -502,8 +506,8 @@ __global__ void __launch_bounds__(Roles<PRE>::kThreads, 1)
             int i = 0, unit = 0;
             const auto issue_s = [&](int item, bool first, int un) {
                 const int st = item % kKStages;
-                if (first) chunk_wait(&sh.dead, b.q_full + un % kUnitRing, (uint32_t)(un / kUnitRing & 1), p.err);
-                chunk_wait(&sh.dead, b.k_full + st, (uint32_t)(item / kKStages & 1), p.err);
+                if (first) chunk_wait(&sh.watch, b.q_full + un % kUnitRing, (uint32_t)(un / kUnitRing & 1), p.err);
+                chunk_wait(&sh.watch, b.k_full + st, (uint32_t)(item / kKStages & 1), p.err);
                 tc_fence_after();
                 const uint32_t kb = k0 + st * 2 * S::kHalf;
                 tc_mma_split<NT, D>(tmem + (uint32_t)(item % kSBufs) * NT, tmem + kQ, [](int s) { return 8 * s; }, D / 2,
@@ -519,11 +523,11 @@ __global__ void __launch_bounds__(Roles<PRE>::kThreads, 1)
                 for (int j = 0; j < take; ++j, ++i) {
                     if (j + kAhead < take) issue_s(i + kAhead, false, unit);
                     const int st = i % kVStages;
-                    chunk_wait(&sh.dead, b.v_full + st, (uint32_t)(i / kVStages & 1), p.err);
-                    chunk_wait(&sh.dead, b.p_full + i % kSBufs, (uint32_t)(i / kSBufs & 1), p.err);
+                    chunk_wait(&sh.watch, b.v_full + st, (uint32_t)(i / kVStages & 1), p.err);
+                    chunk_wait(&sh.watch, b.p_full + i % kSBufs, (uint32_t)(i / kSBufs & 1), p.err);
                     // (of two buffers, O of two tiles before was read before P of this one arrived)
                     if (kOBufs == 1 && i > 0)
-                        chunk_wait(&sh.dead, b.o_read + (i - 1 & 1), (uint32_t)((i - 1) / 2 & 1), p.err);
+                        chunk_wait(&sh.watch, b.o_read + (i - 1 & 1), (uint32_t)((i - 1) / 2 & 1), p.err);
                     tc_fence_after();
                     const uint32_t vb = v0 + st * 2 * S::kHalf;
                     // P: 16 columns of high, 16 of low halves per 32 positions
@@ -561,7 +565,7 @@ __global__ void __launch_bounds__(Roles<PRE>::kThreads, 1)
                     const int slot = (job + kv * PG) % S::kSlots, fill = (job + kv * PG) / S::kSlots;
                     const int st = kv ? i % kVStages : i % kKStages, stages = kv ? kVStages : kKStages;
                     // lane 0: the page, lane 1: its place in the operand tile
-                    lanes_wait(&sh.dead,
+                    lanes_wait(&sh.watch,
                                lane == 0   ? b.slot_full[fill & 1] + slot
                                : lane == 1 ? free_bar(kv ? b.v_empty : b.k_empty, i, stages)
                                            : nullptr,
@@ -675,7 +679,7 @@ __global__ void __launch_bounds__(Roles<PRE>::kThreads, 1)
             for (i = first; i < i0 + take; i += kGroups) {
                 const uint32_t ts = s0_addr + (uint32_t)(i % kSBufs) * NT;
                 const int j = at + (i - i0), ring = i % kScaleRing;
-                lanes_wait(&sh.dead, lane == 0 ? b.scales + ring : lane == 1 ? b.s_full + i % kSBufs : nullptr,
+                lanes_wait(&sh.watch, lane == 0 ? b.scales + ring : lane == 1 ? b.s_full + i % kSBufs : nullptr,
                            (uint32_t)(lane == 0 ? i / kScaleRing : i / kSBufs) & 1, p.err);
                 tc_fence_after();
                 if (busy) {
@@ -963,7 +967,8 @@ __global__ void __launch_bounds__(Roles<PRE>::kThreads, 1)
                 __syncwarp();
                 if (lane == 0) mbar_arrive(b.merge_read + quad);
             }
-            if (busy && wild) rows_without_operands<D>(p, done, from * NT, (from + take) * NT, part);
+            if (busy && wild)
+                rows_without_operands<D>(p, done, from * NT, (from + take) * NT, part, &sh.watch);
         }
         if (tid == 0) splits[blockIdx.x] = split;
     } else if (count > 0) {

@@ -46,7 +46,7 @@ struct FewShared {
     uint64_t full[F::kWarps][F::kRing];
     int id[F::kWarps][F::kRing];
     long long scan[F::kWarps], before[F::kThreads], mine[F::kThreads];
-    volatile int dead;
+    ChunkWatch watch;
 };
 
 __device__ __forceinline__ void mma_tf32(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
@@ -111,7 +111,7 @@ __global__ void __launch_bounds__(Few<D>::kThreads, 1)
     uint8_t* ring = smem + (size_t)warp * kRing * F::kPageBytes;
     if (lane == 0) {
         for (int i = 0; i < kRing; ++i) mbar_init(&sh.full[warp][i], 1);
-        if (warp == 0) sh.dead = 0;
+        if (warp == 0) watch_init(sh.watch);
         fence_barrier_init();
         fence_proxy_async_shared();
     }
@@ -224,7 +224,7 @@ __global__ void __launch_bounds__(Few<D>::kThreads, 1)
     };
     // the next page in the ring; its pool page (-1: zeros)
     const auto take_page = [&](const float*& rows) {
-        if (lane == 0) chunk_wait(&sh.dead, &sh.full[warp][slot], (uint32_t)phase, p.err);
+        if (lane == 0) chunk_wait(&sh.watch, &sh.full[warp][slot], (uint32_t)phase, p.err);
         __syncwarp();
         rows = reinterpret_cast<const float*>(ring + slot * F::kPageBytes);
         return sh.id[warp][slot];
@@ -235,7 +235,7 @@ __global__ void __launch_bounds__(Few<D>::kThreads, 1)
             slot = 0;
             phase ^= 1;
         }
-        if (more && !sh.dead)
+        if (more && !sh.watch.dead)
             fetch_next();
         else
             --held;
@@ -482,7 +482,7 @@ __global__ void __launch_bounds__(Few<D>::kThreads, 1)
         }
     } while (WHOLE || now.next_piece(p));
     if (!WHOLE && lane == 0) splits[share.index] = split;
-    if (sh.dead) land_copies();
+    if (sh.watch.dead) land_copies();
 }
 
 }  // namespace

@@ -97,15 +97,25 @@ __device__ __forceinline__ bool sleep_on(uint64_t* bar, uint32_t parity) {
         : "memory");
     return ok != 0;
 }
-// A wait that runs out sets *dead, after which nobody in the CTA waits any more.
-__device__ __forceinline__ bool chunk_wait(volatile int* dead, uint64_t* bar, uint32_t parity, int* err) {
+// What the waits of a CTA go by.  One that takes longer than `limit` (ns) sets `dead`,
+// after which nobody waits any more.  Rows summed in fp32 add their own time to the
+// limit: 128 of them over 65536 positions take 0.7 s, for which the other warps wait.
+struct ChunkWatch {
+    volatile int dead;
+    unsigned long long limit;
+};
+__device__ __forceinline__ void watch_init(ChunkWatch& watch) {
+    watch.dead = 0;
+    watch.limit = kWaitLimitNs;
+}
+__device__ __forceinline__ bool chunk_wait(ChunkWatch* watch, uint64_t* bar, uint32_t parity, int* err) {
     if (sleep_on(bar, parity)) return true;
-    const uint64_t t0 = global_timer_ns();
-    while (!*dead) {
+    const unsigned long long t0 = global_timer_ns();
+    while (!watch->dead) {
         if (sleep_on(bar, parity)) return true;
-        if (global_timer_ns() - t0 > kWaitLimitNs) {
+        if (global_timer_ns() - t0 > *static_cast<volatile unsigned long long*>(&watch->limit)) {
             record_error(err, kDevWaitTimeout);
-            *dead = 1;
+            watch->dead = 1;
         }
     }
     return false;
@@ -120,10 +130,10 @@ __device__ __forceinline__ void land_copies() {
 // The same for several barriers at once: every lane with one of its own (bar not
 // null) waits for it, all return together.  With the roles' code spread over the
 // instruction cache a wait costs some 300 cycles even where nothing is missing.
-__device__ __forceinline__ void lanes_wait(volatile int* dead, uint64_t* bar, uint32_t parity, int* err) {
+__device__ __forceinline__ void lanes_wait(ChunkWatch* watch, uint64_t* bar, uint32_t parity, int* err) {
     bool ok = !bar || sleep_on(bar, parity);
     if (__all_sync(0xffffffffu, ok)) return;
-    if (!ok) chunk_wait(dead, bar, parity, err);
+    if (!ok) chunk_wait(watch, bar, parity, err);
     __syncwarp();
 }
 // What a share leaves for chunk_combine_kernel: its last unit, if that begins
