@@ -279,8 +279,19 @@ tb_status tb_rope_append_paged_dev(void *stream, const float *q_dev, int64_t ld_
  * (larger ones stay right).
  * The workspace is tb_paged_attention_chunk_workspace bytes of device memory for
  * the same bounds (where that is 0, NULL will do), 16-byte aligned, for this
- * call's use until it has run: calls that may overlap need their own.  head_dim
- * 16, 32, 64 or 128; num_heads / num_kv_heads <= 128. */
+ * call's use until it has run: calls that may overlap need their own.  It is up
+ * to 30 MB, and where many rows share their keys as much more as one layer's K
+ * and V of batch * max_len tokens, at most 1 GiB: a max_len near the longest length
+ * keeps it small.  head_dim 16, 32, 64 or 128; num_heads / num_kv_heads <= 128.
+ * Accuracy: sums, maxima and row sums are fp32; products are of factors carried
+ * to 2^-22 of themselves, so a score is off by at most 3 * 2^-22 of
+ * sum |q_i k_i| / sqrt(head_dim), and a weight by as much relative to itself.
+ * Sequences with more than eight rows of a KV head carry a query row, and the K
+ * and the V of a page and head, at one power-of-two scale each: what lies below
+ * 2^-39 of the largest magnitude there is lost.  With queries and keys of unit
+ * size the result is within 1e-5 (relative L2) of 64 bits, whatever the size of
+ * the values.  Keys and values from 2^20, queries from 2^40, scores beyond 7e5 and
+ * what is not finite are summed in plain fp32 instead, some hundred times slower. */
 tb_status tb_paged_attention_chunk_workspace(int32_t rows, int32_t batch, int32_t max_new, int32_t max_len,
                                              int32_t num_heads, int32_t num_kv_heads, int32_t head_dim,
                                              int64_t *bytes);
@@ -300,8 +311,10 @@ tb_status tb_paged_attention_chunk_dev(void *stream, const float *q_dev, int64_t
  * largest (<= 0 off).  The token is the first kept index whose running mass
  * exceeds uniform times the kept mass.  prob_dev and entropy_dev (NULL or
  * [rows]) get the token's probability and the entropy (nats) of the kept
- * distribution, as TokenOutput has them.  NaN counts as -inf, a weight below
- * e^-700 of the largest as 0; a row with nothing above -inf gets token -1,
+ * distribution, as TokenOutput has them.  Weights and sums are fp64, the masses
+ * that place top_p whole multiples of 2^-(62 - ceil(log2 vocab_size)) of the
+ * largest weight, so that no launch shape changes a token.  NaN counts as -inf, a
+ * weight below e^-700 of the largest as 0; a row with nothing above -inf gets token -1,
  * probability and entropy 0.  The order of
  * the steps is not tb_runner_set_sampler's, which follows the reference: there
  * the temperature comes last, top_p applies only without top_k, and there is

@@ -5,9 +5,11 @@
 // empty, and making its operands costs more than the products.  Here every warp
 // takes an equal share of all pages of all units, streams them through its own
 // ring of bulk copies and waits for no other warp; units that several warps hold
-// are joined by chunk_combine_kernel.  WHOLE, for little work: the warps of a CTA
-// share a unit's pages and join them at its end, without the second launch.  (Sixteen warps on one unit, joined at its
-// end, spent a fifth of their time at that barrier.)  Per page of 16 tokens:
+// are joined by chunk_combine_kernel.  (In the 64-sequence step below, sixteen warps
+// on one unit after the other, joined at each one's end, spent a fifth of their time
+// at that barrier.)  WHOLE, for so little work that a second launch would cost more:
+// the warps of a CTA do share a unit's pages and join them at its end.
+// Per page of 16 tokens:
 //   scores  mma.sync m16n8k8 on the fp32 page as it lies: A = 16 tokens, B = the
 //           rows' queries from registers, both split into a TF32 high part and
 //           the rest (3 products in separate chains, the small ones apart);
@@ -15,9 +17,9 @@
 //           it by 2^8 (one vote a page);
 //   sums    V in plain fp32 FMAs: a lane holds D / 32 dims of all rows, a row of
 //           V is one conflict-free load, the weights are broadcast loads.
-// Bound by issue slots beside HBM.  Measured: 64 sequences of 512 to 4224 tokens, 32
-// query and 4 KV heads of 64, 73 us for 290 MB, 4.0 TB/s; WHOLE, one token over 129
-// positions, 10 us with its launch.
+// Bound by issue slots (45 % of the cycles) beside HBM.  Measured: 64 sequences of 512
+// to 4224 tokens, 32 query and 4 KV heads of 64, 69 us for 290 MB, 4.2 TB/s; WHOLE, one
+// token over 129 positions, 10 us.
 // The dims of a lane in the scores' products are four neighbours: k is a label,
 // the same for A and B.
 #pragma once

@@ -1,7 +1,7 @@
 // tb_chunk_units.cuh -- what the kernels of the chunk attention (tb_chunk.cu,
-// tb_chunk_few.cu) share: the call's parameters, its division into units and
-// into equal shares of the CTAs, the partial sums of units that several CTAs
-// hold, and one row in plain fp32.
+// tb_chunk_few.cuh) share beside the walk over units (tb_chunk_walk.h): their waits,
+// the search for a CTA's share, the partial sums of units that several CTAs hold,
+// and one row in plain fp32.
 #pragma once
 
 #include <climits>

@@ -28,9 +28,9 @@
 // each other's shared memory ahead of a barrier, after which it is read locally.
 //
 // Bound by the barriers' and reads' latency for few rows, by instruction issue for
-// many.  Measured: one row of 32000 11 us, 64 rows 24 us; 256 rows of 131072, each
-// with its own settings, 162 us (0.8 TB/s); greedy alone 43 us, without truncation
-// 113, top-p 0.9 254.
+// many.  Measured: one row of 32000 12 us, 64 rows 24 us; 256 rows of 131072, each
+// with its own settings, 161 us (0.8 TB/s); greedy alone 43 us, without truncation
+// 114, top-k 40 153, top-p 0.9 219 (at temperature 0.8).
 #include <cfloat>
 #include <climits>
 
@@ -786,8 +786,9 @@ extern "C" tb_status tb_sample_rows_dev(void* stream, const float* logits, int64
                        prob, entropy};
     // CTAs of a row: while the rows leave SMs idle and a CTA would still have 2048
     // elements to read, or while a CTA's part leaves no room for others on its SM.
-    // Measured, us: one row of 32000 P = 1 31, 2 21, 4 16, 8 14; 64 rows 62, 41, 35,
-    // 43; 256 rows of 131072 P = 4 267, 8 222
+    // Measured, us by P = 1, 2, 4, 8: rows of 32000: one 22, 16, 13, 12; 16 36, 25, 19, 19;
+    // 64 41, 28, 24, 29; 128 41, 34, 33, 52; 256 53, 46, 58, 101.  Of 4096: one 8, 9, 10,
+    // 10; 64 13, 13, 17, 24.  256 rows of 131072: P = 4 177, 8 161
     int P = 1;
     while (P < kMaxCluster &&
            (((long long)rows * P < entry.num_sms && V / (2 * P) >= 2048) || V / P > 16 * 1024))

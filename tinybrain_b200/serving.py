@@ -13,13 +13,16 @@ may be captured into a CUDA graph.  The cache is the framework's pool,
 ValueError before anything runs; bad pages and positions found on the device
 are reported by `check_device`.
 
-A step (row counts on the device; buffers of the largest step):
+A step (row counts on the device; buffers of the largest step).  The tokens are
+sampled from each sequence's last row alone (of one without new tokens: some row):
 
     build_page_tables(cached, new, free, table, offsets, total, seq, pos, slot, info)
+    last = (offsets[1:] - 1).clamp(min=0)
     for layer in range(num_layers):
         ...                                             # q, k, v projections
         rope_append(q, k, v, pos, slot, rope, pool, q, layer=layer, num_rows=offsets[-1:])
         paged_attention_chunk(q, offsets, total, pool, table, out, layer=layer, max_new=.., max_len=..)
+    ...                                                 # logits of the rows `last`: [sequences, vocab]
     token = sample_rows(logits, uniform, temperature=.., top_k=.., top_p=.., min_p=..)[0]
 """
 from __future__ import annotations
@@ -175,7 +178,9 @@ def paged_attention_chunk(q, row_offsets, total_lens, pool, page_table, out=None
     sequence's new tokens and length (they shape the launch; larger ones stay
     right).  workspace: a uint8 tensor of paged_attention_chunk_workspace bytes
     that no overlapping call uses; None takes one from torch's allocator for
-    this call.  Returns out."""
+    this call: up to 30 MB, and for long prompts as much more as one layer's K and V
+    of sequences * max_len tokens, at most 1 GiB (a tight max_len keeps it small).
+    The header states the accuracy.  Returns out."""
     gpu, pages, layers, kv, d = _pool(pool, layer)
     batch, stride = _table(page_table, gpu)
     qp, ld_q = _rows(q, "q", gpu)
