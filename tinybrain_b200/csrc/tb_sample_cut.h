@@ -19,8 +19,12 @@ constexpr double kNoWeight = 700.0;  // nats below the maximum where weights end
 // made for no less, and half a step of a large `top` can be many times T.
 TB_CUT float lowest_weighted(float top, float T) {
     const double end = (double)top - kNoWeight * (double)T;
+#ifdef __CUDA_ARCH__
+    return __double2float_ru(end);  // the same in one instruction
+#else
     const float cut = (float)end;
     return (double)cut < end ? nextafterf(cut, INFINITY) : cut;
+#endif
 }
 
 }  // namespace tb

@@ -561,10 +561,6 @@ __global__ void __launch_bounds__(kRowThreads) sample_rows_kernel(RowsParams p) 
     }
     if (threadIdx.x < kRoots) sh.root[threadIdx.x] = exp2((double)threadIdx.x / kRoots);
     if (threadIdx.x < 2) sh.listed[threadIdx.x] = 0;
-    if (threadIdx.x == 0) {
-        sh.pick = -1;
-        sh.pick_weight = 0.0;
-    }
     if (P > 1) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
     const float T = p.temperature ? p.temperature[row] : 1.0f;
     const int k = p.top_k ? p.top_k[row] : 0;
@@ -686,6 +682,10 @@ __global__ void __launch_bounds__(kRowThreads) sample_rows_kernel(RowsParams p) 
     // fours of 128 elements, and the first whose sum passes the goal has it
     if (run / kRowWarps != r.rank) return;
     r.turn_to(run % kRowWarps);
+    if (threadIdx.x == 0) {  // a draw that finds none (here: at the start the stores took 0.2 us)
+        sh.pick = -1;
+        sh.pick_weight = 0.0;
+    }
     double running = run_before;
     for (int first = 0; first < r.n; first += 128 * kRowWarps) {
         const int o = first + 128 * r.warp + 4 * r.lane;
