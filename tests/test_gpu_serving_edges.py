@@ -74,6 +74,19 @@ def test_head_groups_that_do_not_divide_a_tile_ragged(serving, G, kv, d):  # noq
     check(serving, attend_case(G, total, new, G * kv, kv, d, evict=[(0, 0)], extra_rows=1))
 
 
+@pytest.mark.parametrize("G", [9, 10, 11, 13, 15, 17, 21, 25, 31, 33, 43, 50, 65, 90, 127, 128])
+@pytest.mark.parametrize("beforehand", [False, True])
+@pytest.mark.parametrize("more", [-1, 1])
+def test_large_head_groups_about_a_tile_end(serving, G, beforehand, more):  # noqa: F811
+    d, kv, per = [16, 32, 64][G % 3], 4, 128 // G
+    n = 41 * per + more
+    total = n + 500
+    need = lambda bound: serving.paged_attention_chunk_workspace(n, 1, n, bound, G * kv, kv, d)  # noqa: E731
+    tiles = -(-total // 128)
+    assert need(total) - need(1) >= 8 * kv * tiles * 128 * d  # its operands: both ways are run
+    check(serving, attend_case(G, [total], [n], G * kv, kv, d, evict=[(0, 2)]), max_len=None if beforehand else 1)
+
+
 @pytest.mark.parametrize("G,kv,d", [(3, 4, 64), (5, 2, 32), (6, 2, 128), (7, 4, 64)])
 @pytest.mark.parametrize("max_new,max_len", [(1, 1), (1, 4096), (2, 500)])
 def test_head_groups_with_more_tokens_than_the_bounds_tell(serving, G, kv, d, max_new, max_len):  # noqa: F811

@@ -51,12 +51,11 @@ namespace {
 //
 // Bound by the softmax warps' instructions (a weight takes an exponential, two
 // conversions and some ten others).  Measured: 2048 tokens over 8192 positions, 32
-// query and 4 KV heads of 64, 305 to 313 us (by card), 0.70 to 0.69 of the three
-// products' time at the measured 1679 TFLOP/s; 8 us for the operands.  Converted by
-// the CTAs that read them, 713 tokens of seven sequences of 664 to 1694, 32 heads of
-// 128: 167 us; 64
-// tokens over 1920, 32 and 4 heads of 64: 23 us, of which 4 pass before the share
-// is known and 2 in reading the queries.
+// query and 4 KV heads of 64, 305 to 314 us (by card), 0.70 of the three products'
+// time at the measured 1679 TFLOP/s; 8 us for the operands.  Converted by the CTAs
+// that read them, 713 tokens of seven sequences of 664 to 1694, 32 heads of 128:
+// 167 us; 64 tokens over 1920, 32 and 4 heads of 64: 23 us, of which 4 pass before
+// the share is known and 2 in reading the queries.
 //
 // With c the row's scale times the page's, a score is c S and a weighted value
 // 2^(c S - M) v = 2^(c S + e - M) (v 2^-e): the page's value exponent e enters
